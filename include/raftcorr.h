@@ -39,6 +39,9 @@
  *   rc_pool2x, rc_interp_bilinear           core/update.py:87-95
  *   rc_upsample_flow_fwd/bwd                core/raft_stereo.py:55-67
  *   rc_sequence_loss_fwd/bwd                train_stereo.py:35-70
+ * and without a counterpart in the reference, in front of the volume (feature maps that attend along the
+ * epipolar row before they are correlated) and for any other caller with sequences of heads:
+ *   rc_qk_norm_rotate_fwd/bwd, rc_cross_attn_fwd/bwd
  */
 #ifndef RAFTCORR_H
 #define RAFTCORR_H
@@ -49,13 +52,14 @@
 extern "C" {
 #endif
 
-#define RC_VERSION 200          /* 0.2.0: forward pyramids keep the even levels only */
+#define RC_VERSION 210          /* 0.2.0: forward pyramids keep the even levels only; 0.2.1: attention operators */
 #define RC_MAX_LEVELS 4
 #define RC_MAX_RADIUS 8
 #define RC_MAX_FUSED_LOOKUPS 32  /* lookups one rc_lookup_bwd_dense call can take */
 #define RC_CONVC1_OUT 64         /* output channels of the motion encoder's convc1 (core/update.py:71) */
 #define RC_CONVC1_MAX_RADIUS 7   /* rc_lookup_convc1_fwd: a level's 2r+1 taps must fit 16 MFMA K slots */
 #define RC_SAMPLER_MAX_RADIUS 7  /* rc_sampler_fwd/bwd: one kernel instantiation per radius (forward: 2r+2 volume entries per lane in registers) */
+#define RC_HEAD_DIM_MAX 256      /* rc_qk_norm_rotate_*, rc_cross_attn_*: elements of one head, a multiple of 8 */
 #define RC_ALT_MAX_RADIUS 6      /* rc_alt_fwd: the union of 16 pixels' tap windows must fit the wave's MFMA tiles */
 
 /* element types of feature maps / volumes */
@@ -442,6 +446,81 @@ int rc_sequence_loss_bwd(const float* const* preds, float* const* grad_preds, co
                          const float* flow_gt, const float* valid, float max_flow,
                          const double* results, const float* grad_loss, int64_t N, int64_t HW,
                          void* stream);
+
+/*
+ * Attention operators.  Operands are sequences of heads, [N, T, H, D] of `dtype` with D the fastest dimension:
+ * element (n, t, h, d) lives at n*stride[0] + t*stride[1] + h*stride[2] + d.  D is a multiple of 8 up to
+ * RC_HEAD_DIM_MAX; base pointers and strides are multiples of 16 bytes (a stride of 0 repeats an operand).  Results
+ * are contiguous.  Sizes of zero are allowed.
+ *
+ * rc_qk_norm_rotate: RMS norm of every head and its rotation by position, queries and keys in one launch:
+ *     r = 1 / sqrt(mean_d x_d^2 + eps),   y_d = x_d r w_d,
+ *     (y_a, y_b) -> (y_a cos A - y_b sin A, y_b cos A + y_a sin A),   A = pos * freqs[i],   i < n_freqs
+ * with (a, b) = (i, n_freqs + i), or (2i, 2i + 1) when `interleaved` is set; elements from 2 n_freqs on are not
+ * rotated.  2 n_freqs is a multiple of 8 and at most D (0: the norm alone).  Angles are reduced to one turn in
+ * double, so far positions lose nothing; everything else is fp32 and rounded once.
+ */
+enum { RC_POS_I32 = 0, RC_POS_I64 = 1, RC_POS_F32 = 2 };
+
+typedef struct rc_heads {
+  const void* x;                    /* [N, T, H, D] */
+  const void* weight;               /* [D] of weight_dtype, or NULL: ones */
+  const void* pos;                  /* [N, T] of pos_dtype, or NULL: 0, 1, ... */
+  int64_t T;
+  int64_t stride[3];                /* elements between sequences, tokens, heads */
+  int64_t pos_stride;               /* elements between the positions of two sequences (0: the same for all) */
+  int32_t H, weight_dtype, pos_dtype, reserved;
+} rc_heads;
+
+/* q, or q and k (k may be NULL: queries alone, the keys of an earlier call are kept).  freqs: n_freqs floats, or
+ * doubles when freqs_f64 is set, in radians per position. */
+int rc_qk_norm_rotate_fwd(const rc_heads* q, const rc_heads* k, void* yq, void* yk, int64_t N, int D,
+                          int dtype, const void* freqs, int freqs_f64, int n_freqs, int interleaved,
+                          float eps, void* stream);
+/* Its adjoint: gq, gk are the contiguous gradients of yq, yk; dq, dk [N, T, H, D] contiguous of `dtype`, dwq, dwk
+ * float [D] (NULL where the gradient is not wanted).  work: rc_qk_norm_rotate_bwd_work_bytes() of scratch (float
+ * partial sums of the weight gradients, added in double in a fixed order: no atomics, reproducible run to run). */
+int64_t rc_qk_norm_rotate_bwd_work_bytes(int D);
+int rc_qk_norm_rotate_bwd(const rc_heads* q, const rc_heads* k, const void* gq, const void* gk, void* dq,
+                          void* dk, float* dwq, float* dwk, void* work, int64_t N, int D, int dtype,
+                          const void* freqs, int freqs_f64, int n_freqs, int interleaved, float eps,
+                          void* stream);
+
+/*
+ * rc_cross_attn: attention of Tq query tokens over the Tk tokens of another sequence,
+ *     S = scale Q K^T,   P = softmax over the allowed keys of S,   O = P V,
+ * Hq query heads in groups of Hq / Hk that share a key and value head (head h reads key head h / (Hq / Hk)).  A key
+ * is allowed if its index is below key_lengths[n] (NULL: all; lengths beyond Tk count as Tk, negative ones as 0) and
+ * its byte of key_mask is not 0 (NULL: all).  What keys and values hold in places that are not allowed has no
+ * influence, infinities and NaN included.  A sequence without an allowed key gives O = 0 and zero gradients.
+ * Scores, softmax statistics and sums are fp32.
+ */
+typedef struct rc_attn {
+  int64_t N, Tq, Tk;
+  int64_t q_stride[3], k_stride[3], v_stride[3]; /* elements between sequences, tokens, heads */
+  int64_t mask_stride;              /* bytes between the mask rows of two sequences (0: the same for all) */
+  const void* key_lengths;          /* [N] int32, or int64 when lengths_i64 is set; NULL */
+  const unsigned char* key_mask;    /* [N, Tk]; NULL */
+  int32_t Hq, Hk, D, dtype;
+  int32_t lengths_i64;
+  float scale;                      /* positive and finite */
+} rc_attn;
+
+/* out [N, Tq, Hq, D]; lse float [N, Hq, Tq]: log-sum-exp of each row's scores in base 2 (scores times log2 e; +inf
+ * for a row without a key), what the backward pass needs; NULL in inference.  work: rc_cross_attn_fwd_work_bytes()
+ * of scratch (0 in most cases: only a few query rows over many keys are split over workgroups); negative: *a is
+ * invalid. */
+int64_t rc_cross_attn_fwd_work_bytes(const rc_attn* a);
+int rc_cross_attn_fwd(const rc_attn* a, const void* q, const void* k, const void* v, void* out, float* lse,
+                      void* work, void* stream);
+/* The adjoint: out and lse of the forward call, dout contiguous like out; dq [N, Tq, Hq, D], dk, dv [N, Tk, Hk, D]
+ * contiguous of `dtype`.  Gradients of a shared head are summed over its group in fp32; no atomics, reproducible run
+ * to run.  dq may be NULL, and dk and dv together, where no gradient is wanted.  work: rc_cross_attn_bwd_work_bytes()
+ * of scratch. */
+int64_t rc_cross_attn_bwd_work_bytes(const rc_attn* a);
+int rc_cross_attn_bwd(const rc_attn* a, const void* q, const void* k, const void* v, const void* out,
+                      const float* lse, const void* dout, void* dq, void* dk, void* dv, void* work,
+                      void* stream);
 
 #ifdef __cplusplus
 }

@@ -13,10 +13,12 @@ RC_CONVC1_OUT = 64
 RC_CONVC1_MAX_RADIUS = 7
 RC_SAMPLER_MAX_RADIUS = 7
 RC_ALT_MAX_RADIUS = 6
+RC_HEAD_DIM_MAX = 256
 RC_F32, RC_F16, RC_BF16 = 0, 1, 2
 RC_COORD_EXACT, RC_COORD_GRIDSAMPLE = 0, 1
+RC_POS_I32, RC_POS_I64, RC_POS_F32 = 0, 1, 2
 RC_WRAP_ROWS = 32
-RC_VERSION = 200
+RC_VERSION = 210
 
 LIB_NAME = "libraftcorr_hip.so"
 # RAFTCORR_LIB: another build of the same library (kernel A/B labs under tools/); it must exist and export everything
@@ -46,8 +48,25 @@ class AltLayout(C.Structure):
                 ("f2_elems", C.c_int64)]
 
 
+class Heads(C.Structure):
+    """rc_heads of include/raftcorr.h."""
+    _fields_ = [("x", C.c_void_p), ("weight", C.c_void_p), ("pos", C.c_void_p),
+                ("T", C.c_int64), ("stride", C.c_int64 * 3), ("pos_stride", C.c_int64),
+                ("H", C.c_int32), ("weight_dtype", C.c_int32), ("pos_dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class Attn(C.Structure):
+    """rc_attn of include/raftcorr.h."""
+    _fields_ = [("N", C.c_int64), ("Tq", C.c_int64), ("Tk", C.c_int64),
+                ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+                ("mask_stride", C.c_int64), ("key_lengths", C.c_void_p), ("key_mask", C.c_void_p),
+                ("Hq", C.c_int32), ("Hk", C.c_int32), ("D", C.c_int32), ("dtype", C.c_int32),
+                ("lengths_i64", C.c_int32), ("scale", C.c_float)]
+
+
 _P, _I, _L = C.c_void_p, C.c_int, C.c_int64
-_LP, _ALP = C.POINTER(Layout), C.POINTER(AltLayout)
+_F = C.c_float
+_LP, _ALP, _HP, _ATP = C.POINTER(Layout), C.POINTER(AltLayout), C.POINTER(Heads), C.POINTER(Attn)
 
 # name -> (restype, argtypes); must list every symbol include/raftcorr.h declares
 SIGNATURES = {
@@ -93,6 +112,13 @@ SIGNATURES = {
     "rc_sequence_loss_fwd": (_I, [C.POINTER(_P), C.POINTER(C.c_float), _I, _L, _P, _P, C.c_float, _P, _P, _L, _L, _P]),
     "rc_sequence_loss_bwd": (_I, [C.POINTER(_P), C.POINTER(_P), C.POINTER(C.c_float), _I, _L, _L, _P, _P,
                                   C.c_float, _P, _P, _L, _L, _P]),
+    "rc_qk_norm_rotate_fwd": (_I, [_HP, _HP, _P, _P, _L, _I, _I, _P, _I, _I, _I, _F, _P]),
+    "rc_qk_norm_rotate_bwd_work_bytes": (_L, [_I]),
+    "rc_qk_norm_rotate_bwd": (_I, [_HP, _HP, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _P, _I, _I, _I, _F, _P]),
+    "rc_cross_attn_fwd_work_bytes": (_L, [_ATP]),
+    "rc_cross_attn_fwd": (_I, [_ATP, _P, _P, _P, _P, _P, _P, _P]),
+    "rc_cross_attn_bwd_work_bytes": (_L, [_ATP]),
+    "rc_cross_attn_bwd": (_I, [_ATP, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
 }
 
 

@@ -1,0 +1,407 @@
+"""Attention along a row, backed by libraftcorr_hip.so: what feature maps go through before they are correlated.
+
+    qk_norm_rotate_hip(q, k, q_weight, k_weight, freqs, ...)   RMS norm and position rotation of query and key heads
+    cross_attention_hip(q, k, v, ...)                          attention over the tokens of another sequence
+    RowAttentionHip(dim, heads)                                both, between the rows of two feature maps
+
+The correlation volume is the score half of an attention between the pixels of two image rows (core/corr.py:148-156 of
+the reference: f1^T f2 / sqrt(D), the rows of one image wider than the other's allowed); these operators add the other
+half.  The reference has no counterpart.  Operands are sequences of heads [N, T, H, D]; the projections around them are
+torch's, like the convolutions of the update block.  There is no CPU or eager fallback: tensors must live on a GPU.
+"""
+import ctypes
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from raft_stereo_amd import _lib
+from raft_stereo_amd._lib import lib, check, Attn, Heads
+from raft_stereo_amd.corr import _DT, _stream, _on_device
+
+_POS = {torch.int32: _lib.RC_POS_I32, torch.int64: _lib.RC_POS_I64, torch.float32: _lib.RC_POS_F32}
+_MAX_STRIDE_BYTES = 1 << 24     # between tokens or heads: a tile's rows are addressed with 32 bits
+
+
+def _check_heads(t, what):
+    if not torch.is_tensor(t) or not t.is_cuda:
+        raise RuntimeError(f"raft_stereo_amd attention kernels need GPU tensors (there is no CPU path): {what}")
+    if t.dtype not in _DT:
+        raise TypeError(f"unsupported dtype {t.dtype} for {what}")
+    if t.dim() != 4:
+        raise ValueError(f"{what} must be [N, T, heads, D], got {tuple(t.shape)}")
+    if t.shape[3] % 8 or not 8 <= t.shape[3] <= _lib.RC_HEAD_DIM_MAX:
+        raise ValueError(f"the head dimension of {what} must be a multiple of 8 in 8..{_lib.RC_HEAD_DIM_MAX}, "
+                         f"got {t.shape[3]}")
+
+
+def _check_same(t, like, what, of):
+    if t.dtype != like.dtype:
+        raise TypeError(f"{what} is {t.dtype}, {of} {like.dtype}")
+    if t.device != like.device:
+        raise RuntimeError(f"{what} and {of} live on different devices")
+
+
+def _heads_view(t):
+    """`t` as (tensor, strides of sequence, token and head) the kernels can address: dense heads, everything on 16-byte
+    boundaries (slices of a wider projection qualify, and expanded dimensions).  Anything else is copied."""
+    es = t.element_size()
+    st = [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s * es % 16 for s in st) or max(st[1:]) * es >= _MAX_STRIDE_BYTES:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = list(t.stride()[:3])
+        if max(s if n > 1 else 0 for n, s in zip(t.shape[1:3], st[1:])) * es >= _MAX_STRIDE_BYTES:
+            raise ValueError(f"heads of {tuple(t.shape)} are too wide: a token has to stay under 16 MiB")
+    return t, st
+
+
+def _dense(t):
+    """`t` contiguous and on a 16-byte boundary."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+# --------------------------------------------------------------------------------------------- norm and rotation
+def _check_weight(w, x, what):
+    if w is None:
+        return
+    if w.dim() != 1 or w.shape[0] != x.shape[3]:
+        raise ValueError(f"{what} must be [{x.shape[3]}], got {tuple(w.shape)}")
+    if w.dtype not in _DT:
+        raise TypeError(f"unsupported dtype {w.dtype} for {what}")
+    if w.device != x.device:
+        raise RuntimeError(f"{what} lives on a different device than the heads")
+
+
+def _check_pos(pos, x, what):
+    """Positions as (tensor, elements between two sequences)."""
+    if pos is None:
+        return None, 0
+    if pos.dtype not in _POS:
+        raise TypeError(f"{what} must be int32, int64 or float32, got {pos.dtype}")
+    if pos.device != x.device:
+        raise RuntimeError(f"{what} lives on a different device than the heads")
+    N, T = x.shape[:2]
+    if tuple(pos.shape) not in ((T,), (N, T)):
+        raise ValueError(f"{what} must be [{T}] or [{N}, {T}], got {tuple(pos.shape)}")
+    if T > 1 and pos.stride(-1) != 1:
+        pos = pos.contiguous()
+    return pos, (pos.stride(0) if pos.dim() == 2 and N > 1 else 0)
+
+
+def _heads_desc(x, st, weight, pos, pos_stride):
+    d = Heads()
+    d.x = x.data_ptr()
+    d.T, d.H = x.shape[1], x.shape[2]
+    d.stride[0], d.stride[1], d.stride[2] = st
+    if weight is not None:
+        d.weight, d.weight_dtype = weight.data_ptr(), _DT[weight.dtype]
+    if pos is not None:
+        d.pos, d.pos_dtype, d.pos_stride = pos.data_ptr(), _POS[pos.dtype], pos_stride
+    return d
+
+
+class _Sides:
+    """The checked operands of one norm + rotation call, as the library takes them."""
+    __slots__ = ("q", "k", "q_st", "k_st", "qw", "kw", "q_pos", "k_pos", "q_ps", "k_ps", "freqs", "eps", "interleaved")
+
+    def describe(self):
+        dq = _heads_desc(self.q, self.q_st, self.qw, self.q_pos, self.q_ps)
+        dk = None if self.k is None else _heads_desc(self.k, self.k_st, self.kw, self.k_pos, self.k_ps)
+        fr = self.freqs
+        tail = (_DT[self.q.dtype], None if fr is None else fr.data_ptr(), int(fr is not None and fr.dtype is torch.float64),
+                0 if fr is None else fr.shape[0], int(self.interleaved), self.eps)
+        return dq, dk, tail
+
+
+def _norm_rotate_raw(s):
+    dev = s.q.device
+    dq, dk, tail = s.describe()
+    with _on_device(dev):
+        yq = torch.empty(s.q.shape, dtype=s.q.dtype, device=dev)
+        yk = None if s.k is None else torch.empty(s.k.shape, dtype=s.k.dtype, device=dev)
+        rc = lib.rc_qk_norm_rotate_fwd(dq, dk, yq.data_ptr(), None if yk is None else yk.data_ptr(), s.q.shape[0],
+                                       s.q.shape[3], *tail, _stream(dev))
+        if rc:
+            check(rc, "rc_qk_norm_rotate_fwd")
+    return yq, yk
+
+
+class _NormRotateFn(torch.autograd.Function):
+    """Keeps its inputs for the backward pass, which works the norm out again."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, s):
+        s.q, s.k, s.qw, s.kw = q, k, q_weight, k_weight
+        yq, yk = _norm_rotate_raw(s)
+        ctx.save_for_backward(q, k, q_weight, k_weight, s.freqs, s.q_pos, s.k_pos)
+        ctx.rest = (s.q_st, s.k_st, s.q_ps, s.k_ps, s.eps, s.interleaved)
+        s.q = s.k = s.qw = s.kw = s.freqs = s.q_pos = s.k_pos = None
+        ctx.set_materialize_grads(False)
+        return yq, yk
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        s = _Sides()
+        s.q, s.k, s.qw, s.kw, s.freqs, s.q_pos, s.k_pos = ctx.saved_tensors
+        s.q_st, s.k_st, s.q_ps, s.k_ps, s.eps, s.interleaved = ctx.rest
+        if gq is None and gk is None:
+            return None, None, None, None, None
+        dev, D = s.q.device, s.q.shape[3]
+        want = ctx.needs_input_grad
+        gq = torch.zeros(s.q.shape, dtype=s.q.dtype, device=dev) if gq is None else _dense(gq)
+        if s.k is not None:
+            gk = torch.zeros(s.k.shape, dtype=s.k.dtype, device=dev) if gk is None else _dense(gk)
+        dq_desc, dk_desc, tail = s.describe()
+        with _on_device(dev):
+            dq = torch.empty(s.q.shape, dtype=s.q.dtype, device=dev)
+            dk = None if s.k is None else torch.empty(s.k.shape, dtype=s.k.dtype, device=dev)
+            dwq = torch.empty(D, dtype=torch.float32, device=dev) if s.qw is not None and want[2] else None
+            dwk = torch.empty(D, dtype=torch.float32, device=dev) if s.kw is not None and want[3] else None
+            work = None
+            if dwq is not None or dwk is not None:
+                work = torch.empty(int(lib.rc_qk_norm_rotate_bwd_work_bytes(D)), dtype=torch.uint8, device=dev)
+            ptr = lambda t: None if t is None else t.data_ptr()
+            check(lib.rc_qk_norm_rotate_bwd(dq_desc, dk_desc, gq.data_ptr(), ptr(gk), dq.data_ptr(), ptr(dk), ptr(dwq),
+                                            ptr(dwk), ptr(work), s.q.shape[0], D, *tail, _stream(dev)),
+                  "rc_qk_norm_rotate_bwd")
+        cast = lambda d, w: None if d is None else d.to(w.dtype)
+        return dq, dk, cast(dwq, s.qw), cast(dwk, s.kw), None
+
+
+def qk_norm_rotate_hip(q, k=None, q_weight=None, k_weight=None, freqs=None, q_pos=None, k_pos=None, eps=1e-6,
+                       interleaved=False):
+    """RMS norm of every query and key head and its rotation by position, in one pass.
+
+    q `[N, Tq, Hq, D]` and k `[N, Tk, Hk, D]` (its own length and number of heads; None: queries alone, where the keys
+    were made by an earlier call).  `y = x / sqrt(mean(x^2) + eps) * weight` over D, weights `[D]` (None: ones); then
+    pair i is turned by the angle `pos * freqs[i]`: elements `(i, i + n)`, or `(2i, 2i + 1)` if `interleaved`, of the
+    first `2 n` for the n frequencies in `freqs` (float32 or float64, radians per position; None: the norm alone).
+    Positions are `[T]` or `[N, T]`, int32, int64 or float32 (None: 0, 1, ...); angles are reduced to one turn in
+    64 bits, so positions far along lose nothing.  Everything else is fp32 and rounded once.  n must be a multiple of 4.
+    Returns `(q', k')`, contiguous, or `q'` alone if k is None.  Differentiable w.r.t. q, k and the weights."""
+    _check_heads(q, "q")
+    _check_weight(q_weight, q, "q_weight")
+    if k is not None:
+        _check_heads(k, "k")
+        _check_same(k, q, "k", "q")
+        if k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+            raise ValueError(f"q and k must agree in sequences and head dimension: {tuple(q.shape)} vs {tuple(k.shape)}")
+        _check_weight(k_weight, k, "k_weight")
+    elif k_weight is not None or k_pos is not None:
+        raise ValueError("k_weight and k_pos need k")
+    if freqs is not None:
+        if freqs.dim() != 1 or freqs.shape[0] % 4 or 2 * freqs.shape[0] > q.shape[3]:
+            raise ValueError(f"freqs must be [n] with n a multiple of 4 and at most {q.shape[3] // 2}, "
+                             f"got {tuple(freqs.shape)}")
+        if freqs.dtype not in (torch.float32, torch.float64):
+            raise TypeError(f"freqs must be float32 or float64, got {freqs.dtype}")
+        if freqs.device != q.device:
+            raise RuntimeError("freqs lives on a different device than the heads")
+        freqs = freqs.detach().contiguous() if freqs.shape[0] else None
+    elif q_pos is not None or k_pos is not None:
+        raise ValueError("positions need freqs")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    s = _Sides()
+    s.freqs, s.eps, s.interleaved = freqs, float(eps), bool(interleaved)
+    s.q_pos, s.q_ps = _check_pos(q_pos, q, "q_pos")
+    s.k_pos, s.k_ps = (None, 0) if k is None else _check_pos(k_pos, k, "k_pos")
+    # views are taken here, so that autograd carries the gradient of a copy back through torch's own clone
+    q, s.q_st = _heads_view(q)
+    k, s.k_st = (None, None) if k is None else _heads_view(k)
+    q_weight = None if q_weight is None else q_weight.contiguous()
+    k_weight = None if k_weight is None else k_weight.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        yq, yk = _NormRotateFn.apply(q, k, q_weight, k_weight, s)
+    else:
+        s.q, s.k, s.qw, s.kw = q, k, q_weight, k_weight
+        yq, yk = _norm_rotate_raw(s)
+    return yq if k is None else (yq, yk)
+
+
+# ------------------------------------------------------------------------------------------------ cross attention
+def _attn_desc(q, k, v, strides, key_mask, key_lengths, scale):
+    a = Attn()
+    N, a.Tq, a.Hq, a.D = q.shape
+    a.N, a.Tk, a.Hk = N, k.shape[1], k.shape[2]
+    a.dtype, a.scale = _DT[q.dtype], scale
+    for dst, st in zip((a.q_stride, a.k_stride, a.v_stride), strides):
+        dst[0], dst[1], dst[2] = st
+    if key_mask is not None:
+        a.key_mask, a.mask_stride = key_mask.data_ptr(), key_mask.stride(0) if N > 1 else 0
+    if key_lengths is not None:
+        a.key_lengths, a.lengths_i64 = key_lengths.data_ptr(), int(key_lengths.dtype is torch.int64)
+    return a
+
+
+def _work(nbytes, what, dev):
+    if nbytes < 0:
+        check(int(nbytes), what)
+    return torch.empty(int(nbytes), dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def _attention_raw(q, k, v, strides, key_mask, key_lengths, scale, want_lse):
+    dev = q.device
+    N, Tq, Hq, _ = q.shape
+    a = _attn_desc(q, k, v, strides, key_mask, key_lengths, scale)
+    with _on_device(dev):
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        lse = torch.empty((N, Hq, Tq), dtype=torch.float32, device=dev) if want_lse else None
+        work = _work(lib.rc_cross_attn_fwd_work_bytes(a), "rc_cross_attn_fwd_work_bytes", dev)
+        rc = lib.rc_cross_attn_fwd(a, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                   None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(),
+                                   _stream(dev))
+        if rc:
+            check(rc, "rc_cross_attn_fwd")
+    return out, lse
+
+
+class _CrossAttentionFn(torch.autograd.Function):
+    """Keeps the operands, the result and each row's log-sum-exp; the backward pass works the scores out again."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, strides, key_mask, key_lengths, scale):
+        out, lse = _attention_raw(q, k, v, strides, key_mask, key_lengths, scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, key_mask, key_lengths)
+        ctx.strides, ctx.scale = strides, scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        q, k, v, out, lse, key_mask, key_lengths = ctx.saved_tensors
+        dev = q.device
+        g = _dense(grad_out)
+        a = _attn_desc(q, k, v, ctx.strides, key_mask, key_lengths, ctx.scale)
+        want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        with _on_device(dev):
+            dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if want_q else None
+            dk = torch.empty(k.shape, dtype=k.dtype, device=dev) if want_kv else None
+            dv = torch.empty(v.shape, dtype=v.dtype, device=dev) if want_kv else None
+            work = _work(lib.rc_cross_attn_bwd_work_bytes(a), "rc_cross_attn_bwd_work_bytes", dev)
+            ptr = lambda t: None if t is None else t.data_ptr()
+            check(lib.rc_cross_attn_bwd(a, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                                        g.data_ptr(), ptr(dq), ptr(dk), ptr(dv), ptr(work), _stream(dev)),
+                  "rc_cross_attn_bwd")
+        return dq, dk, dv, None, None, None, None
+
+
+def cross_attention_hip(q, k, v, key_mask=None, key_lengths=None, scale=None):
+    """Attention of query tokens over the tokens of another sequence: `softmax(scale q k^T) v` for each head.
+
+    q `[N, Tq, Hq, D]`, k and v `[N, Tk, Hk, D]`, Hq a multiple of Hk (the Hq / Hk query heads in a row share a key and
+    value head), any lengths from 0 on; scale defaults to `1 / sqrt(D)`.  A key takes part if its index is below
+    `key_lengths[n]` (int32 or int64 `[N]`; beyond Tk counts as Tk, negative as 0) and `key_mask[n, t]` is True (bool
+    `[N, Tk]`); what the others hold, infinities and NaN included, has no influence.  A sequence without any key gives
+    zeros, and zero gradients.  Scores, the softmax's maximum and sum, and all products' sums are fp32; 16-bit operands
+    have their probabilities (and in the backward pass their scores' gradients) rounded to 16 bits for the second
+    product.  Returns `[N, Tq, Hq, D]` contiguous.  Differentiable w.r.t. q, k and v, the same bits on every run."""
+    for t, what in ((q, "q"), (k, "k"), (v, "v")):
+        _check_heads(t, what)
+    for t, what in ((k, "k"), (v, "v")):
+        _check_same(t, q, what, "q")
+    N, Tq, Hq, D = q.shape
+    if k.shape != v.shape or k.shape[0] != N or k.shape[3] != D:
+        raise ValueError(f"k and v must be [{N}, Tk, heads, {D}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    Tk, Hk = k.shape[1], k.shape[2]
+    if Hk < 1 or Hq < 1 or Hq % Hk:
+        raise ValueError(f"{Hq} query heads are no multiple of {Hk} key heads")
+    if key_mask is not None:
+        if key_mask.dtype is not torch.bool:
+            raise TypeError(f"key_mask must be bool (True: the key takes part), got {key_mask.dtype}")
+        if tuple(key_mask.shape) != (N, Tk):
+            raise ValueError(f"key_mask must be [{N}, {Tk}], got {tuple(key_mask.shape)}")
+        if key_mask.device != q.device:
+            raise RuntimeError("key_mask lives on a different device than q")
+        if Tk > 1 and key_mask.stride(1) != 1:
+            key_mask = key_mask.contiguous()
+    if key_lengths is not None:
+        if key_lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"key_lengths must be int32 or int64, got {key_lengths.dtype}")
+        if tuple(key_lengths.shape) != (N,):
+            raise ValueError(f"key_lengths must be [{N}], got {tuple(key_lengths.shape)}")
+        if key_lengths.device != q.device:
+            raise RuntimeError("key_lengths lives on a different device than q")
+        key_lengths = key_lengths.contiguous()
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    # views are taken here, so that autograd carries the gradient of a copy back through torch's own clone
+    (q, qs), (k, ks), (v, vs) = _heads_view(q), _heads_view(k), _heads_view(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _CrossAttentionFn.apply(q, k, v, (qs, ks, vs), key_mask, key_lengths, scale)
+    return _attention_raw(q, k, v, (qs, ks, vs), key_mask, key_lengths, scale, False)[0]
+
+
+# ------------------------------------------------------------------------------------------- rows of feature maps
+class RowAttentionHip(nn.Module):
+    """Lets two feature maps attend to each other along their rows before they are correlated.
+
+    `forward(fmap1, fmap2, width1=None, width2=None)` takes `[B, dim, H, W1]` and `[B, dim, H, W2]` and returns both
+    maps with the attention's result added: every pixel of a row looks at all pixels of the same row of the other map
+    (rectified stereo: its match lies there, which is also why the correlation is one-dimensional, core/corr.py:148-156).
+    Queries and keys are normalised per head and rotated by their column.  `width1` / `width2` (int32 or int64 `[B]`):
+    columns of each image that hold data; the padding behind them is not attended to.  Handed to
+    `make_corr_fn(..., attention=module)`, it runs in front of the volume."""
+
+    def __init__(self, dim, heads=4, kv_heads=None, head_dim=None, base=10000.0, eps=1e-6):
+        super().__init__()
+        kv_heads = heads if kv_heads is None else kv_heads
+        if heads < 1 or kv_heads < 1 or heads % kv_heads:
+            raise ValueError(f"{heads} query heads are no multiple of {kv_heads} key heads")
+        head_dim = dim // heads if head_dim is None else head_dim
+        if head_dim % 8 or not 8 <= head_dim <= _lib.RC_HEAD_DIM_MAX:
+            raise ValueError(f"head_dim must be a multiple of 8 in 8..{_lib.RC_HEAD_DIM_MAX}, got {head_dim}")
+        self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
+        self.base, self.eps = base, eps
+        self.q = nn.Linear(dim, heads * head_dim, bias=False)
+        self.k = nn.Linear(dim, kv_heads * head_dim, bias=False)
+        self.v = nn.Linear(dim, kv_heads * head_dim, bias=False)
+        self.out = nn.Linear(heads * head_dim, dim)
+        self.q_weight = nn.Parameter(torch.ones(head_dim))
+        self.k_weight = nn.Parameter(torch.ones(head_dim))
+        self.register_buffer("freqs", self._make_freqs("cpu"), persistent=False)
+
+    def _make_freqs(self, device):
+        n = self.head_dim // 8 * 4
+        return (self.base ** (-torch.arange(n, dtype=torch.float64) / n)).to(device)   # the same bits on any device
+
+    def _apply(self, *args, **kwargs):
+        """`.half()` and the like move the frequencies, but do not round them."""
+        super()._apply(*args, **kwargs)
+        if self.freqs.dtype is not torch.float64:
+            self.freqs = self._make_freqs(self.freqs.device)
+        return self
+
+    def _project(self, rows, layer, heads):
+        y = F.linear(rows, layer.weight.to(rows.dtype))
+        return y.view(*y.shape[:2], heads, self.head_dim)
+
+    def _onto(self, fmap, rows, q, k, v, lengths):
+        a = cross_attention_hip(q, k, v, key_lengths=lengths)
+        y = F.linear(a.flatten(2), self.out.weight.to(a.dtype), self.out.bias.to(a.dtype))
+        B, C, H, W = fmap.shape
+        return (rows + y).view(B, H, W, C).permute(0, 3, 1, 2).contiguous()
+
+    def forward(self, fmap1, fmap2, width1=None, width2=None):
+        if fmap1.dim() != 4 or fmap2.dim() != 4 or fmap1.shape[:3] != fmap2.shape[:3]:
+            raise ValueError(f"fmap shapes disagree: {tuple(fmap1.shape)} vs {tuple(fmap2.shape)}")
+        if fmap1.dtype != fmap2.dtype:
+            raise TypeError(f"unsupported feature dtypes {fmap1.dtype}/{fmap2.dtype}")
+        H = fmap1.shape[2]
+        rows, heads, lengths = [], [], []
+        for fmap, width in ((fmap1, width1), (fmap2, width2)):
+            x = fmap.permute(0, 2, 3, 1).flatten(0, 1).contiguous()                       # [B*H, W, dim]
+            rows.append(x)
+            q, k = qk_norm_rotate_hip(self._project(x, self.q, self.heads), self._project(x, self.k, self.kv_heads),
+                                      self.q_weight, self.k_weight, self.freqs, eps=self.eps)
+            heads.append((q, k, self._project(x, self.v, self.kv_heads)))
+            if width is not None and tuple(width.shape) != (fmap.shape[0],):
+                raise ValueError(f"widths must be [{fmap.shape[0]}], got {tuple(width.shape)}")
+            lengths.append(None if width is None else width.repeat_interleave(H))
+        (q1, k1, v1), (q2, k2, v2) = heads
+        return (self._onto(fmap1, rows[0], q1, k2, v2, lengths[1]),
+                self._onto(fmap2, rows[1], q2, k1, v1, lengths[0]))
