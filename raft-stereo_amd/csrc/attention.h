@@ -1,0 +1,342 @@
+// What the attention kernels share: arguments, the matrix-instruction fragments, and the staging of tiles of rows.
+//
+// A tile is a number of rows (tokens of one head) in LDS, RB bytes each (the head padded with zeros to a power of
+// two), cut into 16-byte chunks.  Chunk c of row r lies at r * RB + ((c ^ f(r)) << 4).  f is chosen so that both ways
+// of reading a tile are free of bank conflicts: eight lanes that read the same chunk of eight consecutive rows (a
+// fragment whose reduction runs along the row) and sixteen lanes that read 32 bytes each of four consecutive rows (the
+// transposing read, a fragment whose reduction runs across rows).
+//
+// The 32x32 matrix instructions give lane l = 32 h + c the column c and, in register i, the row 8 (i / 4) + 4 h + i % 4
+// of the result.  As the order of the reduction index is free as long as both operands agree, a result (probabilities,
+// keys by queries) is the right operand of the next product as it stands: slot (h, j) of the 16 keys from 16 b is key
+// 16 b + 8 (j / 4) + 4 h + j % 4, and the left operand's rows are read in that order.
+#pragma once
+#include "rc_common.h"
+
+#include <math.h>
+
+typedef short at_s4 __attribute__((ext_vector_type(4)));
+typedef short at_s8 __attribute__((ext_vector_type(8)));
+typedef float at_f16 __attribute__((ext_vector_type(16)));
+typedef float at_f4 __attribute__((ext_vector_type(4)));
+typedef float at_f2 __attribute__((ext_vector_type(2)));
+typedef uint32_t at_u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t at_u2 __attribute__((ext_vector_type(2)));
+typedef _Float16 at_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 at_h2 __attribute__((ext_vector_type(2)));
+typedef __bf16 at_b8 __attribute__((ext_vector_type(8)));
+typedef __bf16 at_b2 __attribute__((ext_vector_type(2)));
+
+struct at_args {
+  int64_t qs[3], ks[3], vs[3];  // elements between sequences, tokens, heads
+  const void* lengths;
+  const uint64_t* bits;  // [N][words], bit t % 64 of word t / 64: key t takes part; NULL: the lengths say it
+  int64_t words;
+  int32_t N, Tq, Tk, Hq, Hk, G, D;
+  int32_t lengths_i64;
+  float scale, scale_log2;
+};
+
+// host side (attention_fwd.hip)
+int at_check(const rc_attn* a);
+int at_check_operand(const rc_attn* a, int64_t rows, const void* p);
+at_args at_to_dev(const rc_attn* a, void* bits);
+int64_t at_bits_bytes(const rc_attn* a);  // scratch of the mask's bits, a multiple of 256
+int at_launch_bits(const rc_attn* a, void* bits, hipStream_t st);
+
+__device__ __forceinline__ int at_length(const at_args& a, int n) {
+  if (a.lengths == nullptr) return a.Tk;
+  int64_t l = a.lengths_i64 ? reinterpret_cast<const int64_t*>(a.lengths)[n]
+                            : (int64_t) reinterpret_cast<const int32_t*>(a.lengths)[n];
+  l = l < 0 ? 0 : l;
+  return __builtin_amdgcn_readfirstlane((int)(l > a.Tk ? a.Tk : l));
+}
+
+// the keys k0 .. k0 + 31 (k0 a multiple of 32) that take part, one bit each
+__device__ __forceinline__ uint32_t at_key_bits(const at_args& a, int n, int len, int k0) {
+  const int left = len - k0;
+  uint32_t w = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+  if (a.bits != nullptr && left > 0)
+    w &= reinterpret_cast<const uint32_t*>(a.bits)[((int64_t)n * a.words) * 2 + (k0 >> 5)];
+  return __builtin_amdgcn_readfirstlane(w);
+}
+
+// ------------------------------------------------------------------------------------------------ matrix fragments
+// One step of a product: 16 bytes per lane of each operand, elements along the reduction.
+__device__ __forceinline__ at_f16 at_mma(rc_half, at_u4 a, at_u4 b, at_f16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(at_h8, a), __builtin_bit_cast(at_h8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ at_f16 at_mma(rc_bf16, at_u4 a, at_u4 b, at_f16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(at_b8, a), __builtin_bit_cast(at_b8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ at_f16 at_mma(float, at_u4 a, at_u4 b, at_f16 c) {
+  // (whole vectors are cast: __builtin_bit_cast of one element takes the first)
+  const at_f4 x = __builtin_bit_cast(at_f4, a), y = __builtin_bit_cast(at_f4, b);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
+  return c;
+}
+
+__device__ __forceinline__ uint32_t at_pack(rc_half, float x, float y) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((at_f2){x, y}, at_h2));
+}
+__device__ __forceinline__ uint32_t at_pack(rc_bf16, float x, float y) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((at_f2){x, y}, at_b2));
+}
+
+// The halves of the wave exchange: afterwards a holds the lower halves of both, b the upper ones.
+__device__ __forceinline__ void at_swap(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+// both halves see their two values
+__device__ __forceinline__ void at_both(float x, float& lo, float& hi) {
+  uint32_t a = __builtin_bit_cast(uint32_t, x), b = a;
+  at_swap(a, b);
+  lo = __builtin_bit_cast(float, a);
+  hi = __builtin_bit_cast(float, b);
+}
+__device__ __forceinline__ float at_half_max(float x) {
+  float lo, hi;
+  at_both(x, lo, hi);
+  return fmaxf(lo, hi);
+}
+__device__ __forceinline__ float at_half_sum(float x) {
+  float lo, hi;
+  at_both(x, lo, hi);
+  return lo + hi;
+}
+
+// ------------------------------------------------------------------------------------------------- rows in LDS
+template <typename T, int DC> struct at_row {
+  static constexpr int ES = sizeof(T);
+  static constexpr int DS = DC <= 32 ? 32 : DC <= 64 ? 64 : DC <= 128 ? 128 : 256;
+  static constexpr int RB = DS * ES;    // bytes of a row
+  static constexpr int CH = RB / 16;    // chunks of a row
+  static constexpr int STEPS = DC * ES / 32;  // of a product along the row (two chunks each)
+};
+
+template <int CH> __device__ __forceinline__ int at_swizzle(int row) {
+  return CH >= 8 ? ((row & 3) << 1) | ((row >> 2) & 1) : (row & 2) | ((row >> 2) & 1);
+}
+template <typename T, int DC> __device__ __forceinline__ uint32_t at_chunk(int row, int chunk) {
+  using R = at_row<T, DC>;
+  return (uint32_t)(row * R::RB + ((chunk ^ at_swizzle<R::CH>(row)) << 4));
+}
+
+typedef unsigned char __attribute__((address_space(3))) * at_lds;
+
+// A lane's places in a tile.  The swizzle touches the lowest three bits of a chunk's number and goes by the lowest three
+// of the row's, so a few offsets, worked out once, reach everything with constant distances.
+template <typename T, int DC> struct at_places {
+  using R = at_row<T, DC>;
+  static constexpr int NA = R::CH >= 8 ? 4 : 2;
+  static constexpr int NX = sizeof(T) == 4 ? 4 : R::CH >= 8 ? 2 : 1;
+  uint32_t along[NA];   // row c, chunk 2 i + h
+  uint32_t across[NX];  // 16-bit: the transposing read's row and chunk, columns 32 i ..; fp32: row 4 h + i, column c
+
+  __device__ __forceinline__ void init(int lane) {
+    const int c = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) along[i] = at_chunk<T, DC>(c, 2 * i + h);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < NX; ++i) across[i] = at_chunk<T, DC>(4 * h + i, c >> 2) + (c & 3) * 4;
+    } else {
+      const int i = lane & 15, g = lane >> 4;
+#pragma unroll
+      for (int x = 0; x < NX; ++x)
+        across[x] = at_chunk<T, DC>(4 * (g >> 1) + (i >> 2), 4 * x + 2 * (g & 1) + ((i >> 1) & 1)) + (i & 1) * 8;
+    }
+  }
+  // left operand of step st of a product along the rows: rows row .. row + 31 (a multiple of 32)
+  __device__ __forceinline__ at_u4 rows(const unsigned char* tile, int row, int st) const {
+    return *reinterpret_cast<const at_u4*>(tile + along[st % NA] + (row * R::RB + st / NA * (NA * 32)));
+  }
+  // left operand of a product across the rows (16-bit types): the 16 rows from `row` (a multiple of 16), in the order of
+  // a result's registers, columns 32 db .. 32 db + 31
+  __device__ __forceinline__ at_u4 cols(const unsigned char* tile, int row, int db) const {
+    typedef at_s4 __attribute__((address_space(3))) * lds_s4p;
+    const unsigned char* p = tile + across[db % NX] + (row * R::RB + db / NX * (NX * 64));
+    const at_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4p)p);
+    const at_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4p)(p + 8 * R::RB));
+    return __builtin_bit_cast(at_u4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  // the same in fp32: row 8 (i / 4) + 4 h + i % 4 behind `row`
+  __device__ __forceinline__ float col(const unsigned char* tile, int row, int i, int db) const {
+    return *reinterpret_cast<const float*>(tile + across[i % 4] + ((row + 8 * (i / 4)) * R::RB + db * 128));
+  }
+};
+
+// acc[db] += (32 rows of the tile from `row`)^T x, for all columns of the head: x is a result of 32 rows by 32 columns
+// (16-bit types: rounded to T).
+template <typename T, int DC>
+__device__ __forceinline__ void at_mma_cols(const at_places<T, DC>& at, const unsigned char* tile, int row, const at_f16& x,
+                                            at_f16* acc) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      at_u4 p;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[j] = at_pack(T(), x[8 * b + 2 * j], x[8 * b + 2 * j + 1]);
+#pragma unroll
+      for (int db = 0; db < DC / 32; ++db) acc[db] = at_mma(T(), at.cols(tile, row + 16 * b, db), p, acc[db]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int db = 0; db < DC / 32; ++db)
+        acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(at.col(tile, row, i, db), x[i], acc[db], 0, 0, 0);
+  }
+}
+
+// Tiles are filled by loads that go straight to LDS: one instruction moves 1 KiB, lane l's 16 bytes land at 16 l, so
+// the swizzle is applied to the addresses that the lanes fetch from.  Chunks behind the head's end and rows that do
+// not take part are fetched from beyond the buffer's range, which gives zeros (so whatever those rows hold, NaN
+// included, never meets a product).
+constexpr uint32_t AT_RANGE = 0x80010000u, AT_OUTSIDE = 0xc0000000u;
+
+template <typename T, int DC, int ROWS, int WAVES> struct at_stage {
+  using R = at_row<T, DC>;
+  static constexpr int PER = 1024 / R::RB;                  // rows per instruction
+  static constexpr int N = ROWS * R::RB / 1024 / WAVES;     // instructions per wave, STEP rows apart
+  static constexpr int STEP = PER * WAVES;
+  static constexpr int PD = STEP >= 8 ? 1 : 8 / STEP;       // instructions after which the swizzle repeats
+  static_assert(R::RB <= 1024 && ROWS * R::RB % (1024 * WAVES) == 0 && N % PD == 0, "whole instructions for every wave");
+  uint32_t off[PD];
+  int64_t ahead;  // bytes from one group of PD instructions to the next
+
+  // D: elements of a head; stride: bytes between rows
+  __device__ __forceinline__ void init(int wave, int lane, int D, uint32_t stride) {
+    ahead = (int64_t)PD * STEP * stride;
+#pragma unroll
+    for (int p = 0; p < PD; ++p) {
+      const int r = p * STEP + wave * PER + lane / R::CH, chunk = (lane % R::CH) ^ at_swizzle<R::CH>(r);
+      off[p] = chunk * 16 < D * R::ES ? (uint32_t)r * stride + (uint32_t)chunk * 16u : AT_OUTSIDE;
+    }
+  }
+  // base: the tile's first row; take[p]: the rows of the 32 that instruction p's rows lie in that take part, a bit each
+  __device__ __forceinline__ void issue(const char* base, uint32_t lds, int wave, int lane, bool full, const uint32_t (&take)[N]) const {
+#pragma unroll
+    for (int p = 0; p < N; ++p) {
+      const uint64_t b = (uint64_t)(base + (p / PD) * ahead);
+      typedef int i4 __attribute__((ext_vector_type(4)));
+      const i4 rs = {__builtin_amdgcn_readfirstlane((int)b), __builtin_amdgcn_readfirstlane((int)(b >> 32) & 0xffff),
+                     (int)AT_RANGE, 0x00020000};
+      uint32_t o = off[p % PD];
+      if (!full) o = (take[p] >> ((p * STEP + wave * PER + lane / R::CH) & 31)) & 1 ? o : AT_OUTSIDE;
+      const uint32_t dst = lds + (uint32_t)(p * WAVES + wave) * 1024u;
+      unsigned keep;
+      asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+                   : "=&s"(keep)
+                   : "v"(o), "s"(rs), "s"(__builtin_amdgcn_readfirstlane(dst))
+                   : "memory");
+    }
+  }
+};
+
+// The key and value tiles of a work item, in the order that it goes through them.
+template <typename T, int DC, int KT, int WAVES> struct at_key_tiles {
+  using S = at_stage<T, DC, KT, WAVES>;
+  S k, v;
+  const char *kp, *vp;
+  int64_t kstep, vstep;
+  int n, k0, k_end;  // sequence, first key of the tile that is fetched next, end of the item's keys
+
+  __device__ __forceinline__ void init(const at_args& a, const T* kb, const T* vb, int seq, int hk, int begin, int end,
+                                       int wave, int lane) {
+    n = seq;
+    k0 = begin;
+    k_end = end;
+    kp = reinterpret_cast<const char*>(kb + (int64_t)n * a.ks[0] + (int64_t)hk * a.ks[2] + (int64_t)begin * a.ks[1]);
+    vp = reinterpret_cast<const char*>(vb + (int64_t)n * a.vs[0] + (int64_t)hk * a.vs[2] + (int64_t)begin * a.vs[1]);
+    kstep = a.ks[1] * (int64_t)(sizeof(T) * KT);
+    vstep = a.vs[1] * (int64_t)(sizeof(T) * KT);
+    k.init(wave, lane, a.D, (uint32_t)(a.ks[1] * sizeof(T)));
+    v.init(wave, lane, a.D, (uint32_t)(a.vs[1] * sizeof(T)));
+  }
+  __device__ __forceinline__ void fetch(const at_args& a, uint32_t lds_k, uint32_t lds_v, int wave, int lane) {
+    uint32_t take[S::N];
+    const bool full = a.bits == nullptr && k_end - k0 >= KT;
+#pragma unroll
+    for (int p = 0; p < S::N; ++p)
+      take[p] = full ? 0xffffffffu : at_key_bits(a, n, k_end, k0 + ((p * S::STEP + wave * S::PER) & ~31));
+    k.issue(kp, lds_k, wave, lane, full, take);
+    v.issue(vp, lds_v, wave, lane, full, take);
+    kp += kstep;
+    vp += vstep;
+    k0 += KT;
+  }
+};
+
+// every load of this wave has landed, and every wave has said so
+__device__ __forceinline__ void at_landed() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void at_sync() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Block id -> work item: ids go round the 8 XCDs, items that share keys should share an XCD's L2, so each XCD gets a
+// run of consecutive items.  The grid has at_grid() blocks.
+__device__ __forceinline__ int64_t at_item(int64_t items) {
+  const int64_t per = (items + 7) / 8;
+  const int64_t i = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  return (blockIdx.x >> 3) < per && i < items ? i : -1;
+}
+static inline uint32_t at_grid(int64_t items) { return (uint32_t)((items + 7) / 8 * 8); }
+
+// four consecutive elements of a row
+__device__ __forceinline__ void at_store4(float* p, at_f4 v) { *reinterpret_cast<at_f4*>(p) = v; }
+
+// Writes a result (rows: elements 32 db .. of the head, column: this lane's row of memory at p) times f.
+template <typename T, int DC>
+__device__ __forceinline__ void at_store_rows(T* p, bool live, const at_f16* acc, float f, int D, int lane) {
+  const int h = lane >> 5;
+#pragma unroll
+  for (int db = 0; db < DC / 32; ++db) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        // registers 8 b .. + 3 hold elements 4 h + 0..3 of 16, the next four 8 + 4 h + 0..3: the halves swap, and each
+        // lane has eight in a row
+        at_u4 w;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t x = at_pack(T(), acc[db][8 * b + 2 * j] * f, acc[db][8 * b + 2 * j + 1] * f);
+          uint32_t y = at_pack(T(), acc[db][8 * b + 4 + 2 * j] * f, acc[db][8 * b + 5 + 2 * j] * f);
+          at_swap(x, y);
+          w[j] = x;
+          w[2 + j] = y;
+        }
+        const int d = 32 * db + 16 * b + 8 * h;
+        if (live && d < D) *reinterpret_cast<at_u4*>(p + d) = w;
+      }
+    } else {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int d = 32 * db + 8 * b + 4 * h;
+        const at_f4 w = {acc[db][4 * b] * f, acc[db][4 * b + 1] * f, acc[db][4 * b + 2] * f, acc[db][4 * b + 3] * f};
+        if (live && d < D) *reinterpret_cast<at_f4*>(p + d) = w;
+      }
+    }
+  }
+}
+
+// Right operand of a product along rows: this lane's row (or zeros), STEPS chunks.
+template <typename T, int DC>
+__device__ __forceinline__ void at_load_row(const T* p, bool live, int D, int lane, at_u4* f) {
+  constexpr int E = 16 / (int)sizeof(T);
+  const int h = lane >> 5;
+#pragma unroll
+  for (int s = 0; s < at_row<T, DC>::STEPS; ++s) {
+    const int d = (2 * s + h) * E;
+    f[s] = live && d < D ? *reinterpret_cast<const at_u4*>(p + d) : (at_u4)(0u);
+  }
+}

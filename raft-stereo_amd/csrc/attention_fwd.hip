@@ -1,0 +1,439 @@
+// Attention of query tokens over the tokens of another sequence, forward.
+//
+//   S = scale Q K^T,  P = softmax(S) over the allowed keys,  O = P V,  lse2 = log2 sum exp2(S log2 e)
+//
+// One pass over the keys with the running maximum m and sum l of the softmax.  The rows of a work item are the query
+// tokens of all heads that share a key head (row m = token m / G, head m % G), so that a tile of keys and values is
+// staged once for the group.  Both products run transposed: S^T = K Q^T leaves a query in each lane with its scores in
+// registers (maximum and sum need one exchange between the wave's halves), and is, exponentiated and rounded, the right
+// operand of O^T = V^T P^T as it stands -- probabilities never touch LDS.
+#include "attention.h"
+
+#include <initializer_list>
+
+namespace {
+
+// Scores are compared and exponentiated in units of log2: p = exp2(s c - m), c = scale log2 e.  The accumulators are
+// rescaled only when a maximum grows by more than this (p stays under 2^8, where fp16 and fp32 have range to spare).
+constexpr float AT_SLACK = 8.0f;
+
+struct at_split {
+  float* o;     // [item][split][rows][D]: unnormalised sums
+  float* ml;    // [item][split][2][rows]: maxima, sums
+  int32_t n;    // splits of the keys
+  int32_t keys; // of one split, a multiple of the tile
+};
+
+template <typename T, int DC, int NWQ, int NWK, int NKB> struct at_fwd_cfg {
+  using R = at_row<T, DC>;
+  static constexpr int WAVES = NWQ * NWK;
+  static constexpr int ROWS = 32 * NWQ;       // query rows of a work item
+  static constexpr int KT = 32 * NKB * NWK;   // keys of a tile
+  static constexpr int TILE = KT * R::RB;
+  static constexpr int LDS = 4 * TILE;        // keys and values, two tiles each
+};
+
+// NWQ waves side by side own 32 rows each; NWK waves share the same rows and take 32 NKB keys each of every tile.
+template <typename T, int DC, int NWQ, int NWK, int NKB, int OCC>
+__global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k,
+                                                                     const T* __restrict__ v, T* __restrict__ out,
+                                                                     float* __restrict__ lse, at_split sp, at_args a,
+                                                                     int row_tiles, int64_t items) {
+  using C = at_fwd_cfg<T, DC, NWQ, NWK, NKB>;
+  using R = at_row<T, DC>;
+  constexpr int NDB = DC / 32;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int64_t item = at_item(items);
+  if (item < 0) return;
+  // rows fastest, then splits, then heads and sequences: neighbours share keys
+  const int rt = (int)(item % row_tiles);
+  const int64_t rest = item / row_tiles;
+  const int split = (int)(rest % sp.n);
+  const int nh = (int)(rest / sp.n);
+  const int n = nh / a.Hk, hk = nh - n * a.Hk;
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wq = wave % NWQ, wk = wave / NWQ;
+  const int c = lane & 31, h = lane >> 5;
+  const int rows = a.Tq * a.G, row = (rt * NWQ + wq) * 32 + c;
+  const bool live = row < rows;
+  const int t = (live ? row : 0) / a.G, g = (live ? row : 0) - t * a.G;
+
+  const int len = at_length(a, n);
+  const int k_begin = split * sp.keys, k_end = min(len, k_begin + sp.keys);
+  const int tiles = k_end > k_begin ? (k_end - k_begin + C::KT - 1) / C::KT : 0;
+
+  at_key_tiles<T, DC, C::KT, C::WAVES> kv;
+  kv.init(a, k, v, n, hk, k_begin, k_end, wave, lane);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(at_lds)smem;
+  if (tiles > 0) kv.fetch(a, lds0, lds0 + 2 * C::TILE, wave, lane);
+
+  at_u4 qf[R::STEPS];
+  at_load_row<T, DC>(q + (int64_t)n * a.qs[0] + (int64_t)t * a.qs[1] + (int64_t)(hk * a.G + g) * a.qs[2], live, a.D, lane, qf);
+
+  at_places<T, DC> at;
+  at.init(lane);
+  at_f16 acc[NDB];
+#pragma unroll
+  for (int i = 0; i < NDB; ++i) acc[i] = (at_f16)(0.0f);
+  float m = -INFINITY, l = 0.0f;
+  uint32_t any = 0;
+
+  for (int j = 0; j < tiles; ++j) {
+    at_landed();
+    if (j + 1 < tiles) kv.fetch(a, lds0 + ((j + 1) & 1) * C::TILE, lds0 + (2 + ((j + 1) & 1)) * C::TILE, wave, lane);
+    const unsigned char* kt = smem + (j & 1) * C::TILE;
+    const unsigned char* vt = smem + (2 + (j & 1)) * C::TILE;
+    const int kr = 32 * NKB * wk;  // this wave's first key of the tile
+
+    at_f16 s[NKB];
+#pragma unroll
+    for (int b = 0; b < NKB; ++b) s[b] = (at_f16)(0.0f);
+#pragma unroll
+    for (int st = 0; st < R::STEPS; ++st)
+#pragma unroll
+      for (int b = 0; b < NKB; ++b)
+        s[b] = at_mma(T(), at.rows(kt, kr + 32 * b, st), qf[st], s[b]);
+
+#pragma unroll
+    for (int b = 0; b < NKB; ++b) {
+      uint32_t w = at_key_bits(a, n, k_end, k_begin + j * C::KT + kr + 32 * b);
+      any |= w;
+      if (w != 0xffffffffu) {
+        w >>= 4 * h;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][i] = (w >> (8 * (i / 4) + i % 4)) & 1 ? s[b][i] : -INFINITY;
+      }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int b = 0; b < NKB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
+    mx = at_half_max(mx) * a.scale_log2;
+    if (__any(mx > m + AT_SLACK)) {
+      const float mn = fmaxf(m, mx);
+      const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) acc[i] *= f;
+    }
+    const float mu = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int b = 0; b < NKB; ++b) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[b][i] = __builtin_amdgcn_exp2f(s[b][i] * a.scale_log2 - mu);
+        l += s[b][i];
+      }
+      at_mma_cols<T, DC>(at, vt, kr + 32 * b, s[b], acc);
+    }
+  }
+  l = at_half_sum(l);
+
+  if constexpr (NWK > 1) {
+    // the waves that share rows meet in LDS: each writes its maximum and sums, and takes a share of the elements
+    at_sync();
+    float* mbuf = reinterpret_cast<float*>(smem);                          // [WAVES][2][32]
+    float* obuf = mbuf + C::WAVES * 64;                                    // [WAVES][NDB * 16][64]
+    if (h == 0) {
+      mbuf[wave * 64 + c] = m;
+      mbuf[wave * 64 + 32 + c] = l;
+    }
+    reinterpret_cast<uint32_t*>(obuf + C::WAVES * NDB * 1024)[wave] = any;
+#pragma unroll
+    for (int i = 0; i < NDB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) obuf[((wave * NDB + i) * 16 + r) * 64 + lane] = acc[i][r];
+    at_sync();
+    float ms[NWK], top = -INFINITY;
+    l = 0.0f;
+    any = 0;
+#pragma unroll
+    for (int x = 0; x < NWK; ++x) {
+      ms[x] = mbuf[(x * NWQ + wq) * 64 + c];
+      top = fmaxf(top, ms[x]);
+      any |= reinterpret_cast<const uint32_t*>(obuf + C::WAVES * NDB * 1024)[x * NWQ + wq];
+    }
+#pragma unroll
+    for (int x = 0; x < NWK; ++x) {
+      ms[x] = ms[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms[x] - top);
+      l += ms[x] * mbuf[(x * NWQ + wq) * 64 + 32 + c];
+    }
+    m = top;
+#pragma unroll
+    for (int i = 0; i < NDB; ++i) {
+      if (i % NWK != wk) continue;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int x = 0; x < NWK; ++x) sum += ms[x] * obuf[(((x * NWQ + wq) * NDB + i) * 16 + r) * 64 + lane];
+        acc[i][r] = sum;
+      }
+    }
+  }
+  any = __builtin_amdgcn_readfirstlane(any);
+
+  if (sp.n > 1) {
+    // no key at all: sum 0; keys, but every score -inf: NaN, as 0 / 0 is
+    l = any ? (l == 0.0f ? NAN : l) : 0.0f;
+    float* ml = sp.ml + item * 2 * C::ROWS + wq * 32;
+    if (wk == 0 && h == 0) {
+      ml[c] = m;
+      ml[C::ROWS + c] = l;
+    }
+    float* o = sp.o + (item * C::ROWS + wq * 32 + c) * a.D;
+#pragma unroll
+    for (int i = 0; i < NDB; ++i) {
+      if (NWK > 1 && i % NWK != wk) continue;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int d = 32 * i + 8 * b + 4 * h;
+        const at_f4 w = {acc[i][4 * b], acc[i][4 * b + 1], acc[i][4 * b + 2], acc[i][4 * b + 3]};
+        if (live && d < a.D) *reinterpret_cast<at_f4*>(o + d) = w;
+      }
+    }
+    return;
+  }
+  const float f = any ? 1.0f / l : 0.0f;
+  if (!any) {
+#pragma unroll
+    for (int i = 0; i < NDB; ++i) acc[i] = (at_f16)(0.0f);
+  }
+  const int hq = hk * a.G + g;
+  T* o = out + ((int64_t)((int64_t)n * a.Tq + t) * a.Hq + hq) * a.D;
+  if constexpr (NWK == 1) {
+    at_store_rows<T, DC>(o, live, acc, f, a.D, lane);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NDB; ++i)
+      if (i % NWK == wk) at_store_rows<T, 32>(o + 32 * i, live, acc + i, f, a.D - 32 * i, lane);
+  }
+  if (lse != nullptr && live && h == 0 && wk == 0)
+    lse[((int64_t)n * a.Hq + hq) * a.Tq + t] = any ? m + __builtin_amdgcn_logf(l) : INFINITY;
+}
+
+// Joins the splits: a wave per row, weights exp2(m_i - max).
+template <typename T>
+__global__ __launch_bounds__(256) void at_join_kernel(T* __restrict__ out, float* __restrict__ lse, at_split sp, at_args a,
+                                                      int row_tiles, int tile_rows, int64_t all_rows) {
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= all_rows) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t nh = i / ((int64_t)a.Tq * a.G);
+  const int row = (int)(i - nh * ((int64_t)a.Tq * a.G));
+  const int rt = row / tile_rows, r = row - rt * tile_rows;
+  const int64_t item0 = nh * sp.n * row_tiles + rt;  // + split * row_tiles
+  float top = -INFINITY, l = 0.0f;
+  for (int s = 0; s < sp.n; ++s) top = fmaxf(top, sp.ml[(item0 + (int64_t)s * row_tiles) * 2 * tile_rows + r]);
+  float acc[4] = {0, 0, 0, 0};
+  for (int s = 0; s < sp.n; ++s) {
+    const int64_t item = item0 + (int64_t)s * row_tiles;
+    const float mi = sp.ml[item * 2 * tile_rows + r], li = sp.ml[item * 2 * tile_rows + tile_rows + r];
+    if (li == 0.0f) continue;  // no key in this split
+    const float w = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - top);
+    l += w * li;
+    const float* o = sp.o + (item * tile_rows + r) * a.D;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (lane * 4 + e < a.D) acc[e] += w * o[lane * 4 + e];
+  }
+  const int n = (int)(nh / a.Hk), hk = (int)(nh - (int64_t)n * a.Hk), t = row / a.G, hq = hk * a.G + row - t * a.G;
+  const bool none = l == 0.0f;
+  T* o = out + (((int64_t)n * a.Tq + t) * a.Hq + hq) * a.D + lane * 4;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (lane * 4 + e < a.D) o[e] = rc_from_float<T>(none ? 0.0f : acc[e] / l);
+  if (lse != nullptr && lane == 0) lse[((int64_t)n * a.Hq + hq) * a.Tq + t] = none ? INFINITY : top + __builtin_amdgcn_logf(l);
+}
+
+// The mask and the lengths as one bit per key: a scalar load tells a tile what it may skip.
+__global__ __launch_bounds__(256) void at_bits_kernel(const unsigned char* __restrict__ mask, int64_t stride,
+                                                      uint64_t* __restrict__ bits, int64_t words, int Tk, int64_t total) {
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // a wave per word
+  if (w >= total) return;
+  const int64_t n = w / words, key = (w - n * words) * 64 + (threadIdx.x & 63);
+  const bool on = key < Tk && mask[n * stride + key] != 0;
+  const unsigned long long b = __ballot(on);
+  if ((threadIdx.x & 63) == 0) bits[w] = b;
+}
+
+template <typename T, int DC, int NWQ, int NWK, int NKB, int OCC>
+int at_launch(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, void* out, float* lse,
+              at_split sp, hipStream_t st) {
+  using C = at_fwd_cfg<T, DC, NWQ, NWK, NKB>;
+  constexpr int lds = NWK > 1 && C::WAVES * (64 + DC / 32 * 1024 + 4) * 4 > C::LDS ? C::WAVES * (64 + DC / 32 * 1024 + 4) * 4 : C::LDS;
+  static_assert(lds <= 160 * 1024, "LDS");
+  auto kernel = at_fwd_kernel<T, DC, NWQ, NWK, NKB, OCC>;
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) {
+      rc_set_error("rc_cross_attn_fwd: %d bytes of LDS refused: %s", lds, hipGetErrorString(e));
+      return (int)e;
+    }
+  }
+  const int64_t rows = a->Tq * d.G, row_tiles = (rows + C::ROWS - 1) / C::ROWS;
+  const int64_t items = a->N * a->Hk * sp.n * row_tiles;
+  kernel<<<at_grid(items), 64 * C::WAVES, lds, st>>>((const T*)q, (const T*)k, (const T*)v, (T*)out, lse, sp, d,
+                                                     (int)row_tiles, items);
+  int rc = rc_check_launch("rc_cross_attn_fwd");
+  if (rc || sp.n == 1) return rc;
+  const int64_t all = a->N * a->Hk * rows;
+  at_join_kernel<T><<<(uint32_t)((all + 3) / 4), 256, 0, st>>>((T*)out, lse, sp, d, (int)row_tiles, C::ROWS, all);
+  return rc_check_launch("rc_cross_attn_fwd (join)");
+}
+
+int at_padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : D <= 192 ? 192 : 256; }
+
+// How the work is cut: rows of an item, and splits of the keys.
+struct at_plan {
+  int few;            // rows fit one wave: four (two) waves share them and divide the keys
+  int tile_rows;
+  int64_t row_tiles, items;
+  at_split sp;
+};
+
+at_plan at_make_plan(const rc_attn* a) {
+  at_plan p = {};
+  const int64_t rows = a->Tq * (a->Hq / a->Hk);
+  p.few = rows <= 32;
+  p.tile_rows = p.few ? 32 : 128;
+  p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+  p.items = a->N * a->Hk * p.row_tiles;
+  // fewer work items than fill the card twice: the keys are divided too, down to 256 of them
+  int64_t n = 1;
+  if (p.items > 0 && p.items < 512) {
+    n = (512 + p.items - 1) / p.items;
+    const int64_t most = (a->Tk + 255) / 256;
+    n = n < most ? n : most;
+    n = n < 1 ? 1 : n;
+  }
+  const int64_t keys = ((a->Tk + n - 1) / n + 255) / 256 * 256;
+  p.sp.n = (int)(keys ? (a->Tk + keys - 1) / keys : 1);
+  if (p.sp.n < 1) p.sp.n = 1;
+  p.sp.keys = (int)(keys ? keys : 256);
+  return p;
+}
+
+template <typename T, int DC>
+int at_run(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, void* out, float* lse,
+           const at_plan& p, hipStream_t st) {
+  // waves of an item's keys, keys of a wave in a tile, resident workgroups: what registers and 160 KiB of LDS allow
+  constexpr int RB = at_row<T, DC>::RB;
+  constexpr int NWK = RB >= 1024 ? 1 : RB >= 512 ? 2 : 4;
+  constexpr int NKB = RB >= 512 ? 1 : 2;
+  constexpr int OCC = RB >= 512 && DC > 128 ? (DC == 192 && RB < 1024 ? 2 : 1) : RB >= 1024 ? 1 : DC * (int)sizeof(T) >= 192 ? 2 : 3;
+  if (p.few) return at_launch<T, DC, 1, NWK, 1, 1>(a, d, q, k, v, out, lse, p.sp, st);
+  return at_launch<T, DC, 4, 1, NKB, OCC>(a, d, q, k, v, out, lse, p.sp, st);
+}
+
+template <typename T>
+int at_run_d(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, void* out, float* lse,
+             const at_plan& p, hipStream_t st) {
+  switch (at_padded(a->D)) {
+    case 32: return at_run<T, 32>(a, d, q, k, v, out, lse, p, st);
+    case 64: return at_run<T, 64>(a, d, q, k, v, out, lse, p, st);
+    case 96: return at_run<T, 96>(a, d, q, k, v, out, lse, p, st);
+    case 128: return at_run<T, 128>(a, d, q, k, v, out, lse, p, st);
+    case 192: return at_run<T, 192>(a, d, q, k, v, out, lse, p, st);
+    default: return at_run<T, 256>(a, d, q, k, v, out, lse, p, st);
+  }
+}
+
+}  // namespace
+
+int at_check(const rc_attn* a) {
+  RC_REQUIRE(a != nullptr, RC_EINVAL, "rc_cross_attn: null description");
+  RC_REQUIRE(a->dtype == RC_F32 || a->dtype == RC_F16 || a->dtype == RC_BF16, RC_EUNSUPPORTED, "unknown dtype %d", a->dtype);
+  RC_REQUIRE(a->D >= 8 && a->D <= RC_HEAD_DIM_MAX && a->D % 8 == 0, RC_EUNSUPPORTED,
+             "head dimension %d is no multiple of 8 in 8..%d", a->D, RC_HEAD_DIM_MAX);
+  RC_REQUIRE(a->N >= 0 && a->N < (1ll << 31) && a->Tq >= 0 && a->Tk >= 0 && a->Hq >= 1 && a->Hk >= 1, RC_EINVAL,
+             "rc_cross_attn: negative size, or no head");
+  RC_REQUIRE(a->Hq % a->Hk == 0, RC_EINVAL, "rc_cross_attn: %d query heads are no multiple of %d key heads", a->Hq, a->Hk);
+  RC_REQUIRE(a->Tq < (1ll << 30) && a->Tk < (1ll << 30) && a->N * a->Tq < (1ll << 31) && a->N * a->Tk < (1ll << 31) &&
+                 a->N * a->Tq * a->Hq < (1ll << 31) && a->N * a->Tk * a->Hk < (1ll << 31) && a->N * a->Hk < (1ll << 31),
+             RC_EINVAL, "rc_cross_attn: more than 2^31 heads");
+  RC_REQUIRE(a->scale > 0.0f && a->scale < INFINITY, RC_EINVAL, "rc_cross_attn: scale must be positive and finite");
+  const int64_t es = a->dtype == RC_F32 ? 4 : 2;
+  const int64_t* st[3] = {a->q_stride, a->k_stride, a->v_stride};
+  for (int o = 0; o < 3; ++o)
+    for (int i = 0; i < 3; ++i)
+      RC_REQUIRE(st[o][i] >= 0 && st[o][i] * es % 16 == 0 && (i == 0 || st[o][i] * es < (1ll << 24)), RC_EINVAL,
+                 "rc_cross_attn: stride %lld of %c is negative, no multiple of 16 bytes, or 16 MiB or more between tokens "
+                 "or heads", (long long)st[o][i], "qkv"[o]);
+  RC_REQUIRE(a->key_mask == nullptr || a->mask_stride >= 0, RC_EINVAL, "rc_cross_attn: negative mask stride");
+  return RC_OK;
+}
+
+int at_check_operand(const rc_attn* a, int64_t rows, const void* p) {
+  RC_REQUIRE(rows == 0 || (p != nullptr && (uintptr_t)p % 16 == 0), RC_EINVAL,
+             "rc_cross_attn: an operand is null or not aligned to 16 bytes");
+  return RC_OK;
+}
+
+at_args at_to_dev(const rc_attn* a, void* bits) {
+  at_args d;
+  for (int i = 0; i < 3; ++i) {
+    d.qs[i] = a->q_stride[i];
+    d.ks[i] = a->k_stride[i];
+    d.vs[i] = a->v_stride[i];
+  }
+  d.lengths = a->key_lengths;
+  d.bits = a->key_mask && a->Tk ? (const uint64_t*)bits : nullptr;
+  d.words = (a->Tk + 63) / 64;
+  d.N = (int32_t)a->N;
+  d.Tq = (int32_t)a->Tq;
+  d.Tk = (int32_t)a->Tk;
+  d.Hq = a->Hq;
+  d.Hk = a->Hk;
+  d.G = a->Hq / a->Hk;
+  d.D = a->D;
+  d.lengths_i64 = a->lengths_i64;
+  d.scale = a->scale;
+  d.scale_log2 = a->scale * 1.44269504088896340736f;
+  return d;
+}
+
+int64_t at_bits_bytes(const rc_attn* a) {
+  return a->key_mask ? (a->N * ((a->Tk + 63) / 64) * 8 + 255) / 256 * 256 : 0;
+}
+
+int at_launch_bits(const rc_attn* a, void* bits, hipStream_t st) {
+  const int64_t words = (a->Tk + 63) / 64, total = a->N * words;
+  if (a->key_mask == nullptr || total == 0) return RC_OK;
+  at_bits_kernel<<<(uint32_t)((total + 3) / 4), 256, 0, st>>>(a->key_mask, a->mask_stride, (uint64_t*)bits, words, (int)a->Tk, total);
+  return rc_check_launch("rc_cross_attn (mask)");
+}
+
+extern "C" int64_t rc_cross_attn_fwd_work_bytes(const rc_attn* a) {
+  const int rc = at_check(a);
+  if (rc) return rc < 0 ? rc : RC_EINVAL;
+  const at_plan p = at_make_plan(a);
+  const int64_t parts = p.sp.n > 1 ? p.items * p.sp.n * p.tile_rows * (a->D + 2) * (int64_t)sizeof(float) : 0;
+  return at_bits_bytes(a) + parts;
+}
+
+extern "C" int rc_cross_attn_fwd(const rc_attn* a, const void* q, const void* k, const void* v, void* out, float* lse,
+                                 void* work, void* stream) {
+  int rc = at_check(a);
+  if (rc) return rc;
+  for (const void* p : {q, (const void*)out})
+    if ((rc = at_check_operand(a, a->N * a->Tq, p))) return rc;
+  for (const void* p : {k, v})
+    if ((rc = at_check_operand(a, a->N * a->Tk, p))) return rc;
+  if (a->N * a->Tq == 0) return RC_OK;
+  at_plan p = at_make_plan(a);
+  RC_REQUIRE((p.sp.n == 1 && at_bits_bytes(a) == 0) || (work != nullptr && (uintptr_t)work % 16 == 0), RC_EINVAL,
+             "rc_cross_attn_fwd: work is null or not aligned to 16 bytes");
+  RC_REQUIRE(p.items * p.sp.n < (1ll << 31) - 8, RC_EINVAL, "rc_cross_attn_fwd: too many rows");
+  hipStream_t st = (hipStream_t)stream;
+  if ((rc = at_launch_bits(a, work, st))) return rc;
+  p.sp.o = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + at_bits_bytes(a));
+  p.sp.ml = p.sp.o + p.items * p.sp.n * p.tile_rows * a->D;
+  const at_args d = at_to_dev(a, work);
+  if (a->dtype == RC_F32) return at_run_d<float>(a, d, q, k, v, out, lse, p, st);
+  if (a->dtype == RC_F16) return at_run_d<rc_half>(a, d, q, k, v, out, lse, p, st);
+  return at_run_d<rc_bf16>(a, d, q, k, v, out, lse, p, st);
+}
