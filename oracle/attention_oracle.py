@@ -55,7 +55,10 @@ def attention(q, k, v, g=None, ok=None, scale=None, dtype="f32"):
     mag = (np.abs(Q) @ np.swapaxes(np.abs(K), 2, 3)) * scale
     worst = mag.max(axis=3, keepdims=True, initial=0.0)
     rel = F32 * (2 * (D + 8) * worst + 16 + Tk)
-    tiny = 2.0 ** -25 if dtype == "f16" else 0.0                   # half a step of fp16's smallest numbers
+    # exp2 gives zero for what is below fp32's smallest normal number: a probability, its sum being at least 1, may be off
+    # by that much however small it is
+    flush = 2.0 ** -126
+    tiny = flush + 2.0 ** -25 if dtype == "f16" else flush       # (half a step of fp16's smallest numbers)
     rnd = 0.0 if dtype == "f32" else u
     A = P @ np.abs(V)
     o_err = (rnd + rel + Tk * F32) * A + tiny * np.abs(V).sum(axis=2, keepdims=True)
@@ -72,7 +75,7 @@ def attention(q, k, v, g=None, ok=None, scale=None, dtype="f32"):
     delta_err = (np.abs(Gr) * (o_err + u * np.abs(O) + D * F32 * np.abs(O))).sum(axis=3, keepdims=True)
     dp_err = D * F32 * (np.abs(Gr) @ np.swapaxes(np.abs(V), 2, 3))
     ds_mag = P * (np.abs(dP) + np.abs(delta))
-    ds_err = rnd * np.abs(dS) + P * (delta_err + dp_err) + (rel + 4 * F32) * ds_mag
+    ds_err = rnd * np.abs(dS) + P * (delta_err + dp_err) + (rel + 4 * F32) * ds_mag + flush * (np.abs(dP) + np.abs(delta))
     # fp16: scores' gradients are scaled so that a row's or column's largest is far from fp16's smallest
     least = 2.0 ** -30 if dtype == "f16" else 0.0
     rows_err = ds_err + least * np.abs(dS).max(axis=3, keepdims=True, initial=0.0)
@@ -82,7 +85,7 @@ def attention(q, k, v, g=None, ok=None, scale=None, dtype="f32"):
     dK = np.swapaxes(dS, 2, 3) @ Q * scale
     k_err = np.swapaxes(cols_err + G * Tq * F32 * np.abs(dS), 2, 3) @ np.abs(Q) * scale
     dV = np.swapaxes(P, 2, 3) @ Gr
-    p_err = P * (rnd + rel + G * Tq * F32) + tiny * 2.0 ** -8
+    p_err = P * (rnd + rel + G * Tq * F32) + flush + (tiny - flush) * 2.0 ** -8
     v_err = np.swapaxes(p_err * np.ones_like(P), 2, 3) @ np.abs(Gr)
     res["dq"] = (back(dQ), back(q_err + u * np.abs(dQ) + 1e-37))
     for name, d, e in (("dk", dK, k_err), ("dv", dV, v_err)):

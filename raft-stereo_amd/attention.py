@@ -22,6 +22,7 @@ from raft_stereo_amd.corr import _DT, _stream, _on_device
 
 _POS = {torch.int32: _lib.RC_POS_I32, torch.int64: _lib.RC_POS_I64, torch.float32: _lib.RC_POS_F32}
 _MAX_STRIDE_BYTES = 1 << 24     # between tokens or heads: a tile's rows are addressed with 32 bits
+_MAX_SPAN_BYTES = 1 << 30       # from a token's first head to its last
 
 
 def _check_heads(t, what):
@@ -48,7 +49,8 @@ def _heads_view(t):
     boundaries (slices of a wider projection qualify, and expanded dimensions).  Anything else is copied."""
     es = t.element_size()
     st = [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s * es % 16 for s in st) or max(st[1:]) * es >= _MAX_STRIDE_BYTES:
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s * es % 16 for s in st) or max(st[1:]) * es >= _MAX_STRIDE_BYTES \
+            or t.shape[2] * st[2] * es >= _MAX_SPAN_BYTES:
         t = t.clone(memory_format=torch.contiguous_format)
         st = list(t.stride()[:3])
         if max(s if n > 1 else 0 for n, s in zip(t.shape[1:3], st[1:])) * es >= _MAX_STRIDE_BYTES:

@@ -52,10 +52,15 @@ __device__ __forceinline__ int at_length(const at_args& a, int n) {
   return __builtin_amdgcn_readfirstlane((int)(l > a.Tk ? a.Tk : l));
 }
 
+// one bit for each of the first `left` of 32 rows
+__device__ __forceinline__ uint32_t at_first_bits(int left) {
+  return left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+}
+
 // the keys k0 .. k0 + 31 (k0 a multiple of 32) that take part, one bit each
 __device__ __forceinline__ uint32_t at_key_bits(const at_args& a, int n, int len, int k0) {
   const int left = len - k0;
-  uint32_t w = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+  uint32_t w = at_first_bits(left);
   if (a.bits != nullptr && left > 0)
     w &= reinterpret_cast<const uint32_t*>(a.bits)[((int64_t)n * a.words) * 2 + (k0 >> 5)];
   return __builtin_amdgcn_readfirstlane(w);
@@ -75,6 +80,29 @@ __device__ __forceinline__ at_f16 at_mma(float, at_u4 a, at_u4 b, at_f16 c) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
   return c;
+}
+
+// products of 16 bytes of elements, summed in fp32
+__device__ __forceinline__ float at_dot(rc_half, at_u4 a, at_u4 b) {
+  const at_h8 x = __builtin_bit_cast(at_h8, a), y = __builtin_bit_cast(at_h8, b);
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += (float)x[i] * (float)y[i];
+  return s;
+}
+__device__ __forceinline__ float at_dot(rc_bf16, at_u4 a, at_u4 b) {
+  const at_b8 x = __builtin_bit_cast(at_b8, a), y = __builtin_bit_cast(at_b8, b);
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += (float)x[i] * (float)y[i];
+  return s;
+}
+__device__ __forceinline__ float at_dot(float, at_u4 a, at_u4 b) {
+  const at_f4 x = __builtin_bit_cast(at_f4, a), y = __builtin_bit_cast(at_f4, b);
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s += x[i] * y[i];
+  return s;
 }
 
 __device__ __forceinline__ uint32_t at_pack(rc_half, float x, float y) {
@@ -196,7 +224,7 @@ __device__ __forceinline__ void at_mma_cols(const at_places<T, DC>& at, const un
 // the swizzle is applied to the addresses that the lanes fetch from.  Chunks behind the head's end and rows that do
 // not take part are fetched from beyond the buffer's range, which gives zeros (so whatever those rows hold, NaN
 // included, never meets a product).
-constexpr uint32_t AT_RANGE = 0x80010000u, AT_OUTSIDE = 0xc0000000u;
+constexpr uint32_t AT_RANGE = 0x80010000u, AT_OUTSIDE = 0xc0000000u;  // (+ a row's length: still outside, no wrap)
 
 template <typename T, int DC, int ROWS, int WAVES> struct at_stage {
   using R = at_row<T, DC>;
@@ -215,6 +243,15 @@ template <typename T, int DC, int ROWS, int WAVES> struct at_stage {
     for (int p = 0; p < PD; ++p) {
       const int r = p * STEP + wave * PER + lane / R::CH, chunk = (lane % R::CH) ^ at_swizzle<R::CH>(r);
       off[p] = chunk * 16 < D * R::ES ? (uint32_t)r * stride + (uint32_t)chunk * 16u : AT_OUTSIDE;
+    }
+  }
+  // words[i]: rows 32 i .. that take part -> the word of each instruction's rows
+  static __device__ __forceinline__ void spread(const uint32_t (&words)[ROWS / 32], int wave, uint32_t (&take)[N]) {
+#pragma unroll
+    for (int p = 0; p < N; ++p) {
+      take[p] = words[0];
+#pragma unroll
+      for (int i = 1; i < ROWS / 32; ++i) take[p] = (p * STEP + wave * PER) >> 5 == i ? words[i] : take[p];
     }
   }
   // base: the tile's first row; take[p]: the rows of the 32 that instruction p's rows lie in that take part, a bit each
@@ -260,9 +297,10 @@ template <typename T, int DC, int KT, int WAVES> struct at_key_tiles {
   __device__ __forceinline__ void fetch(const at_args& a, uint32_t lds_k, uint32_t lds_v, int wave, int lane) {
     uint32_t take[S::N];
     const bool full = a.bits == nullptr && k_end - k0 >= KT;
+    uint32_t words[KT / 32];
 #pragma unroll
-    for (int p = 0; p < S::N; ++p)
-      take[p] = full ? 0xffffffffu : at_key_bits(a, n, k_end, k0 + ((p * S::STEP + wave * S::PER) & ~31));
+    for (int i = 0; i < KT / 32; ++i) words[i] = full ? 0xffffffffu : at_key_bits(a, n, k_end, k0 + 32 * i);
+    S::spread(words, wave, take);
     k.issue(kp, lds_k, wave, lane, full, take);
     v.issue(vp, lds_v, wave, lane, full, take);
     kp += kstep;
@@ -283,6 +321,20 @@ __device__ __forceinline__ void at_sync() {
   asm volatile("" ::: "memory");
 }
 
+// up to 64 floats to LDS, zeros behind the first `left`
+__device__ __forceinline__ void at_fetch_floats(const float* base, int left, uint32_t lds, int lane) {
+  const uint64_t b = (uint64_t)base;
+  typedef int i4 __attribute__((ext_vector_type(4)));
+  const i4 rs = {__builtin_amdgcn_readfirstlane((int)b), __builtin_amdgcn_readfirstlane((int)(b >> 32) & 0xffff), (int)AT_RANGE,
+                 0x00020000};
+  const uint32_t o = lane < left ? (uint32_t)lane * 4u : AT_OUTSIDE;
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep)
+               : "v"(o), "s"(rs), "s"(__builtin_amdgcn_readfirstlane(lds))
+               : "memory");
+}
+
 // Block id -> work item: ids go round the 8 XCDs, items that share keys should share an XCD's L2, so each XCD gets a
 // run of consecutive items.  The grid has at_grid() blocks.
 __device__ __forceinline__ int64_t at_item(int64_t items) {
@@ -291,9 +343,6 @@ __device__ __forceinline__ int64_t at_item(int64_t items) {
   return (blockIdx.x >> 3) < per && i < items ? i : -1;
 }
 static inline uint32_t at_grid(int64_t items) { return (uint32_t)((items + 7) / 8 * 8); }
-
-// four consecutive elements of a row
-__device__ __forceinline__ void at_store4(float* p, at_f4 v) { *reinterpret_cast<at_f4*>(p) = v; }
 
 // Writes a result (rows: elements 32 db .. of the head, column: this lane's row of memory at p) times f.
 template <typename T, int DC>
@@ -329,14 +378,23 @@ __device__ __forceinline__ void at_store_rows(T* p, bool live, const at_f16* acc
   }
 }
 
-// Right operand of a product along rows: this lane's row (or zeros), STEPS chunks.
-template <typename T, int DC>
-__device__ __forceinline__ void at_load_row(const T* p, bool live, int D, int lane, at_u4* f) {
-  constexpr int E = 16 / (int)sizeof(T);
-  const int h = lane >> 5;
-#pragma unroll
-  for (int s = 0; s < at_row<T, DC>::STEPS; ++s) {
-    const int d = (2 * s + h) * E;
-    f[s] = live && d < D ? *reinterpret_cast<const at_u4*>(p + d) : (at_u4)(0u);
+// Right operand of a product along rows: this lane's row, STEPS chunks.  base: the same for the whole wave; off: bytes to
+// this lane's row, AT_OUTSIDE if it has none (zeros then).
+struct at_rows_of {
+  __amdgpu_buffer_rsrc_t rs;
+  __device__ __forceinline__ explicit at_rows_of(const void* base) {
+    const uint64_t b = (uint64_t)base;
+    const uint64_t u = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) |
+                       (uint32_t)__builtin_amdgcn_readfirstlane((int)b);
+    rs = __builtin_amdgcn_make_buffer_rsrc((void*)u, 0, (int)AT_RANGE, 0x00020000);
   }
-}
+  template <typename T> __device__ __forceinline__ at_u4 chunk(uint32_t off, int D, int st, int h) const {
+    const uint32_t b = (uint32_t)(2 * st + h) * 16u;
+    const uint32_t o = b < (uint32_t)D * (uint32_t)sizeof(T) ? off + b : AT_OUTSIDE;
+    return __builtin_bit_cast(at_u4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)o, 0, 0));
+  }
+  template <typename T, int DC> __device__ __forceinline__ void row(uint32_t off, int D, int lane, at_u4* f) const {
+#pragma unroll
+    for (int st = 0; st < at_row<T, DC>::STEPS; ++st) f[st] = chunk<T>(off, D, st, lane >> 5);
+  }
+};

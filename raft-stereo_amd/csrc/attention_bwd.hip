@@ -1,171 +1,444 @@
-// Attention of query tokens over the tokens of another sequence, and its adjoint.
+// Attention of query tokens over the tokens of another sequence, backward.
 //
-//   S = scale Q K^T,  P = softmax(S) over the allowed keys,  O = P V
-//   lse2 = log2 sum exp2(S log2 e);   delta = sum_d dO O;   dS = P (dO V^T - delta)
-//   dV = P^T dO,   dQ = scale dS K,   dK = scale dS^T Q
+//   P = exp2(S c - lse2),  delta = sum_d dO O,  dS = P (dO V^T - delta)
+//   dV = P^T dO,  dQ = scale dS K,  dK = scale dS^T Q
+//
+// Two kernels, each of which owns what it adds up, so there are no atomics and every run gives the same bits; the price
+// is that S and dO V^T are worked out twice (7 products instead of 5).
+//   at_dq_kernel   a wave has 32 query rows and goes through the keys: S^T = K Q^T and dP^T = V dO^T leave a query in
+//                  each lane, dS^T is the right operand of dQ^T = K^T dS^T as it stands.  It also works out delta.
+//   at_dkv_kernel  a wave has 32 keys and goes through the query rows of all heads that share them: S = Q K^T and
+//                  dP = dO V^T leave a key in each lane; dV^T = dO^T P, dK^T = Q^T dS.
 #include "attention.h"
+
+#include <initializer_list>
 
 namespace {
 
-constexpr int AT_WAVES = 4;
-
-__device__ __forceinline__ bool at_allowed(const at_args& a, int n, int key, int len) {
-  return key < len && (a.bits == nullptr || (a.bits[(int64_t)n * a.words + (key >> 6)] >> (key & 63)) & 1);
-}
-
-__device__ __forceinline__ float at_wave_sum(float v) {
+// fp16 has no room for scores' gradients as they come (of a long row they lie below its smallest normal number, of a
+// scaled loss beyond its largest).  Each lane's column has a power of two of its own, that of the running largest, and
+// its sums are rescaled when a larger one comes along, like a softmax's.  (P is at most 1: 2^12 throughout.)
+template <typename T> struct at_fit {
+  static constexpr bool ON = sizeof(T) == 2 && __is_same(T, rc_half);
+  float s = ON ? 0.0f : 1.0f;
+  template <int NDB> __device__ __forceinline__ void fit(at_f16& x, at_f16* acc) {
+    if constexpr (ON) {
+      float mx = 0.0f;
 #pragma unroll
-  for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m);
-  return v;
-}
-
-template <typename T> __device__ __forceinline__ float at_dot(const float* a, const T* b, int D) {
-  float s = 0.0f;
-  for (int d = 0; d < D; ++d) s += a[d] * rc_to_float(b[d]);
-  return s;
-}
-
-// delta[n, h, t] = sum_d dO O, one wave per row
-template <typename T>
-__global__ __launch_bounds__(AT_WAVES * 64) void at_delta_kernel(const T* __restrict__ out, const T* __restrict__ dout,
-                                                                 float* __restrict__ delta, at_args a) {
-  const int64_t row = (int64_t)blockIdx.x * AT_WAVES + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (row >= (int64_t)a.N * a.Tq * a.Hq) return;
-  float s = 0.0f;
-  for (int d = lane; d < a.D; d += 64) s += rc_to_float(out[row * a.D + d]) * rc_to_float(dout[row * a.D + d]);
-  s = at_wave_sum(s);
-  const int h = (int)(row % a.Hq);
-  const int64_t nt = row / a.Hq;
-  const int n = (int)(nt / a.Tq), t = (int)(nt - (int64_t)n * a.Tq);
-  if (lane == 0) delta[((int64_t)n * a.Hq + h) * a.Tq + t] = s;
-}
-
-template <typename T>
-__global__ __launch_bounds__(AT_WAVES * 64) void at_dq_kernel(const T* __restrict__ q, const T* __restrict__ k,
-                                                              const T* __restrict__ v, const T* __restrict__ dout,
-                                                              const float* __restrict__ lse,
-                                                              const float* __restrict__ delta, T* __restrict__ dq,
-                                                              at_args a) {
-  __shared__ float qrow[AT_WAVES][RC_HEAD_DIM_MAX], grow[AT_WAVES][RC_HEAD_DIM_MAX];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t rows = (int64_t)a.N * a.Tq * a.Hq;
-  int64_t row = (int64_t)blockIdx.x * AT_WAVES + wave;
-  const bool live = row < rows;
-  row = live ? row : rows - 1;
-  const int h = (int)(row % a.Hq);
-  const int64_t nt = row / a.Hq;
-  const int n = (int)(nt / a.Tq), t = (int)(nt - (int64_t)n * a.Tq);
-  const int hk = h / (a.Hq / a.Hk);
-  const T* qp = q + n * a.qs[0] + t * a.qs[1] + h * a.qs[2];
-  for (int d = lane; d < a.D; d += 64) {
-    qrow[wave][d] = rc_to_float(qp[d]);
-    grow[wave][d] = rc_to_float(dout[row * a.D + d]);
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(x[i]));
+      mx = at_half_max(mx);
+      const bool need = mx * s > 32768.0f || (s == 0.0f && mx > 0.0f);
+      if (__any(need)) {
+        const int e = max(__builtin_amdgcn_frexp_expf(mx), -110);
+        const float to = need ? ldexpf(1.0f, 11 - e) : s;
+        const float f = s == 0.0f ? 1.0f : to / s;
+#pragma unroll
+        for (int i = 0; i < NDB; ++i) acc[i] *= f;
+        s = to;
+      }
+      x *= s;
+    }
   }
-  __syncthreads();
+  __device__ __forceinline__ float undo() const { return ON ? (s == 0.0f ? 1.0f : 1.0f / s) : 1.0f; }
+};
+template <typename T> constexpr float AT_P_LIFT = at_fit<T>::ON ? 12.0f : 0.0f;
+
+struct at_parts {
+  float* p;       // [split][...]: fp32 parts in the result's layout; NULL: one split, the result itself is written
+  int64_t part;   // elements of one split
+  int32_t n;      // splits
+  int32_t per;    // keys, or tiles of query rows, of one split
+};
+
+template <typename T, int DC, int KT, int WAVES> struct at_dq_lds {
+  static constexpr int TILE = KT * at_row<T, DC>::RB;
+  static constexpr int BYTES = 4 * TILE;
+};
+
+template <typename T, int DC, int NW, int NKB, int OCC>
+__global__ __launch_bounds__(64 * NW, OCC) void at_dq_kernel(const T* __restrict__ q, const T* __restrict__ k,
+                                                             const T* __restrict__ v, const T* __restrict__ out,
+                                                             const float* __restrict__ lse, const T* __restrict__ dout,
+                                                             float* __restrict__ delta, T* __restrict__ dq, at_parts sp,
+                                                             at_args a, int row_tiles, int64_t items) {
+  using R = at_row<T, DC>;
+  constexpr int NDB = DC / 32, KT = 32 * NKB;
+  constexpr int TILE = at_dq_lds<T, DC, KT, NW>::TILE;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int64_t item = at_item(items);
+  if (item < 0) return;
+  const int rt = (int)(item % row_tiles);
+  const int64_t rest = item / row_tiles;
+  const int split = (int)(rest % sp.n), nh = (int)(rest / sp.n);
+  const int n = nh / a.Hk, hk = nh - n * a.Hk;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int c = lane & 31, h = lane >> 5;
+  const int row0 = (rt * NW + wave) * 32, row = row0 + c;
+  const bool live = row < a.Tq * a.G;
+  const int first = min(row0 / a.G, a.Tq - 1);  // the wave's first token
+  const int t = live ? row / a.G : first, g = live ? row - t * a.G : 0, hq = hk * a.G + g;
+
   const int len = at_length(a, n);
-  const float L = lse[((int64_t)n * a.Hq + h) * a.Tq + t], dl = delta[((int64_t)n * a.Hq + h) * a.Tq + t];
-  float acc[4] = {0, 0, 0, 0};
-  for (int k0 = 0; k0 < len; k0 += 64) {
-    const int key = k0 + lane;
-    const bool ok = at_allowed(a, n, key, len);
-    float ds = 0.0f;
-    if (ok) {
-      const float s = at_dot(qrow[wave], k + n * a.ks[0] + key * a.ks[1] + hk * a.ks[2], a.D) * a.scale_log2;
-      const float dp = at_dot(grow[wave], v + n * a.vs[0] + key * a.vs[1] + hk * a.vs[2], a.D);
-      ds = exp2f(s - L) * (dp - dl);
-    }
-    const unsigned long long okm = __ballot(ok);
-    for (int j = 0; j < 64 && k0 + j < len; ++j) {
-      if (!((okm >> j) & 1)) continue;
-      const float dj = __shfl(ds, j);
-      const T* kp = k + n * a.ks[0] + (int64_t)(k0 + j) * a.ks[1] + hk * a.ks[2];
+  const int k_begin = split * sp.per, k_end = min(len, k_begin + sp.per);
+  const int tiles = k_end > k_begin ? (k_end - k_begin + KT - 1) / KT : 0;
+  at_key_tiles<T, DC, KT, NW> kv;
+  kv.init(a, k, v, n, hk, k_begin, k_end, wave, lane);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(at_lds)smem;
+  if (tiles > 0) kv.fetch(a, lds0, lds0 + 2 * TILE, wave, lane);
+
+  const int64_t orow = (((int64_t)n * a.Tq + t) * a.Hq + hq) * a.D, srow = ((int64_t)n * a.Hq + hq) * a.Tq + t;
+  at_u4 qf[R::STEPS], gf[R::STEPS];
+  at_rows_of(q + (int64_t)n * a.qs[0] + (int64_t)first * a.qs[1] + (int64_t)hk * a.G * a.qs[2])
+      .row<T, DC>(live ? (uint32_t)(t - first) * (uint32_t)(a.qs[1] * sizeof(T)) + (uint32_t)g * (uint32_t)(a.qs[2] * sizeof(T))
+                       : AT_OUTSIDE,
+                  a.D, lane, qf);
+  const int64_t obase = (((int64_t)n * a.Tq + first) * a.Hq + hk * a.G) * a.D;
+  const uint32_t ooff = live ? (uint32_t)(orow - obase) * (uint32_t)sizeof(T) : AT_OUTSIDE;
+  at_rows_of(dout + obase).row<T, DC>(ooff, a.D, lane, gf);
+  const float ls = live ? lse[srow] : INFINITY;
+  float dl = 0.0f;
+  {
+    const at_rows_of of(out + obase);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < a.D) acc[i] += dj * rc_to_float(kp[lane + 64 * i]);
+    for (int s = 0; s < R::STEPS; ++s) {
+      dl += at_dot(T(), of.chunk<T>(ooff, a.D, s, h), gf[s]);
+      if (s % 8 == 7) asm volatile("" ::: "memory");  // (not all of the row at once: registers)
+    }
+    dl = at_half_sum(dl);
+    if (live && h == 0 && split == 0) delta[srow] = dl;
+  }
+  at_places<T, DC> at;
+  at.init(lane);
+  at_f16 acc[NDB];
+#pragma unroll
+  for (int i = 0; i < NDB; ++i) acc[i] = (at_f16)(0.0f);
+  at_fit<T> fit;
+
+  for (int j = 0; j < tiles; ++j) {
+    at_landed();
+    if (j + 1 < tiles) kv.fetch(a, lds0 + ((j + 1) & 1) * TILE, lds0 + (2 + ((j + 1) & 1)) * TILE, wave, lane);
+    const unsigned char* kt = smem + (j & 1) * TILE;
+    const unsigned char* vt = smem + (2 + (j & 1)) * TILE;
+#pragma unroll
+    for (int b = 0; b < NKB; ++b) {
+      at_f16 s = (at_f16)(0.0f), dp = (at_f16)(0.0f);
+#pragma unroll
+      for (int st = 0; st < R::STEPS; ++st) {
+        s = at_mma(T(), at.rows(kt, 32 * b, st), qf[st], s);
+        dp = at_mma(T(), at.rows(vt, 32 * b, st), gf[st], dp);
+        if (R::RB >= 1024 && st % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // registers: no reading further ahead
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * a.scale_log2 - ls) * (dp[i] - dl);
+      uint32_t w = at_key_bits(a, n, k_end, k_begin + j * KT + 32 * b);
+      if (w != 0xffffffffu) {
+        w >>= 4 * h;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = (w >> (8 * (i / 4) + i % 4)) & 1 ? s[i] : 0.0f;
+      }
+      fit.template fit<NDB>(s, acc);
+      at_mma_cols<T, DC>(at, kt, 32 * b, s, acc);
     }
   }
-  if (!live) return;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < a.D) dq[row * a.D + lane + 64 * i] = rc_from_float<T>(acc[i] * a.scale);
+  if (dq == nullptr) return;
+  const float f = a.scale * fit.undo();
+  if (sp.n > 1) at_store_rows<float, DC>(sp.p + split * sp.part + orow, live, acc, f, a.D, lane);
+  else at_store_rows<T, DC>(dq + orow, live, acc, f, a.D, lane);
 }
 
-// One wave per key row: 64 query rows of the group at a time.
-template <typename T>
-__global__ __launch_bounds__(AT_WAVES * 64) void at_dkv_kernel(const T* __restrict__ q, const T* __restrict__ k,
-                                                               const T* __restrict__ v, const T* __restrict__ dout,
-                                                               const float* __restrict__ lse,
-                                                               const float* __restrict__ delta, T* __restrict__ dk,
-                                                               T* __restrict__ dv, at_args a) {
-  __shared__ float krow[AT_WAVES][RC_HEAD_DIM_MAX], vrow[AT_WAVES][RC_HEAD_DIM_MAX];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t rows = (int64_t)a.N * a.Tk * a.Hk;
-  int64_t row = (int64_t)blockIdx.x * AT_WAVES + wave;
-  const bool live = row < rows;
-  row = live ? row : rows - 1;
-  const int hk = (int)(row % a.Hk), group = a.Hq / a.Hk;
-  const int64_t nt = row / a.Hk;
-  const int n = (int)(nt / a.Tk), t = (int)(nt - (int64_t)n * a.Tk);
-  const bool ok = at_allowed(a, n, (int)t, at_length(a, n));
-  for (int d = lane; d < a.D; d += 64) {
-    krow[wave][d] = rc_to_float(k[n * a.ks[0] + t * a.ks[1] + hk * a.ks[2] + d]);
-    vrow[wave][d] = rc_to_float(v[n * a.vs[0] + t * a.vs[1] + hk * a.vs[2] + d]);
+template <typename T, int DC, int RT> struct at_dkv_lds {
+  static constexpr int TILE = RT * at_row<T, DC>::RB;
+  static constexpr int STAT = 256;  // bytes of a tile's lse2 (delta): 64 floats, what one load moves
+  static constexpr int BYTES = 4 * TILE + 4 * STAT;
+};
+
+// rows t0 .. of one query head: Q, dO, lse2 and delta
+template <typename T, int DC, int RT, int NW> struct at_query_tiles {
+  using S = at_stage<T, DC, RT, NW>;
+  S sq, sg;
+
+  __device__ __forceinline__ void init(const at_args& a, int wave, int lane) {
+    sq.init(wave, lane, a.D, (uint32_t)(a.qs[1] * sizeof(T)));
+    sg.init(wave, lane, a.D, (uint32_t)(a.Hq * a.D * (int)sizeof(T)));
   }
-  __syncthreads();
-  float ak[4] = {0, 0, 0, 0}, av[4] = {0, 0, 0, 0};
-  if (ok) {
-    for (int g = 0; g < group; ++g) {
-      const int h = hk * group + g;
-      for (int t0 = 0; t0 < a.Tq; t0 += 64) {
-        const int tq = t0 + lane;
-        float p = 0.0f, ds = 0.0f;
-        if (tq < a.Tq) {
-          const float s = at_dot(krow[wave], q + n * a.qs[0] + tq * a.qs[1] + h * a.qs[2], a.D) * a.scale_log2;
-          const float dp = at_dot(vrow[wave], dout + (((int64_t)n * a.Tq + tq) * a.Hq + h) * a.D, a.D);
-          p = exp2f(s - lse[((int64_t)n * a.Hq + h) * a.Tq + tq]);
-          ds = p * (dp - delta[((int64_t)n * a.Hq + h) * a.Tq + tq]);
-        }
-        for (int j = 0; j < 64 && t0 + j < a.Tq; ++j) {
-          const float pj = __shfl(p, j), dj = __shfl(ds, j);
-          const T* qp = q + n * a.qs[0] + (t0 + j) * a.qs[1] + h * a.qs[2];
-          const T* gp = dout + (((int64_t)n * a.Tq + t0 + j) * a.Hq + h) * a.D;
+  __device__ __forceinline__ void fetch(const at_args& a, const T* q, const T* dout, const float* lse, const float* delta, int n,
+                                        int hq, int t0, uint32_t lds_q, uint32_t lds_g, uint32_t lds_l, uint32_t lds_d, int wave,
+                                        int lane) const {
+    const int left = a.Tq - t0;
+    uint32_t take[S::N];
+    uint32_t words[RT / 32];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (lane + 64 * i < a.D) {
-              ak[i] += dj * rc_to_float(qp[lane + 64 * i]);
-              av[i] += pj * rc_to_float(gp[lane + 64 * i]);
-            }
+    for (int i = 0; i < RT / 32; ++i) words[i] = at_first_bits(left - 32 * i);
+    S::spread(words, wave, take);
+    const bool full = left >= RT;
+    sq.issue(reinterpret_cast<const char*>(q + (int64_t)n * a.qs[0] + (int64_t)t0 * a.qs[1] + (int64_t)hq * a.qs[2]), lds_q, wave,
+             lane, full, take);
+    sg.issue(reinterpret_cast<const char*>(dout + (((int64_t)n * a.Tq + t0) * a.Hq + hq) * a.D), lds_g, wave, lane, full, take);
+    const int64_t srow = ((int64_t)n * a.Hq + hq) * a.Tq + t0;
+    if (wave == 0) at_fetch_floats(lse + srow, left, lds_l, lane);
+    if (wave == NW - 1) at_fetch_floats(delta + srow, left, lds_d, lane);
+  }
+};
+
+template <typename T, int DC, int NW, int NRB, bool DO_K, bool DO_V, int OCC>
+__global__ __launch_bounds__(64 * NW, OCC) void at_dkv_kernel(const T* __restrict__ q, const T* __restrict__ k,
+                                                              const T* __restrict__ v, const float* __restrict__ lse,
+                                                              const T* __restrict__ dout, const float* __restrict__ delta,
+                                                              T* __restrict__ dk, T* __restrict__ dv, at_parts sp, at_args a,
+                                                              int key_tiles, int row_tiles, int64_t items) {
+  using R = at_row<T, DC>;
+  constexpr int NDB = DC / 32, RT = 32 * NRB;
+  using L = at_dkv_lds<T, DC, RT>;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+  const int64_t item = at_item(items);
+  if (item < 0) return;
+  const int kt = (int)(item % key_tiles);
+  const int64_t rest = item / key_tiles;
+  const int split = (int)(rest % sp.n), nh = (int)(rest / sp.n);
+  const int n = nh / a.Hk, hk = nh - n * a.Hk;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int c = lane & 31, h = lane >> 5;
+  const int key0 = (kt * NW + wave) * 32, key = key0 + c;
+  const int len = at_length(a, n);
+  const uint32_t mine = at_key_bits(a, n, len, key0);
+  const bool live = key < a.Tk, takes = (mine >> c) & 1;
+
+  // tiles of query rows, all heads of the group one after the other; none if no key of the workgroup takes part
+  uint32_t some = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) some |= at_key_bits(a, n, len, (kt * NW + w) * 32);
+  const int begin = split * sp.per, end = some ? min(a.G * row_tiles, begin + sp.per) : begin;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(at_lds)smem;
+  const uint32_t stat0 = lds0 + 4 * L::TILE;
+  at_query_tiles<T, DC, RT, NW> qt;
+  qt.init(a, wave, lane);
+  int g = row_tiles ? begin / row_tiles : 0, t0 = (begin - g * row_tiles) * RT;  // of the tile that is fetched next
+  auto fetch = [&](int buf) {
+    qt.fetch(a, q, dout, lse, delta, n, hk * a.G + g, t0, lds0 + buf * L::TILE, lds0 + (2 + buf) * L::TILE, stat0 + buf * L::STAT,
+             stat0 + (2 + buf) * L::STAT, wave, lane);
+    t0 += RT;
+    if (t0 >= a.Tq) {
+      t0 = 0;
+      ++g;
+    }
+  };
+  if (begin < end) fetch(0);
+
+  at_u4 kf[R::STEPS], vf[DO_K ? R::STEPS : 1];
+  at_rows_of(k + (int64_t)n * a.ks[0] + (int64_t)key0 * a.ks[1] + (int64_t)hk * a.ks[2])
+      .row<T, DC>(takes ? (uint32_t)c * (uint32_t)(a.ks[1] * sizeof(T)) : AT_OUTSIDE, a.D, lane, kf);
+  if constexpr (DO_K)
+    at_rows_of(v + (int64_t)n * a.vs[0] + (int64_t)key0 * a.vs[1] + (int64_t)hk * a.vs[2])
+        .row<T, DC>(takes ? (uint32_t)c * (uint32_t)(a.vs[1] * sizeof(T)) : AT_OUTSIDE, a.D, lane, vf);
+  at_places<T, DC> at;
+  at.init(lane);
+  at_f16 acck[DO_K ? NDB : 1], accv[DO_V ? NDB : 1];
+#pragma unroll
+  for (int i = 0; i < NDB; ++i) {
+    if constexpr (DO_K) acck[i] = (at_f16)(0.0f);
+    if constexpr (DO_V) accv[i] = (at_f16)(0.0f);
+  }
+  at_fit<T> fit;
+
+  for (int j = begin; j < end; ++j) {
+    const int buf = (j - begin) & 1;
+    at_landed();
+    if (j + 1 < end) fetch(buf ^ 1);
+    const unsigned char* qs = smem + buf * L::TILE;
+    const unsigned char* gs = smem + (2 + buf) * L::TILE;
+    const float* ls = reinterpret_cast<const float*>(smem + 4 * L::TILE + buf * L::STAT);
+    const float* ds = reinterpret_cast<const float*>(smem + 4 * L::TILE + (2 + buf) * L::STAT);
+#pragma unroll
+    for (int b = 0; b < NRB; ++b) {
+      at_f16 s = (at_f16)(0.0f);
+#pragma unroll
+      for (int st = 0; st < R::STEPS; ++st) s = at_mma(T(), at.rows(qs, 32 * b, st), kf[st], s);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const at_f4 l4 = *reinterpret_cast<const at_f4*>(ls + 32 * b + 8 * x + 4 * h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[4 * x + i] = __builtin_amdgcn_exp2f(s[4 * x + i] * a.scale_log2 - (l4[i] - AT_P_LIFT<T>));
+      }
+      if constexpr (DO_V) at_mma_cols<T, DC>(at, gs, 32 * b, s, accv);
+      if constexpr (DO_K) {
+        at_f16 dp = (at_f16)(0.0f);
+#pragma unroll
+        for (int st = 0; st < R::STEPS; ++st) dp = at_mma(T(), at.rows(gs, 32 * b, st), vf[st], dp);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const at_f4 d4 = *reinterpret_cast<const at_f4*>(ds + 32 * b + 8 * x + 4 * h);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[4 * x + i] *= dp[4 * x + i] - d4[i];
         }
+        fit.template fit<NDB>(s, acck);
+        at_mma_cols<T, DC>(at, qs, 32 * b, s, acck);
       }
     }
   }
-  if (!live) return;
+  // a key that takes no part has a column of its own, whatever it holds: it is not written
+  const float unlift = at_fit<T>::ON ? 1.0f / 4096.0f : 1.0f;
+  const float fk = a.scale * fit.undo() * unlift, fv = unlift;
+  const int64_t o = (((int64_t)n * a.Tk + key) * a.Hk + hk) * a.D;
+  if (!takes) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < a.D) {
-      dk[row * a.D + lane + 64 * i] = rc_from_float<T>(ak[i] * a.scale);
-      dv[row * a.D + lane + 64 * i] = rc_from_float<T>(av[i]);
+    for (int i = 0; i < NDB; ++i) {
+      if constexpr (DO_K) acck[i] = (at_f16)(0.0f);
+      if constexpr (DO_V) accv[i] = (at_f16)(0.0f);
     }
+  }
+  if (sp.n > 1) {
+    float* p = sp.p + (int64_t)split * 2 * sp.part + o;
+    if constexpr (DO_K) at_store_rows<float, DC>(p, live, acck, fk, a.D, lane);
+    if constexpr (DO_V) at_store_rows<float, DC>(p + sp.part, live, accv, fv, a.D, lane);
+  } else {
+    if constexpr (DO_K) at_store_rows<T, DC>(dk + o, live, acck, fk, a.D, lane);
+    if constexpr (DO_V) at_store_rows<T, DC>(dv + o, live, accv, fv, a.D, lane);
+  }
 }
 
-int64_t at_blocks(int64_t rows) { return (rows + AT_WAVES - 1) / AT_WAVES; }
-
+// The splits' parts, added in their order; four elements per thread.
 template <typename T>
-int at_bwd(const rc_attn* a, const void* q, const void* k, const void* v, const void* out, const float* lse,
-           const void* dout, void* dq, void* dk, void* dv, void* work, hipStream_t st) {
-  const at_args d = at_to_dev(a, work);
-  float* delta = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + at_bits_bytes(a));
-  const int64_t rows = a->N * a->Tq * a->Hq, keys = a->N * a->Tk * a->Hk;
-  if (rows) {  // (the gradients of keys and values need delta too)
-    at_delta_kernel<T><<<at_blocks(rows), AT_WAVES * 64, 0, st>>>((const T*)out, (const T*)dout, delta, d);
-    if (dq) at_dq_kernel<T><<<at_blocks(rows), AT_WAVES * 64, 0, st>>>((const T*)q, (const T*)k, (const T*)v, (const T*)dout, lse,
-                                                               delta, (T*)dq, d);
+__global__ __launch_bounds__(256) void at_add_kernel(const float* __restrict__ p, int64_t stride, int n, T* __restrict__ out,
+                                                     int64_t quads) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= quads) return;
+  at_f4 s = *reinterpret_cast<const at_f4*>(p + 4 * i);
+  for (int x = 1; x < n; ++x) s += *reinterpret_cast<const at_f4*>(p + x * stride + 4 * i);
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  t4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = rc_from_float<T>(s[e]);
+  *reinterpret_cast<t4*>(out + 4 * i) = o;
+}
+
+// What a call of these sizes needs: splits where there are too few work items, and the scratch of their parts.
+struct at_bwd_plan {
+  int64_t q_tiles, k_tiles, q_items, k_items;
+  int q_splits, k_splits, q_per;
+  int64_t bits, delta, parts;  // bytes
+};
+
+constexpr int AT_TILE_ROWS = 128;  // query rows, or keys, of a work item
+constexpr int AT_Q_TILE = 32;      // smallest tile of query rows in at_dkv_kernel
+constexpr int64_t AT_FILL = 512;   // work items that fill the card twice
+
+at_bwd_plan at_make_bwd_plan(const rc_attn* a) {
+  at_bwd_plan p = {};
+  const int64_t rows = a->Tq * (a->Hq / a->Hk), groups = a->N * a->Hk;
+  p.q_tiles = (rows + AT_TILE_ROWS - 1) / AT_TILE_ROWS;
+  p.k_tiles = (a->Tk + AT_TILE_ROWS - 1) / AT_TILE_ROWS;
+  p.q_items = groups * p.q_tiles;
+  p.k_items = groups * p.k_tiles;
+  auto splits = [](int64_t items, int64_t most) {
+    if (items == 0 || items >= AT_FILL) return 1;
+    const int64_t n = (AT_FILL + items - 1) / items;
+    return (int)(n < most ? n : most < 1 ? 1 : most);
+  };
+  // a split has 512 keys at least, or 512 query rows
+  const int qs = splits(p.q_items, a->Tk / 512);
+  p.q_per = (int)(((a->Tk + qs - 1) / qs + 63) / 64 * 64);
+  if (p.q_per < 64) p.q_per = 64;
+  p.q_splits = a->Tk ? (int)((a->Tk + p.q_per - 1) / p.q_per) : 1;
+  p.k_splits = splits(p.k_items, rows / 512);
+  p.bits = at_bits_bytes(a);
+  p.delta = (a->N * a->Tq * a->Hq * 4 + 255) / 256 * 256;
+  const int64_t pq = p.q_splits > 1 ? (int64_t)p.q_splits * a->N * a->Tq * a->Hq * a->D * 4 : 0;
+  const int64_t pk = p.k_splits > 1 ? (int64_t)p.k_splits * 2 * a->N * a->Tk * a->Hk * a->D * 4 : 0;
+  p.parts = pq > pk ? pq : pk;  // one after the other
+  return p;
+}
+
+template <typename K> int at_allow_lds(K kernel, int bytes) {
+  if (bytes <= 64 * 1024) return RC_OK;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == hipSuccess) return RC_OK;
+  rc_set_error("rc_cross_attn_bwd: %d bytes of LDS refused: %s", bytes, hipGetErrorString(e));
+  return (int)e;
+}
+
+struct at_bwd_call {
+  const rc_attn* a;
+  at_args d;
+  at_bwd_plan p;
+  const void *q, *k, *v, *out, *dout;
+  const float* lse;
+  void *dq, *dk, *dv;
+  float *delta, *parts;
+  hipStream_t st;
+};
+
+template <typename T, int DC, int NRB, bool DO_K, bool DO_V, int OCC> int at_launch_dkv(const at_bwd_call& c) {
+  constexpr int RT = 32 * NRB;
+  using L = at_dkv_lds<T, DC, RT>;
+  static_assert(L::BYTES <= 160 * 1024, "LDS");
+  auto kernel = at_dkv_kernel<T, DC, 4, NRB, DO_K, DO_V, OCC>;
+  int rc = at_allow_lds(kernel, L::BYTES);
+  if (rc) return rc;
+  const int64_t row_tiles = (c.a->Tq + RT - 1) / RT, all = row_tiles * c.d.G;
+  at_parts sp = {};
+  sp.per = (int)((all + c.p.k_splits - 1) / c.p.k_splits);
+  if (sp.per < 1) sp.per = 1;
+  sp.n = c.p.k_splits;
+  sp.p = c.parts;
+  sp.part = c.a->N * c.a->Tk * c.a->Hk * c.a->D;
+  const int64_t items = c.p.k_items * sp.n;
+  kernel<<<at_grid(items), 256, L::BYTES, c.st>>>((const T*)c.q, (const T*)c.k, (const T*)c.v, c.lse, (const T*)c.dout, c.delta,
+                                                  (T*)c.dk, (T*)c.dv, sp, c.d, (int)c.p.k_tiles, (int)row_tiles, items);
+  return rc_check_launch("rc_cross_attn_bwd (keys)");
+}
+
+template <typename T> int at_add(const at_bwd_call& c, int64_t offset, int64_t stride, int n, void* out, int64_t elems) {
+  at_add_kernel<T><<<(uint32_t)((elems / 4 + 255) / 256), 256, 0, c.st>>>(c.parts + offset, stride, n, (T*)out, elems / 4);
+  return rc_check_launch("rc_cross_attn_bwd (parts)");
+}
+
+template <typename T, int DC> int at_bwd(const at_bwd_call& c) {
+  // tiles and resident workgroups: what registers (512 per lane and SIMD) and 160 KiB of LDS allow
+  constexpr int RB = at_row<T, DC>::RB;
+  constexpr int NB = RB >= 512 ? 1 : 2;
+  constexpr int OCC = RB >= 512 ? 1 : 2;
+  constexpr int KOCC = DC * sizeof(T) <= 128 ? 2 : 1;
+  int rc = RC_OK;
+  if (c.p.q_items) {  // (the gradients of keys and values need delta)
+    constexpr int bytes = at_dq_lds<T, DC, 32 * NB, 4>::BYTES;
+    static_assert(bytes <= 160 * 1024, "LDS");
+    auto kernel = at_dq_kernel<T, DC, 4, NB, OCC>;
+    if ((rc = at_allow_lds(kernel, bytes))) return rc;
+    at_parts sp = {};
+    sp.n = c.p.q_splits;
+    sp.per = c.p.q_per;
+    sp.p = c.parts;
+    sp.part = c.a->N * c.a->Tq * c.a->Hq * c.a->D;
+    const int64_t items = c.p.q_items * sp.n;
+    kernel<<<at_grid(items), 256, bytes, c.st>>>((const T*)c.q, (const T*)c.k, (const T*)c.v, (const T*)c.out, c.lse,
+                                                 (const T*)c.dout, c.delta, (T*)c.dq, sp, c.d, (int)c.p.q_tiles, items);
+    if ((rc = rc_check_launch("rc_cross_attn_bwd (queries)"))) return rc;
+    if (c.dq && sp.n > 1 && (rc = at_add<T>(c, 0, sp.part, sp.n, c.dq, sp.part))) return rc;
   }
-  if (keys && dk)
-    at_dkv_kernel<T><<<at_blocks(keys), AT_WAVES * 64, 0, st>>>((const T*)q, (const T*)k, (const T*)v, (const T*)dout,
-                                                                lse, delta, (T*)dk, (T*)dv, d);
-  return rc_check_launch("rc_cross_attn_bwd");
+  if (!c.dk || !c.p.k_items) return RC_OK;
+  // wide heads in fp32, and in fp16 with its scaling: registers for one of the two at a time
+  if constexpr (RB >= 1024 || (at_fit<T>::ON && DC > 128)) {
+    if ((rc = at_launch_dkv<T, DC, 1, true, false, 1>(c))) return rc;
+    if ((rc = at_launch_dkv<T, DC, 1, false, true, 1>(c))) return rc;
+  } else {
+    if ((rc = at_launch_dkv<T, DC, NB, true, true, KOCC>(c))) return rc;
+  }
+  if (c.p.k_splits > 1) {
+    const int64_t part = c.a->N * c.a->Tk * c.a->Hk * c.a->D;
+    if ((rc = at_add<T>(c, 0, 2 * part, c.p.k_splits, c.dk, part))) return rc;
+    if ((rc = at_add<T>(c, part, 2 * part, c.p.k_splits, c.dv, part))) return rc;
+  }
+  return RC_OK;
+}
+
+template <typename T> int at_bwd_d(const at_bwd_call& c) {
+  const int D = c.a->D;
+  if (D <= 32) return at_bwd<T, 32>(c);
+  if (D <= 64) return at_bwd<T, 64>(c);
+  if (D <= 96) return at_bwd<T, 96>(c);
+  if (D <= 128) return at_bwd<T, 128>(c);
+  if (D <= 192) return at_bwd<T, 192>(c);
+  return at_bwd<T, 256>(c);
 }
 
 }  // namespace
@@ -173,7 +446,8 @@ int at_bwd(const rc_attn* a, const void* q, const void* k, const void* v, const 
 extern "C" int64_t rc_cross_attn_bwd_work_bytes(const rc_attn* a) {
   const int rc = at_check(a);
   if (rc) return rc < 0 ? rc : RC_EINVAL;
-  return at_bits_bytes(a) + a->N * a->Tq * a->Hq * (int64_t)sizeof(float);
+  const at_bwd_plan p = at_make_bwd_plan(a);
+  return p.bits + p.delta + p.parts;
 }
 
 extern "C" int rc_cross_attn_bwd(const rc_attn* a, const void* q, const void* k, const void* v, const void* out,
@@ -185,14 +459,33 @@ extern "C" int rc_cross_attn_bwd(const rc_attn* a, const void* q, const void* k,
     if ((rc = at_check_operand(a, a->N * a->Tq, p))) return rc;
   for (const void* p : {k, v})
     if ((rc = at_check_operand(a, a->N * a->Tk, p))) return rc;
-  RC_REQUIRE(at_bits_bytes(a) == 0 || (work != nullptr && (uintptr_t)work % 16 == 0), RC_EINVAL,
-             "rc_cross_attn_bwd: work is null or not aligned to 16 bytes");
   RC_REQUIRE((dk == nullptr) == (dv == nullptr), RC_EINVAL, "rc_cross_attn_bwd: dk and dv are wanted together or not at all");
   RC_REQUIRE(((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0, RC_EINVAL,
              "rc_cross_attn_bwd: a gradient is not aligned to 16 bytes");
   if (a->N == 0) return RC_OK;
-  if ((rc = at_launch_bits(a, work, (hipStream_t)stream))) return rc;
-  if (a->dtype == RC_F32) return at_bwd<float>(a, q, k, v, out, lse, dout, dq, dk, dv, work, (hipStream_t)stream);
-  if (a->dtype == RC_F16) return at_bwd<rc_half>(a, q, k, v, out, lse, dout, dq, dk, dv, work, (hipStream_t)stream);
-  return at_bwd<rc_bf16>(a, q, k, v, out, lse, dout, dq, dk, dv, work, (hipStream_t)stream);
+  at_bwd_call c = {};
+  c.a = a;
+  c.p = at_make_bwd_plan(a);
+  RC_REQUIRE(c.p.bits == 0 || (work != nullptr && (uintptr_t)work % 16 == 0), RC_EINVAL,
+             "rc_cross_attn_bwd: work is null or not aligned to 16 bytes");
+  RC_REQUIRE(c.p.q_items * c.p.q_splits < (1ll << 31) - 8 && c.p.k_items * c.p.k_splits < (1ll << 31) - 8 &&
+                 a->N * a->Tq * a->Hq * a->D / 4 < (1ll << 39) && a->N * a->Tk * a->Hk * a->D / 4 < (1ll << 39),
+             RC_EINVAL, "rc_cross_attn_bwd: too many rows");
+  c.q = q;
+  c.k = k;
+  c.v = v;
+  c.out = out;
+  c.dout = dout;
+  c.lse = lse;
+  c.dq = dq;
+  c.dk = dk;
+  c.dv = dv;
+  c.delta = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + c.p.bits);
+  c.parts = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + c.p.bits + c.p.delta);
+  c.st = (hipStream_t)stream;
+  c.d = at_to_dev(a, work);
+  if ((rc = at_launch_bits(a, work, c.st))) return rc;
+  if (a->dtype == RC_F32) return at_bwd_d<float>(c);
+  if (a->dtype == RC_F16) return at_bwd_d<rc_half>(c);
+  return at_bwd_d<rc_bf16>(c);
 }

@@ -55,9 +55,10 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wq = wave % NWQ, wk = wave / NWQ;
   const int c = lane & 31, h = lane >> 5;
-  const int rows = a.Tq * a.G, row = (rt * NWQ + wq) * 32 + c;
+  const int rows = a.Tq * a.G, row0 = (rt * NWQ + wq) * 32, row = row0 + c;
   const bool live = row < rows;
-  const int t = (live ? row : 0) / a.G, g = (live ? row : 0) - t * a.G;
+  const int first = min(row0 / a.G, a.Tq - 1);  // the wave's first token
+  const int t = live ? row / a.G : first, g = live ? row - t * a.G : 0;
 
   const int len = at_length(a, n);
   const int k_begin = split * sp.keys, k_end = min(len, k_begin + sp.keys);
@@ -69,7 +70,10 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
   if (tiles > 0) kv.fetch(a, lds0, lds0 + 2 * C::TILE, wave, lane);
 
   at_u4 qf[R::STEPS];
-  at_load_row<T, DC>(q + (int64_t)n * a.qs[0] + (int64_t)t * a.qs[1] + (int64_t)(hk * a.G + g) * a.qs[2], live, a.D, lane, qf);
+  at_rows_of(q + (int64_t)n * a.qs[0] + (int64_t)first * a.qs[1] + (int64_t)hk * a.G * a.qs[2])
+      .row<T, DC>(live ? (uint32_t)(t - first) * (uint32_t)(a.qs[1] * sizeof(T)) + (uint32_t)g * (uint32_t)(a.qs[2] * sizeof(T))
+                       : AT_OUTSIDE,
+                  a.D, lane, qf);
 
   at_places<T, DC> at;
   at.init(lane);
@@ -363,6 +367,9 @@ int at_check(const rc_attn* a) {
       RC_REQUIRE(st[o][i] >= 0 && st[o][i] * es % 16 == 0 && (i == 0 || st[o][i] * es < (1ll << 24)), RC_EINVAL,
                  "rc_cross_attn: stride %lld of %c is negative, no multiple of 16 bytes, or 16 MiB or more between tokens "
                  "or heads", (long long)st[o][i], "qkv"[o]);
+  RC_REQUIRE((int64_t)a->Hq * a->q_stride[2] * es < (1ll << 30), RC_EINVAL,
+             "rc_cross_attn: the heads of a query token span 1 GiB or more");
+  RC_REQUIRE((int64_t)a->Hq * a->D * es < (1ll << 24), RC_EINVAL, "rc_cross_attn: a query token of 16 MiB or more");
   RC_REQUIRE(a->key_mask == nullptr || a->mask_stride >= 0, RC_EINVAL, "rc_cross_attn: negative mask stride");
   return RC_OK;
 }
