@@ -201,11 +201,7 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
     }
     return;
   }
-  const float f = any ? 1.0f / l : 0.0f;
-  if (!any) {
-#pragma unroll
-    for (int i = 0; i < NDB; ++i) acc[i] = (at_f16)(0.0f);
-  }
+  const float f = any ? 1.0f / l : 0.0f;  // (without a key the sums are 0)
   const int hq = hk * a.G + g;
   T* o = out + ((int64_t)((int64_t)n * a.Tq + t) * a.Hq + hq) * a.D;
   if constexpr (NWK == 1) {
@@ -328,7 +324,7 @@ int at_run(const rc_attn* a, const at_args& d, const void* q, const void* k, con
   constexpr int RB = at_row<T, DC>::RB;
   constexpr int NWK = RB >= 1024 ? 1 : RB >= 512 ? 2 : 4;
   constexpr int NKB = RB >= 512 ? 1 : 2;
-  constexpr int OCC = RB >= 512 && DC > 128 ? (DC == 192 && RB < 1024 ? 2 : 1) : RB >= 1024 ? 1 : DC * (int)sizeof(T) >= 192 ? 2 : 3;
+  constexpr int OCC = RB >= 1024 ? 1 : DC * (int)sizeof(T) >= 192 ? 2 : 3;
   if (p.few) return at_launch<T, DC, 1, NWK, 1, 1>(a, d, q, k, v, out, lse, p.sp, st);
   return at_launch<T, DC, 4, 1, NKB, OCC>(a, d, q, k, v, out, lse, p.sp, st);
 }
