@@ -27,12 +27,24 @@ typedef _Float16 at_h2 __attribute__((ext_vector_type(2)));
 typedef __bf16 at_b8 __attribute__((ext_vector_type(8)));
 typedef __bf16 at_b2 __attribute__((ext_vector_type(2)));
 
+// n / d for 0 <= n < 2^31 by one multiplication: m = ceil(2^(31 + s) / d), s = ceil(log2 d).
+struct at_div {
+  uint32_t m, s, d;
+  __host__ at_div() : m(0), s(0), d(0) {}
+  __host__ explicit at_div(uint32_t by) : s(0), d(by) {
+    while (s < 31 && (1u << s) < d) ++s;
+    m = (uint32_t)(((1ull << (31 + s)) + d - 1) / (d ? d : 1));
+  }
+  __device__ __forceinline__ int of(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n, m) >> (s - 1)); }
+};
+
 struct at_args {
   int64_t qs[3], ks[3], vs[3];  // elements between sequences, tokens, heads
   const void* lengths;
   const uint64_t* bits;  // [N][words], bit t % 64 of word t / 64: key t takes part; NULL: the lengths say it
   int64_t words;
   int32_t N, Tq, Tk, Hq, Hk, G, D;
+  at_div by_Hk, by_G;
   int32_t lengths_i64;
   float scale, scale_log2;
 };
@@ -61,8 +73,10 @@ __device__ __forceinline__ uint32_t at_first_bits(int left) {
 __device__ __forceinline__ uint32_t at_key_bits(const at_args& a, int n, int len, int k0) {
   const int left = len - k0;
   uint32_t w = at_first_bits(left);
+  // (the address is the same for the whole wave and nothing writes there: a scalar load, which does not wait behind the
+  // tiles' loads)
   if (a.bits != nullptr && left > 0)
-    w &= reinterpret_cast<const uint32_t*>(a.bits)[((int64_t)n * a.words) * 2 + (k0 >> 5)];
+    w &= reinterpret_cast<const uint32_t __attribute__((address_space(4)))*>((uint64_t)a.bits)[((int64_t)n * a.words) * 2 + (k0 >> 5)];
   return __builtin_amdgcn_readfirstlane(w);
 }
 
@@ -80,6 +94,25 @@ __device__ __forceinline__ at_f16 at_mma(float, at_u4 a, at_u4 b, at_f16 c) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
   return c;
+}
+
+// What a block of 32 keys' scores start from: 0, or -inf for the keys whose bit in `take` is not set (the same for the
+// whole wave).  The mask costs a select and a product of one column by one row: -inf or 0 of this lane's key by 1.
+template <typename T> __device__ __forceinline__ at_f16 at_start(uint32_t take, int lane) {
+  at_f16 s = (at_f16)(0.0f);
+  if (take != 0xffffffffu) {
+    const bool out = lane < 32 && !((take >> lane) & 1);
+    const uint32_t inf = sizeof(T) == 4 ? 0xff800000u : __is_same(T, rc_half) ? 0xfc00u : 0xff80u;
+    const uint32_t one = sizeof(T) == 4 ? 0x3f800000u : __is_same(T, rc_half) ? 0x3c00u : 0x3f80u;
+    const at_u4 x = {out ? inf : 0u, 0u, 0u, 0u}, y = {lane < 32 ? one : 0u, 0u, 0u, 0u};
+    if constexpr (sizeof(T) == 4) {
+      const at_f4 u = __builtin_bit_cast(at_f4, x), w = __builtin_bit_cast(at_f4, y);
+      s = __builtin_amdgcn_mfma_f32_32x32x2f32(u[0], w[0], s, 0, 0, 0);
+    } else {
+      s = at_mma(T(), x, y, s);
+    }
+  }
+  return s;
 }
 
 // products of 16 bytes of elements, summed in fp32
@@ -337,10 +370,10 @@ __device__ __forceinline__ void at_fetch_floats(const float* base, int left, uin
 
 // Block id -> work item: ids go round the 8 XCDs, items that share keys should share an XCD's L2, so each XCD gets a
 // run of consecutive items.  The grid has at_grid() blocks.
-__device__ __forceinline__ int64_t at_item(int64_t items) {
-  const int64_t per = (items + 7) / 8;
-  const int64_t i = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  return (blockIdx.x >> 3) < per && i < items ? i : -1;
+__device__ __forceinline__ int at_item(int items) {
+  const uint32_t per = ((uint32_t)items + 7) / 8, x = blockIdx.x >> 3;
+  const uint32_t i = (blockIdx.x & 7) * per + x;
+  return x < per && i < (uint32_t)items ? (int)i : -1;
 }
 static inline uint32_t at_grid(int64_t items) { return (uint32_t)((items + 7) / 8 * 8); }
 

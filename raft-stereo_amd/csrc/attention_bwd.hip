@@ -60,23 +60,22 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dq_kernel(const T* __restrict
                                                              const T* __restrict__ v, const T* __restrict__ out,
                                                              const float* __restrict__ lse, const T* __restrict__ dout,
                                                              float* __restrict__ delta, T* __restrict__ dq, at_parts sp,
-                                                             at_args a, int row_tiles, int64_t items) {
+                                                             at_args a, at_div by_tiles, at_div by_splits, int items) {
   using R = at_row<T, DC>;
   constexpr int NDB = DC / 32, KT = 32 * NKB;
   constexpr int TILE = at_dq_lds<T, DC, KT, NW>::TILE;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  const int64_t item = at_item(items);
+  const int item = at_item(items);
   if (item < 0) return;
-  const int rt = (int)(item % row_tiles);
-  const int64_t rest = item / row_tiles;
-  const int split = (int)(rest % sp.n), nh = (int)(rest / sp.n);
-  const int n = nh / a.Hk, hk = nh - n * a.Hk;
+  const int rest = by_tiles.of(item), rt = item - rest * (int)by_tiles.d;
+  const int nh = by_splits.of(rest), split = rest - nh * (int)by_splits.d;
+  const int n = a.by_Hk.of(nh), hk = nh - n * a.Hk;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c = lane & 31, h = lane >> 5;
   const int row0 = (rt * NW + wave) * 32, row = row0 + c;
   const bool live = row < a.Tq * a.G;
-  const int first = min(row0 / a.G, a.Tq - 1);  // the wave's first token
-  const int t = live ? row / a.G : first, g = live ? row - t * a.G : 0, hq = hk * a.G + g;
+  const int first = min(a.by_G.of(row0), a.Tq - 1);  // the wave's first token
+  const int t = live ? a.by_G.of(row) : first, g = live ? row - t * a.G : 0, hq = hk * a.G + g;
 
   const int len = at_length(a, n);
   const int k_begin = split * sp.per, k_end = min(len, k_begin + sp.per);
@@ -119,9 +118,11 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dq_kernel(const T* __restrict
     if (j + 1 < tiles) kv.fetch(a, lds0 + ((j + 1) & 1) * TILE, lds0 + (2 + ((j + 1) & 1)) * TILE, wave, lane);
     const unsigned char* kt = smem + (j & 1) * TILE;
     const unsigned char* vt = smem + (2 + (j & 1)) * TILE;
+    if (DC <= 64 && row0 >= a.Tq * a.G) continue;  // (this wave only helps with the loads)
 #pragma unroll
     for (int b = 0; b < NKB; ++b) {
-      at_f16 s = (at_f16)(0.0f), dp = (at_f16)(0.0f);
+      // (a key that takes no part has the score -inf, so P = 0, and zeros for its value, so dP = 0)
+      at_f16 s = at_start<T>(at_key_bits(a, n, k_end, k_begin + j * KT + 32 * b), lane), dp = (at_f16)(0.0f);
 #pragma unroll
       for (int st = 0; st < R::STEPS; ++st) {
         s = at_mma(T(), at.rows(kt, 32 * b, st), qf[st], s);
@@ -130,12 +131,6 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dq_kernel(const T* __restrict
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * a.scale_log2 - ls) * (dp[i] - dl);
-      uint32_t w = at_key_bits(a, n, k_end, k_begin + j * KT + 32 * b);
-      if (w != 0xffffffffu) {
-        w >>= 4 * h;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = (w >> (8 * (i / 4) + i % 4)) & 1 ? s[i] : 0.0f;
-      }
       fit.template fit<NDB>(s, acc);
       at_mma_cols<T, DC>(at, kt, 32 * b, s, acc);
     }
@@ -185,17 +180,16 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dkv_kernel(const T* __restric
                                                               const T* __restrict__ v, const float* __restrict__ lse,
                                                               const T* __restrict__ dout, const float* __restrict__ delta,
                                                               T* __restrict__ dk, T* __restrict__ dv, at_parts sp, at_args a,
-                                                              int key_tiles, int row_tiles, int64_t items) {
+                                                              at_div by_tiles, at_div by_splits, at_div by_rows, int items) {
   using R = at_row<T, DC>;
   constexpr int NDB = DC / 32, RT = 32 * NRB;
   using L = at_dkv_lds<T, DC, RT>;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  const int64_t item = at_item(items);
+  const int item = at_item(items);
   if (item < 0) return;
-  const int kt = (int)(item % key_tiles);
-  const int64_t rest = item / key_tiles;
-  const int split = (int)(rest % sp.n), nh = (int)(rest / sp.n);
-  const int n = nh / a.Hk, hk = nh - n * a.Hk;
+  const int rest = by_tiles.of(item), kt = item - rest * (int)by_tiles.d;
+  const int nh = by_splits.of(rest), split = rest - nh * (int)by_splits.d;
+  const int n = a.by_Hk.of(nh), hk = nh - n * a.Hk, row_tiles = (int)by_rows.d;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c = lane & 31, h = lane >> 5;
   const int key0 = (kt * NW + wave) * 32, key = key0 + c;
@@ -212,7 +206,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dkv_kernel(const T* __restric
   const uint32_t stat0 = lds0 + 4 * L::TILE;
   at_query_tiles<T, DC, RT, NW> qt;
   qt.init(a, wave, lane);
-  int g = row_tiles ? begin / row_tiles : 0, t0 = (begin - g * row_tiles) * RT;  // of the tile that is fetched next
+  int g = row_tiles ? by_rows.of(begin) : 0, t0 = (begin - g * row_tiles) * RT;  // of the tile that is fetched next
   auto fetch = [&](int buf) {
     qt.fetch(a, q, dout, lse, delta, n, hk * a.G + g, t0, lds0 + buf * L::TILE, lds0 + (2 + buf) * L::TILE, stat0 + buf * L::STAT,
              stat0 + (2 + buf) * L::STAT, wave, lane);
@@ -248,6 +242,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dkv_kernel(const T* __restric
     const unsigned char* gs = smem + (2 + buf) * L::TILE;
     const float* ls = reinterpret_cast<const float*>(smem + 4 * L::TILE + buf * L::STAT);
     const float* ds = reinterpret_cast<const float*>(smem + 4 * L::TILE + (2 + buf) * L::STAT);
+    if (DC <= 64 && mine == 0) continue;  // (none of this wave's keys takes part: it only helps with the loads)
 #pragma unroll
     for (int b = 0; b < NRB; ++b) {
       at_f16 s = (at_f16)(0.0f);
@@ -383,7 +378,8 @@ template <typename T, int DC, int NRB, bool DO_K, bool DO_V, int OCC> int at_lau
   sp.part = c.a->N * c.a->Tk * c.a->Hk * c.a->D;
   const int64_t items = c.p.k_items * sp.n;
   kernel<<<at_grid(items), 256, L::BYTES, c.st>>>((const T*)c.q, (const T*)c.k, (const T*)c.v, c.lse, (const T*)c.dout, c.delta,
-                                                  (T*)c.dk, (T*)c.dv, sp, c.d, (int)c.p.k_tiles, (int)row_tiles, items);
+                                                  (T*)c.dk, (T*)c.dv, sp, c.d, at_div((uint32_t)c.p.k_tiles),
+                                                  at_div((uint32_t)sp.n), at_div((uint32_t)row_tiles), (int)items);
   return rc_check_launch("rc_cross_attn_bwd (keys)");
 }
 
@@ -411,7 +407,8 @@ template <typename T, int DC> int at_bwd(const at_bwd_call& c) {
     sp.part = c.a->N * c.a->Tq * c.a->Hq * c.a->D;
     const int64_t items = c.p.q_items * sp.n;
     kernel<<<at_grid(items), 256, bytes, c.st>>>((const T*)c.q, (const T*)c.k, (const T*)c.v, (const T*)c.out, c.lse,
-                                                 (const T*)c.dout, c.delta, (T*)c.dq, sp, c.d, (int)c.p.q_tiles, items);
+                                                 (const T*)c.dout, c.delta, (T*)c.dq, sp, c.d, at_div((uint32_t)c.p.q_tiles),
+                                                 at_div((uint32_t)sp.n), (int)items);
     if ((rc = rc_check_launch("rc_cross_attn_bwd (queries)"))) return rc;
     if (c.dq && sp.n > 1 && (rc = at_add<T>(c, 0, sp.part, sp.n, c.dq, sp.part))) return rc;
   }

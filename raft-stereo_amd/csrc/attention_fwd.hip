@@ -38,27 +38,25 @@ template <typename T, int DC, int NWQ, int NWK, int NKB, int OCC>
 __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                                      const T* __restrict__ v, T* __restrict__ out,
                                                                      float* __restrict__ lse, at_split sp, at_args a,
-                                                                     int row_tiles, int64_t items) {
+                                                                     at_div by_tiles, at_div by_splits, int items) {
   using C = at_fwd_cfg<T, DC, NWQ, NWK, NKB>;
   using R = at_row<T, DC>;
   constexpr int NDB = DC / 32;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  const int64_t item = at_item(items);
+  const int item = at_item(items);
   if (item < 0) return;
   // rows fastest, then splits, then heads and sequences: neighbours share keys
-  const int rt = (int)(item % row_tiles);
-  const int64_t rest = item / row_tiles;
-  const int split = (int)(rest % sp.n);
-  const int nh = (int)(rest / sp.n);
-  const int n = nh / a.Hk, hk = nh - n * a.Hk;
+  const int rest = by_tiles.of(item), rt = item - rest * (int)by_tiles.d;
+  const int nh = by_splits.of(rest), split = rest - nh * (int)by_splits.d;
+  const int n = a.by_Hk.of(nh), hk = nh - n * a.Hk;
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wq = wave % NWQ, wk = wave / NWQ;
   const int c = lane & 31, h = lane >> 5;
   const int rows = a.Tq * a.G, row0 = (rt * NWQ + wq) * 32, row = row0 + c;
   const bool live = row < rows;
-  const int first = min(row0 / a.G, a.Tq - 1);  // the wave's first token
-  const int t = live ? row / a.G : first, g = live ? row - t * a.G : 0;
+  const int first = min(a.by_G.of(row0), a.Tq - 1);  // the wave's first token
+  const int t = live ? a.by_G.of(row) : first, g = live ? row - t * a.G : 0;
 
   const int len = at_length(a, n);
   const int k_begin = split * sp.keys, k_end = min(len, k_begin + sp.keys);
@@ -90,25 +88,19 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
     const unsigned char* vt = smem + (2 + (j & 1)) * C::TILE;
     const int kr = 32 * NKB * wk;  // this wave's first key of the tile
 
+    if (row0 >= rows) continue;  // (this wave only helps with the loads)
+
     at_f16 s[NKB];
 #pragma unroll
-    for (int b = 0; b < NKB; ++b) s[b] = (at_f16)(0.0f);
+    for (int b = 0; b < NKB; ++b) {
+      const uint32_t take = at_key_bits(a, n, k_end, k_begin + j * C::KT + kr + 32 * b);
+      any |= take;
+      s[b] = at_start<T>(take, lane);
+    }
 #pragma unroll
     for (int st = 0; st < R::STEPS; ++st)
 #pragma unroll
-      for (int b = 0; b < NKB; ++b)
-        s[b] = at_mma(T(), at.rows(kt, kr + 32 * b, st), qf[st], s[b]);
-
-#pragma unroll
-    for (int b = 0; b < NKB; ++b) {
-      uint32_t w = at_key_bits(a, n, k_end, k_begin + j * C::KT + kr + 32 * b);
-      any |= w;
-      if (w != 0xffffffffu) {
-        w >>= 4 * h;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[b][i] = (w >> (8 * (i / 4) + i % 4)) & 1 ? s[b][i] : -INFINITY;
-      }
-    }
+      for (int b = 0; b < NKB; ++b) s[b] = at_mma(T(), at.rows(kt, kr + 32 * b, st), qf[st], s[b]);
     float mx = s[0][0];
 #pragma unroll
     for (int b = 0; b < NKB; ++b)
@@ -183,12 +175,12 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
   if (sp.n > 1) {
     // no key at all: sum 0; keys, but every score -inf: NaN, as 0 / 0 is
     l = any ? (l == 0.0f ? NAN : l) : 0.0f;
-    float* ml = sp.ml + item * 2 * C::ROWS + wq * 32;
+    float* ml = sp.ml + (int64_t)item * 2 * C::ROWS + wq * 32;
     if (wk == 0 && h == 0) {
       ml[c] = m;
       ml[C::ROWS + c] = l;
     }
-    float* o = sp.o + (item * C::ROWS + wq * 32 + c) * a.D;
+    float* o = sp.o + ((int64_t)item * C::ROWS + wq * 32 + c) * a.D;
 #pragma unroll
     for (int i = 0; i < NDB; ++i) {
       if (NWK > 1 && i % NWK != wk) continue;
@@ -277,7 +269,7 @@ int at_launch(const rc_attn* a, const at_args& d, const void* q, const void* k, 
   const int64_t rows = a->Tq * d.G, row_tiles = (rows + C::ROWS - 1) / C::ROWS;
   const int64_t items = a->N * a->Hk * sp.n * row_tiles;
   kernel<<<at_grid(items), 64 * C::WAVES, lds, st>>>((const T*)q, (const T*)k, (const T*)v, (T*)out, lse, sp, d,
-                                                     (int)row_tiles, items);
+                                                     at_div((uint32_t)row_tiles), at_div((uint32_t)sp.n), (int)items);
   int rc = rc_check_launch("rc_cross_attn_fwd");
   if (rc || sp.n == 1) return rc;
   const int64_t all = a->N * a->Hk * rows;
@@ -393,6 +385,8 @@ at_args at_to_dev(const rc_attn* a, void* bits) {
   d.Hk = a->Hk;
   d.G = a->Hq / a->Hk;
   d.D = a->D;
+  d.by_Hk = at_div((uint32_t)d.Hk);
+  d.by_G = at_div((uint32_t)d.G);
   d.lengths_i64 = a->lengths_i64;
   d.scale = a->scale;
   d.scale_log2 = a->scale * 1.44269504088896340736f;
