@@ -1,10 +1,11 @@
 // What the attention kernels share: arguments, the matrix-instruction fragments, and the staging of tiles of rows.
 //
 // A tile is a number of rows (tokens of one head) in LDS, RB bytes each (the head padded with zeros to a power of
-// two), cut into 16-byte chunks.  Chunk c of row r lies at r * RB + ((c ^ f(r)) << 4).  f is chosen so that both ways
-// of reading a tile are free of bank conflicts: eight lanes that read the same chunk of eight consecutive rows (a
-// fragment whose reduction runs along the row) and sixteen lanes that read 32 bytes each of four consecutive rows (the
-// transposing read, a fragment whose reduction runs across rows).
+// two), cut into 16-byte chunks.  Chunk c of row r lies at r * RB + ((c ^ f(r)) << 4).  LDS has 64 banks, 256 bytes a
+// cycle.  The transposing read (a fragment whose reduction runs across rows) takes 64 bytes of each of four consecutive
+// rows in a cycle: f sends them to the four quarters of the 256 bytes.  A fragment whose reduction runs along the row
+// takes the same chunk of sixteen consecutive rows: f has eight values for them, so two of them meet (all sixteen apart
+// would take twice as many address registers).
 //
 // The 32x32 matrix instructions give lane l = 32 h + c the column c and, in register i, the row 8 (i / 4) + 4 h + i % 4
 // of the result.  As the order of the reduction index is free as long as both operands agree, a result (probabilities,
@@ -179,7 +180,7 @@ template <typename T, int DC> struct at_row {
 };
 
 template <int CH> __device__ __forceinline__ int at_swizzle(int row) {
-  return CH >= 8 ? ((row & 3) << 1) | ((row >> 2) & 1) : (row & 2) | ((row >> 2) & 1);
+  return CH >= 16 ? ((row & 3) << 2) | ((row >> 2) & 1) : CH == 8 ? ((row & 2) << 1) | ((row >> 2) & 1) : (row >> 2) & 1;
 }
 template <typename T, int DC> __device__ __forceinline__ uint32_t at_chunk(int row, int chunk) {
   using R = at_row<T, DC>;
@@ -188,19 +189,19 @@ template <typename T, int DC> __device__ __forceinline__ uint32_t at_chunk(int r
 
 typedef unsigned char __attribute__((address_space(3))) * at_lds;
 
-// A lane's places in a tile.  The swizzle touches the lowest three bits of a chunk's number and goes by the lowest three
-// of the row's, so a few offsets, worked out once, reach everything with constant distances.
+// A lane's places in a tile.  The swizzle goes by the lowest three bits of the row's number and leaves some bits of the
+// chunk's alone, so a few offsets, worked out once, reach everything with constant distances.
 template <typename T, int DC> struct at_places {
   using R = at_row<T, DC>;
-  static constexpr int NA = R::CH >= 8 ? 4 : 2;
-  static constexpr int NX = sizeof(T) == 4 ? 4 : R::CH >= 8 ? 2 : 1;
-  uint32_t along[NA];   // row c, chunk 2 i + h
+  static constexpr int NA = R::CH >= 16 ? 4 : R::CH == 8 ? 2 : 1;       // chunk bits 2 and 3 are mixed with the row's
+  static constexpr int NX = sizeof(T) == 4 ? 4 : NA;
+  uint32_t along[NA];   // row c, chunk 4 i + h
   uint32_t across[NX];  // 16-bit: the transposing read's row and chunk, columns 32 i ..; fp32: row 4 h + i, column c
 
   __device__ __forceinline__ void init(int lane) {
     const int c = lane & 31, h = lane >> 5;
 #pragma unroll
-    for (int i = 0; i < NA; ++i) along[i] = at_chunk<T, DC>(c, 2 * i + h);
+    for (int i = 0; i < NA; ++i) along[i] = at_chunk<T, DC>(c, 4 * i + h);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int i = 0; i < NX; ++i) across[i] = at_chunk<T, DC>(4 * h + i, c >> 2) + (c & 3) * 4;
@@ -213,7 +214,7 @@ template <typename T, int DC> struct at_places {
   }
   // left operand of step st of a product along the rows: rows row .. row + 31 (a multiple of 32)
   __device__ __forceinline__ at_u4 rows(const unsigned char* tile, int row, int st) const {
-    return *reinterpret_cast<const at_u4*>(tile + along[st % NA] + (row * R::RB + st / NA * (NA * 32)));
+    return *reinterpret_cast<const at_u4*>(tile + along[st / 2 % NA] + (row * R::RB + st % 2 * 32 + st / (2 * NA) * (NA * 64)));
   }
   // left operand of a product across the rows (16-bit types): the 16 rows from `row` (a multiple of 16), in the order of
   // a result's registers, columns 32 db .. 32 db + 31
@@ -224,9 +225,12 @@ template <typename T, int DC> struct at_places {
     const at_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4p)(p + 8 * R::RB));
     return __builtin_bit_cast(at_u4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
-  // the same in fp32: row 8 (i / 4) + 4 h + i % 4 behind `row`
+  // the same in fp32: row 8 (i / 4) + 4 h + i % 4 behind `row`.  The column's chunk 8 db + (c >> 2): its bit 3 is mixed
+  // too where a row has more than eight
   __device__ __forceinline__ float col(const unsigned char* tile, int row, int i, int db) const {
-    return *reinterpret_cast<const float*>(tile + across[i % 4] + ((row + 8 * (i / 4)) * R::RB + db * 128));
+    constexpr int MIX = R::CH >= 16 ? 128 : 0;
+    const uint32_t o = MIX && (db & 1) ? across[i % 4] ^ MIX : across[i % 4];
+    return *reinterpret_cast<const float*>(tile + o + ((row + 8 * (i / 4)) * R::RB + (MIX ? db / 2 * 256 : db * 128)));
   }
 };
 
@@ -257,7 +261,30 @@ __device__ __forceinline__ void at_mma_cols(const at_places<T, DC>& at, const un
 // the swizzle is applied to the addresses that the lanes fetch from.  Chunks behind the head's end and rows that do
 // not take part are fetched from beyond the buffer's range, which gives zeros (so whatever those rows hold, NaN
 // included, never meets a product).
-constexpr uint32_t AT_RANGE = 0x80010000u, AT_OUTSIDE = 0xc0000000u;  // (+ a row's length: still outside, no wrap)
+// (an offset, a row's length and the scalar offset, together under 2^31, leave AT_OUTSIDE outside without a wrap)
+constexpr uint32_t AT_RANGE = 0x80010000u, AT_OUTSIDE = 0xc0000000u;
+
+typedef int at_i4 __attribute__((ext_vector_type(4)));
+
+// one load of 1 KiB (ONE: 256 bytes, four per lane) to LDS: base + off (AT_OUTSIDE or more: zeros) + soff.  (m0 is the
+// compiler's for no longer than an instruction that it sets it for: it needs no saving.)
+__device__ __forceinline__ at_i4 at_buffer(const void* base) {
+  const uint64_t b = (uint64_t)base;
+  return at_i4{__builtin_amdgcn_readfirstlane((int)b), __builtin_amdgcn_readfirstlane((int)(b >> 32) & 0xffff), (int)AT_RANGE,
+               0x00020000};
+}
+template <bool ONE = false> __device__ __forceinline__ void at_load_lds(at_i4 rs, uint32_t off, uint32_t soff, uint32_t lds) {
+  if constexpr (ONE)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, %3 offen lds"
+                 :
+                 : "v"(off), "s"(rs), "s"(lds), "s"(soff)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds"
+                 :
+                 : "v"(off), "s"(rs), "s"(lds), "s"(soff)
+                 : "memory");
+}
 
 template <typename T, int DC, int ROWS, int WAVES> struct at_stage {
   using R = at_row<T, DC>;
@@ -267,43 +294,34 @@ template <typename T, int DC, int ROWS, int WAVES> struct at_stage {
   static constexpr int PD = STEP >= 8 ? 1 : 8 / STEP;       // instructions after which the swizzle repeats
   static_assert(R::RB <= 1024 && ROWS * R::RB % (1024 * WAVES) == 0 && N % PD == 0, "whole instructions for every wave");
   uint32_t off[PD];
-  int64_t ahead;  // bytes from one group of PD instructions to the next
+  uint32_t ahead;  // bytes from one group of PD instructions to the next
 
-  // D: elements of a head; stride: bytes between rows
+  // D: elements of a head; stride: bytes between rows (under 16 MiB)
   __device__ __forceinline__ void init(int wave, int lane, int D, uint32_t stride) {
-    ahead = (int64_t)PD * STEP * stride;
+    ahead = PD * STEP * stride;
 #pragma unroll
     for (int p = 0; p < PD; ++p) {
       const int r = p * STEP + wave * PER + lane / R::CH, chunk = (lane % R::CH) ^ at_swizzle<R::CH>(r);
       off[p] = chunk * 16 < D * R::ES ? (uint32_t)r * stride + (uint32_t)chunk * 16u : AT_OUTSIDE;
     }
   }
-  // words[i]: rows 32 i .. that take part -> the word of each instruction's rows
-  static __device__ __forceinline__ void spread(const uint32_t (&words)[ROWS / 32], int wave, uint32_t (&take)[N]) {
+  // words[i], bit r: row 32 i + r takes part -> outside[p]: 0 where this lane's row of instruction p does, else AT_OUTSIDE
+  static __device__ __forceinline__ void spread(const uint32_t (&words)[ROWS / 32], int wave, int lane, uint32_t (&outside)[N]) {
 #pragma unroll
     for (int p = 0; p < N; ++p) {
-      take[p] = words[0];
+      uint32_t w = 0;
 #pragma unroll
-      for (int i = 1; i < ROWS / 32; ++i) take[p] = (p * STEP + wave * PER) >> 5 == i ? words[i] : take[p];
+      for (int i = 0; i < ROWS / 32; ++i) w |= words[i] & (0u - (uint32_t)((p * STEP + wave * PER) >> 5 == i));
+      outside[p] = (uint32_t)__builtin_amdgcn_sbfe((int)~w, (p * STEP + wave * PER + lane / R::CH) & 31, 1) & AT_OUTSIDE;
     }
   }
-  // base: the tile's first row; take[p]: the rows of the 32 that instruction p's rows lie in that take part, a bit each
-  __device__ __forceinline__ void issue(const char* base, uint32_t lds, int wave, int lane, bool full, const uint32_t (&take)[N]) const {
+  // base: the tile's first row; FULL: every row takes part
+  template <bool FULL> __device__ __forceinline__ void issue(const char* base, uint32_t lds, int wave, const uint32_t (&outside)[N]) const {
+    const at_i4 rs = at_buffer(base);
 #pragma unroll
-    for (int p = 0; p < N; ++p) {
-      const uint64_t b = (uint64_t)(base + (p / PD) * ahead);
-      typedef int i4 __attribute__((ext_vector_type(4)));
-      const i4 rs = {__builtin_amdgcn_readfirstlane((int)b), __builtin_amdgcn_readfirstlane((int)(b >> 32) & 0xffff),
-                     (int)AT_RANGE, 0x00020000};
-      uint32_t o = off[p % PD];
-      if (!full) o = (take[p] >> ((p * STEP + wave * PER + lane / R::CH) & 31)) & 1 ? o : AT_OUTSIDE;
-      const uint32_t dst = lds + (uint32_t)(p * WAVES + wave) * 1024u;
-      unsigned keep;
-      asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
-                   : "=&s"(keep)
-                   : "v"(o), "s"(rs), "s"(__builtin_amdgcn_readfirstlane(dst))
-                   : "memory");
-    }
+    for (int p = 0; p < N; ++p)
+      at_load_lds(rs, FULL ? off[p % PD] : off[p % PD] | outside[p], (p / PD) * ahead,
+                  __builtin_amdgcn_readfirstlane(lds + (uint32_t)(p * WAVES + wave) * 1024u));
   }
 };
 
@@ -328,14 +346,18 @@ template <typename T, int DC, int KT, int WAVES> struct at_key_tiles {
     v.init(wave, lane, a.D, (uint32_t)(a.vs[1] * sizeof(T)));
   }
   __device__ __forceinline__ void fetch(const at_args& a, uint32_t lds_k, uint32_t lds_v, int wave, int lane) {
-    uint32_t take[S::N];
-    const bool full = a.bits == nullptr && k_end - k0 >= KT;
-    uint32_t words[KT / 32];
+    uint32_t outside[S::N];
+    if (a.bits == nullptr && k_end - k0 >= KT) {
+      k.template issue<true>(kp, lds_k, wave, outside);
+      v.template issue<true>(vp, lds_v, wave, outside);
+    } else {
+      uint32_t words[KT / 32];
 #pragma unroll
-    for (int i = 0; i < KT / 32; ++i) words[i] = full ? 0xffffffffu : at_key_bits(a, n, k_end, k0 + 32 * i);
-    S::spread(words, wave, take);
-    k.issue(kp, lds_k, wave, lane, full, take);
-    v.issue(vp, lds_v, wave, lane, full, take);
+      for (int i = 0; i < KT / 32; ++i) words[i] = at_key_bits(a, n, k_end, k0 + 32 * i);
+      S::spread(words, wave, lane, outside);
+      k.template issue<false>(kp, lds_k, wave, outside);
+      v.template issue<false>(vp, lds_v, wave, outside);
+    }
     kp += kstep;
     vp += vstep;
     k0 += KT;
@@ -356,16 +378,7 @@ __device__ __forceinline__ void at_sync() {
 
 // up to 64 floats to LDS, zeros behind the first `left`
 __device__ __forceinline__ void at_fetch_floats(const float* base, int left, uint32_t lds, int lane) {
-  const uint64_t b = (uint64_t)base;
-  typedef int i4 __attribute__((ext_vector_type(4)));
-  const i4 rs = {__builtin_amdgcn_readfirstlane((int)b), __builtin_amdgcn_readfirstlane((int)(b >> 32) & 0xffff), (int)AT_RANGE,
-                 0x00020000};
-  const uint32_t o = lane < left ? (uint32_t)lane * 4u : AT_OUTSIDE;
-  unsigned keep;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
-               : "=&s"(keep)
-               : "v"(o), "s"(rs), "s"(__builtin_amdgcn_readfirstlane(lds))
-               : "memory");
+  at_load_lds<true>(at_buffer(base), lane < left ? (uint32_t)lane * 4u : AT_OUTSIDE, 0u, __builtin_amdgcn_readfirstlane(lds));
 }
 
 // Block id -> work item: ids go round the 8 XCDs, items that share keys should share an XCD's L2, so each XCD gets a

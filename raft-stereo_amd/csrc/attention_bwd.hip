@@ -160,15 +160,20 @@ template <typename T, int DC, int RT, int NW> struct at_query_tiles {
                                         int hq, int t0, uint32_t lds_q, uint32_t lds_g, uint32_t lds_l, uint32_t lds_d, int wave,
                                         int lane) const {
     const int left = a.Tq - t0;
-    uint32_t take[S::N];
-    uint32_t words[RT / 32];
+    const char* qp = reinterpret_cast<const char*>(q + (int64_t)n * a.qs[0] + (int64_t)t0 * a.qs[1] + (int64_t)hq * a.qs[2]);
+    const char* gp = reinterpret_cast<const char*>(dout + (((int64_t)n * a.Tq + t0) * a.Hq + hq) * a.D);
+    uint32_t outside[S::N];
+    if (left >= RT) {
+      sq.template issue<true>(qp, lds_q, wave, outside);
+      sg.template issue<true>(gp, lds_g, wave, outside);
+    } else {
+      uint32_t words[RT / 32];
 #pragma unroll
-    for (int i = 0; i < RT / 32; ++i) words[i] = at_first_bits(left - 32 * i);
-    S::spread(words, wave, take);
-    const bool full = left >= RT;
-    sq.issue(reinterpret_cast<const char*>(q + (int64_t)n * a.qs[0] + (int64_t)t0 * a.qs[1] + (int64_t)hq * a.qs[2]), lds_q, wave,
-             lane, full, take);
-    sg.issue(reinterpret_cast<const char*>(dout + (((int64_t)n * a.Tq + t0) * a.Hq + hq) * a.D), lds_g, wave, lane, full, take);
+      for (int i = 0; i < RT / 32; ++i) words[i] = at_first_bits(left - 32 * i);
+      S::spread(words, wave, lane, outside);
+      sq.template issue<false>(qp, lds_q, wave, outside);
+      sg.template issue<false>(gp, lds_g, wave, outside);
+    }
     const int64_t srow = ((int64_t)n * a.Hq + hq) * a.Tq + t0;
     if (wave == 0) at_fetch_floats(lse + srow, left, lds_l, lane);
     if (wave == NW - 1) at_fetch_floats(delta + srow, left, lds_d, lane);
