@@ -1,11 +1,12 @@
 // What the attention kernels share: arguments, the matrix-instruction fragments, and the staging of tiles of rows.
 //
 // A tile is a number of rows (tokens of one head) in LDS, RB bytes each (the head padded with zeros to a power of
-// two), cut into 16-byte chunks.  Chunk c of row r lies at r * RB + ((c ^ f(r)) << 4).  LDS has 64 banks, 256 bytes a
-// cycle.  The transposing read (a fragment whose reduction runs across rows) takes 64 bytes of each of four consecutive
-// rows in a cycle: f sends them to the four quarters of the 256 bytes.  A fragment whose reduction runs along the row
-// takes the same chunk of sixteen consecutive rows: f has eight values for them, so two of them meet (all sixteen apart
-// would take twice as many address registers).
+// two), cut into 16-byte chunks, with PAD bytes behind every eight rows: chunk c of row r lies at
+// r * RB + r / 8 * PAD + ((c ^ f(r)) << 4).  LDS has 64 banks, 256 bytes a cycle.  The transposing read (a fragment whose
+// reduction runs across rows) takes 64 bytes of each of four consecutive rows in a cycle: f sends them to the four
+// quarters of the 256 bytes.  A fragment whose reduction runs along the row takes the same chunk of sixteen consecutive
+// rows: f has eight values for them, and the pad moves the second eight to the places between.  (f by itself could take
+// sixteen values, at twice the address registers.)  Rows of 64 bytes go without the pad, and two of the sixteen meet.
 //
 // The 32x32 matrix instructions give lane l = 32 h + c the column c and, in register i, the row 8 (i / 4) + 4 h + i % 4
 // of the result.  As the order of the reduction index is free as long as both operands agree, a result (probabilities,
@@ -177,6 +178,9 @@ template <typename T, int DC> struct at_row {
   static constexpr int RB = DS * ES;    // bytes of a row
   static constexpr int CH = RB / 16;    // chunks of a row
   static constexpr int STEPS = DC * ES / 32;  // of a product along the row (two chunks each)
+  static constexpr int PAD = CH >= 8 ? 32 : 0;
+  static constexpr int at(int row) { return row * RB + row / 8 * PAD; }  // row: a multiple of 8
+  static constexpr int tile(int rows) { return at(rows); }               // bytes, rows: a multiple of 32
 };
 
 template <int CH> __device__ __forceinline__ int at_swizzle(int row) {
@@ -184,7 +188,7 @@ template <int CH> __device__ __forceinline__ int at_swizzle(int row) {
 }
 template <typename T, int DC> __device__ __forceinline__ uint32_t at_chunk(int row, int chunk) {
   using R = at_row<T, DC>;
-  return (uint32_t)(row * R::RB + ((chunk ^ at_swizzle<R::CH>(row)) << 4));
+  return (uint32_t)(row * R::RB + (row >> 3) * R::PAD + ((chunk ^ at_swizzle<R::CH>(row)) << 4));
 }
 
 typedef unsigned char __attribute__((address_space(3))) * at_lds;
@@ -214,15 +218,15 @@ template <typename T, int DC> struct at_places {
   }
   // left operand of step st of a product along the rows: rows row .. row + 31 (a multiple of 32)
   __device__ __forceinline__ at_u4 rows(const unsigned char* tile, int row, int st) const {
-    return *reinterpret_cast<const at_u4*>(tile + along[st / 2 % NA] + (row * R::RB + st % 2 * 32 + st / (2 * NA) * (NA * 64)));
+    return *reinterpret_cast<const at_u4*>(tile + along[st / 2 % NA] + (R::at(row) + st % 2 * 32 + st / (2 * NA) * (NA * 64)));
   }
   // left operand of a product across the rows (16-bit types): the 16 rows from `row` (a multiple of 16), in the order of
   // a result's registers, columns 32 db .. 32 db + 31
   __device__ __forceinline__ at_u4 cols(const unsigned char* tile, int row, int db) const {
     typedef at_s4 __attribute__((address_space(3))) * lds_s4p;
-    const unsigned char* p = tile + across[db % NX] + (row * R::RB + db / NX * (NX * 64));
+    const unsigned char* p = tile + across[db % NX] + (R::at(row) + db / NX * (NX * 64));
     const at_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4p)p);
-    const at_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4p)(p + 8 * R::RB));
+    const at_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4p)(p + R::at(8)));
     return __builtin_bit_cast(at_u4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
   // the same in fp32: row 8 (i / 4) + 4 h + i % 4 behind `row`.  The column's chunk 8 db + (c >> 2): its bit 3 is mixed
@@ -230,7 +234,7 @@ template <typename T, int DC> struct at_places {
   __device__ __forceinline__ float col(const unsigned char* tile, int row, int i, int db) const {
     constexpr int MIX = R::CH >= 16 ? 128 : 0;
     const uint32_t o = MIX && (db & 1) ? across[i % 4] ^ MIX : across[i % 4];
-    return *reinterpret_cast<const float*>(tile + o + ((row + 8 * (i / 4)) * R::RB + (MIX ? db / 2 * 256 : db * 128)));
+    return *reinterpret_cast<const float*>(tile + o + (R::at(row + 8 * (i / 4)) + (MIX ? db / 2 * 256 : db * 128)));
   }
 };
 
@@ -292,6 +296,7 @@ template <typename T, int DC, int ROWS, int WAVES> struct at_stage {
   static constexpr int N = ROWS * R::RB / 1024 / WAVES;     // instructions per wave, STEP rows apart
   static constexpr int STEP = PER * WAVES;
   static constexpr int PD = STEP >= 8 ? 1 : 8 / STEP;       // instructions after which the swizzle repeats
+  static_assert(R::PAD == 0 || 8 % PER == 0, "an instruction's rows have no pad between them");
   static_assert(R::RB <= 1024 && ROWS * R::RB % (1024 * WAVES) == 0 && N % PD == 0, "whole instructions for every wave");
   uint32_t off[PD];
   uint32_t ahead;  // bytes from one group of PD instructions to the next
@@ -321,7 +326,7 @@ template <typename T, int DC, int ROWS, int WAVES> struct at_stage {
 #pragma unroll
     for (int p = 0; p < N; ++p)
       at_load_lds(rs, FULL ? off[p % PD] : off[p % PD] | outside[p], (p / PD) * ahead,
-                  __builtin_amdgcn_readfirstlane(lds + (uint32_t)(p * WAVES + wave) * 1024u));
+                  __builtin_amdgcn_readfirstlane(lds + (uint32_t)((p * WAVES + wave) * 1024 + (((p * WAVES + wave) * PER) >> 3) * R::PAD)));
   }
 };
 
@@ -331,12 +336,12 @@ template <typename T, int DC, int KT, int WAVES> struct at_key_tiles {
   S k, v;
   const char *kp, *vp;
   int64_t kstep, vstep;
-  int n, k0, k_end;  // sequence, first key of the tile that is fetched next, end of the item's keys
+  int n, next_k, next_v, k_end;  // sequence, first keys of the tiles that are fetched next, end of the item's keys
 
   __device__ __forceinline__ void init(const at_args& a, const T* kb, const T* vb, int seq, int hk, int begin, int end,
                                        int wave, int lane) {
     n = seq;
-    k0 = begin;
+    next_k = next_v = begin;
     k_end = end;
     kp = reinterpret_cast<const char*>(kb + (int64_t)n * a.ks[0] + (int64_t)hk * a.ks[2] + (int64_t)begin * a.ks[1]);
     vp = reinterpret_cast<const char*>(vb + (int64_t)n * a.vs[0] + (int64_t)hk * a.vs[2] + (int64_t)begin * a.vs[1]);
@@ -345,22 +350,29 @@ template <typename T, int DC, int KT, int WAVES> struct at_key_tiles {
     k.init(wave, lane, a.D, (uint32_t)(a.ks[1] * sizeof(T)));
     v.init(wave, lane, a.D, (uint32_t)(a.vs[1] * sizeof(T)));
   }
+  template <bool DO_K, bool DO_V>
   __device__ __forceinline__ void fetch(const at_args& a, uint32_t lds_k, uint32_t lds_v, int wave, int lane) {
+    const int k0 = DO_K ? next_k : next_v;
     uint32_t outside[S::N];
     if (a.bits == nullptr && k_end - k0 >= KT) {
-      k.template issue<true>(kp, lds_k, wave, outside);
-      v.template issue<true>(vp, lds_v, wave, outside);
+      if constexpr (DO_K) k.template issue<true>(kp, lds_k, wave, outside);
+      if constexpr (DO_V) v.template issue<true>(vp, lds_v, wave, outside);
     } else {
       uint32_t words[KT / 32];
 #pragma unroll
       for (int i = 0; i < KT / 32; ++i) words[i] = at_key_bits(a, n, k_end, k0 + 32 * i);
       S::spread(words, wave, lane, outside);
-      k.template issue<false>(kp, lds_k, wave, outside);
-      v.template issue<false>(vp, lds_v, wave, outside);
+      if constexpr (DO_K) k.template issue<false>(kp, lds_k, wave, outside);
+      if constexpr (DO_V) v.template issue<false>(vp, lds_v, wave, outside);
     }
-    kp += kstep;
-    vp += vstep;
-    k0 += KT;
+    if constexpr (DO_K) {
+      kp += kstep;
+      next_k += KT;
+    }
+    if constexpr (DO_V) {
+      vp += vstep;
+      next_v += KT;
+    }
   }
 };
 
@@ -381,14 +393,30 @@ __device__ __forceinline__ void at_fetch_floats(const float* base, int left, uin
   at_load_lds<true>(at_buffer(base), lane < left ? (uint32_t)lane * 4u : AT_OUTSIDE, 0u, __builtin_amdgcn_readfirstlane(lds));
 }
 
-// Block id -> work item: ids go round the 8 XCDs, items that share keys should share an XCD's L2, so each XCD gets a
-// run of consecutive items.  The grid has at_grid() blocks.
-__device__ __forceinline__ int at_item(int items) {
-  const uint32_t per = ((uint32_t)items + 7) / 8, x = blockIdx.x >> 3;
-  const uint32_t i = (blockIdx.x & 7) * per + x;
-  return x < per && i < (uint32_t)items ? (int)i : -1;
-}
-static inline uint32_t at_grid(int64_t items) { return (uint32_t)((items + 7) / 8 * 8); }
+// Block id -> work item.  Ids go round the 8 XCDs; items that share keys stay on one XCD and its L2, and units of them
+// are dealt out in turn, so that sequences of different lengths spread.  A unit is a sequence, whose heads share cache
+// lines, or one key head of it where there are too few sequences to go round (dealing out heads of 64 bytes a token to
+// eight XCDs costs 15 % at 640 sequences of 180; dealing out four sequences leaves half the card idle).  The items of
+// the last units (fewer than 8) are divided evenly.
+struct at_order {
+  at_div subs;    // items of a unit
+  int32_t units;
+  __host__ at_order(int64_t N, int64_t Hk, int64_t items_of_head)
+      : subs((uint32_t)(N >= 16 ? Hk * items_of_head : items_of_head)), units((int32_t)(N >= 16 ? N : N * Hk)) {}
+  __host__ uint32_t grid() const {
+    return (uint32_t)(8 * ((int64_t)(units / 8) * subs.d + ((int64_t)(units % 8) * subs.d + 7) / 8));
+  }
+  // -1: none
+  __device__ __forceinline__ int item() const {
+    const int xcd = blockIdx.x & 7, pos = blockIdx.x >> 3, whole = (units >> 3) * (int)subs.d;
+    if (pos < whole) {
+      const int u = subs.of(pos);
+      return (u * 8 + xcd) * (int)subs.d + pos - u * (int)subs.d;
+    }
+    const int rest = (units & 7) * (int)subs.d, per = (rest + 7) >> 3, i = xcd * per + pos - whole;
+    return pos - whole < per && i < rest ? (units & ~7) * (int)subs.d + i : -1;
+  }
+};
 
 // Writes a result (rows: elements 32 db .. of the head, column: this lane's row of memory at p) times f.
 template <typename T, int DC>

@@ -51,7 +51,7 @@ struct at_parts {
 };
 
 template <typename T, int DC, int KT, int WAVES> struct at_dq_lds {
-  static constexpr int TILE = KT * at_row<T, DC>::RB;
+  static constexpr int TILE = at_row<T, DC>::tile(KT);
   static constexpr int BYTES = 4 * TILE;
 };
 
@@ -60,12 +60,12 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dq_kernel(const T* __restrict
                                                              const T* __restrict__ v, const T* __restrict__ out,
                                                              const float* __restrict__ lse, const T* __restrict__ dout,
                                                              float* __restrict__ delta, T* __restrict__ dq, at_parts sp,
-                                                             at_args a, at_div by_tiles, at_div by_splits, int items) {
+                                                             at_args a, at_order order, at_div by_tiles, at_div by_splits) {
   using R = at_row<T, DC>;
   constexpr int NDB = DC / 32, KT = 32 * NKB;
   constexpr int TILE = at_dq_lds<T, DC, KT, NW>::TILE;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  const int item = at_item(items);
+  const int item = order.item();
   if (item < 0) return;
   const int rest = by_tiles.of(item), rt = item - rest * (int)by_tiles.d;
   const int nh = by_splits.of(rest), split = rest - nh * (int)by_splits.d;
@@ -83,7 +83,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dq_kernel(const T* __restrict
   at_key_tiles<T, DC, KT, NW> kv;
   kv.init(a, k, v, n, hk, k_begin, k_end, wave, lane);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(at_lds)smem;
-  if (tiles > 0) kv.fetch(a, lds0, lds0 + 2 * TILE, wave, lane);
+  if (tiles > 0) kv.template fetch<true, true>(a, lds0, lds0 + 2 * TILE, wave, lane);
 
   const int64_t orow = (((int64_t)n * a.Tq + t) * a.Hq + hq) * a.D, srow = ((int64_t)n * a.Hq + hq) * a.Tq + t;
   at_u4 qf[R::STEPS], gf[R::STEPS];
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dq_kernel(const T* __restrict
 
   for (int j = 0; j < tiles; ++j) {
     at_landed();
-    if (j + 1 < tiles) kv.fetch(a, lds0 + ((j + 1) & 1) * TILE, lds0 + (2 + ((j + 1) & 1)) * TILE, wave, lane);
+    if (j + 1 < tiles) kv.template fetch<true, true>(a, lds0 + ((j + 1) & 1) * TILE, lds0 + (2 + ((j + 1) & 1)) * TILE, wave, lane);
     const unsigned char* kt = smem + (j & 1) * TILE;
     const unsigned char* vt = smem + (2 + (j & 1)) * TILE;
     if (DC <= 64 && row0 >= a.Tq * a.G) continue;  // (this wave only helps with the loads)
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dq_kernel(const T* __restrict
 }
 
 template <typename T, int DC, int RT> struct at_dkv_lds {
-  static constexpr int TILE = RT * at_row<T, DC>::RB;
+  static constexpr int TILE = at_row<T, DC>::tile(RT);
   static constexpr int STAT = 256;  // bytes of a tile's lse2 (delta): 64 floats, what one load moves
   static constexpr int BYTES = 4 * TILE + 4 * STAT;
 };
@@ -185,12 +185,12 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dkv_kernel(const T* __restric
                                                               const T* __restrict__ v, const float* __restrict__ lse,
                                                               const T* __restrict__ dout, const float* __restrict__ delta,
                                                               T* __restrict__ dk, T* __restrict__ dv, at_parts sp, at_args a,
-                                                              at_div by_tiles, at_div by_splits, at_div by_rows, int items) {
+                                                              at_order order, at_div by_tiles, at_div by_splits, at_div by_rows) {
   using R = at_row<T, DC>;
   constexpr int NDB = DC / 32, RT = 32 * NRB;
   using L = at_dkv_lds<T, DC, RT>;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  const int item = at_item(items);
+  const int item = order.item();
   if (item < 0) return;
   const int rest = by_tiles.of(item), kt = item - rest * (int)by_tiles.d;
   const int nh = by_splits.of(rest), split = rest - nh * (int)by_splits.d;
@@ -381,10 +381,10 @@ template <typename T, int DC, int NRB, bool DO_K, bool DO_V, int OCC> int at_lau
   sp.n = c.p.k_splits;
   sp.p = c.parts;
   sp.part = c.a->N * c.a->Tk * c.a->Hk * c.a->D;
-  const int64_t items = c.p.k_items * sp.n;
-  kernel<<<at_grid(items), 256, L::BYTES, c.st>>>((const T*)c.q, (const T*)c.k, (const T*)c.v, c.lse, (const T*)c.dout, c.delta,
-                                                  (T*)c.dk, (T*)c.dv, sp, c.d, at_div((uint32_t)c.p.k_tiles),
-                                                  at_div((uint32_t)sp.n), at_div((uint32_t)row_tiles), (int)items);
+  const at_order order(c.a->N, c.a->Hk, c.p.k_tiles * sp.n);
+  kernel<<<order.grid(), 256, L::BYTES, c.st>>>((const T*)c.q, (const T*)c.k, (const T*)c.v, c.lse, (const T*)c.dout, c.delta,
+                                                  (T*)c.dk, (T*)c.dv, sp, c.d, order,
+                                               at_div((uint32_t)c.p.k_tiles), at_div((uint32_t)sp.n), at_div((uint32_t)row_tiles));
   return rc_check_launch("rc_cross_attn_bwd (keys)");
 }
 
@@ -410,10 +410,10 @@ template <typename T, int DC> int at_bwd(const at_bwd_call& c) {
     sp.per = c.p.q_per;
     sp.p = c.parts;
     sp.part = c.a->N * c.a->Tq * c.a->Hq * c.a->D;
-    const int64_t items = c.p.q_items * sp.n;
-    kernel<<<at_grid(items), 256, bytes, c.st>>>((const T*)c.q, (const T*)c.k, (const T*)c.v, (const T*)c.out, c.lse,
-                                                 (const T*)c.dout, c.delta, (T*)c.dq, sp, c.d, at_div((uint32_t)c.p.q_tiles),
-                                                 at_div((uint32_t)sp.n), (int)items);
+    const at_order order(c.a->N, c.a->Hk, c.p.q_tiles * sp.n);
+    kernel<<<order.grid(), 256, bytes, c.st>>>((const T*)c.q, (const T*)c.k, (const T*)c.v, (const T*)c.out, c.lse,
+                                                 (const T*)c.dout, c.delta, (T*)c.dq, sp, c.d, order,
+                                                 at_div((uint32_t)c.p.q_tiles), at_div((uint32_t)sp.n));
     if ((rc = rc_check_launch("rc_cross_attn_bwd (queries)"))) return rc;
     if (c.dq && sp.n > 1 && (rc = at_add<T>(c, 0, sp.part, sp.n, c.dq, sp.part))) return rc;
   }

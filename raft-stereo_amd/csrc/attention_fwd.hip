@@ -29,23 +29,23 @@ template <typename T, int DC, int NWQ, int NWK, int NKB> struct at_fwd_cfg {
   static constexpr int WAVES = NWQ * NWK;
   static constexpr int ROWS = 32 * NWQ;       // query rows of a work item
   static constexpr int KT = 32 * NKB * NWK;   // keys of a tile
-  static constexpr int TILE = KT * R::RB;
+  static constexpr int TILE = R::tile(KT);
   static constexpr int LDS = 4 * TILE;        // keys and values, two tiles each
 };
 
 // NWQ waves side by side own 32 rows each; NWK waves share the same rows and take 32 NKB keys each of every tile.
-template <typename T, int DC, int NWQ, int NWK, int NKB, int OCC>
+template <typename T, int DC, int NWQ, int NWK, int NKB, bool AHEAD, int OCC>
 __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                                      const T* __restrict__ v, T* __restrict__ out,
                                                                      float* __restrict__ lse, at_split sp, at_args a,
-                                                                     at_div by_tiles, at_div by_splits, int items) {
+                                                                     at_order order, at_div by_tiles, at_div by_splits) {
   using C = at_fwd_cfg<T, DC, NWQ, NWK, NKB>;
   using R = at_row<T, DC>;
   constexpr int NDB = DC / 32;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  const int item = at_item(items);
+  // rows fastest, then splits, then heads and sequences
+  const int item = order.item();
   if (item < 0) return;
-  // rows fastest, then splits, then heads and sequences: neighbours share keys
   const int rest = by_tiles.of(item), rt = item - rest * (int)by_tiles.d;
   const int nh = by_splits.of(rest), split = rest - nh * (int)by_splits.d;
   const int n = a.by_Hk.of(nh), hk = nh - n * a.Hk;
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
   at_key_tiles<T, DC, C::KT, C::WAVES> kv;
   kv.init(a, k, v, n, hk, k_begin, k_end, wave, lane);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(at_lds)smem;
-  if (tiles > 0) kv.fetch(a, lds0, lds0 + 2 * C::TILE, wave, lane);
+  if (tiles > 0) kv.template fetch<true, true>(a, lds0, lds0 + 2 * C::TILE, wave, lane);
 
   at_u4 qf[R::STEPS];
   at_rows_of(q + (int64_t)n * a.qs[0] + (int64_t)first * a.qs[1] + (int64_t)hk * a.G * a.qs[2])
@@ -81,32 +81,41 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
   float m = -INFINITY, l = 0.0f;
   uint32_t any = 0;
 
-  for (int j = 0; j < tiles; ++j) {
-    at_landed();
-    if (j + 1 < tiles) kv.fetch(a, lds0 + ((j + 1) & 1) * C::TILE, lds0 + (2 + ((j + 1) & 1)) * C::TILE, wave, lane);
-    const unsigned char* kt = smem + (j & 1) * C::TILE;
-    const unsigned char* vt = smem + (2 + (j & 1)) * C::TILE;
-    const int kr = 32 * NKB * wk;  // this wave's first key of the tile
-
-    if (row0 >= rows) continue;  // (this wave only helps with the loads)
-
-    at_f16 s[NKB];
+  const int kr = 32 * NKB * wk;  // this wave's first key of a tile
+  const bool idle = row0 >= rows;  // this wave only helps with the loads
+  // While a wave multiplies, its partner on the SIMD exponentiates; the matrix pipe is the scarcer one for wide heads
+  // (2 % at 4095 keys and D 128; heads of 64 and less lose as much)
+  auto priority = [](int on) {
+    if constexpr (DC > 64) {
+      if (on) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(0);
+    }
+  };
+  // the scores of a tile
+  auto start = [&](at_f16 (&s)[NKB], int j) {
 #pragma unroll
     for (int b = 0; b < NKB; ++b) {
       const uint32_t take = at_key_bits(a, n, k_end, k_begin + j * C::KT + kr + 32 * b);
       any |= take;
       s[b] = at_start<T>(take, lane);
     }
+  };
+  auto scores = [&](at_f16 (&s)[NKB], int j, const unsigned char* kt) {
+    start(s, j);
 #pragma unroll
     for (int st = 0; st < R::STEPS; ++st)
 #pragma unroll
       for (int b = 0; b < NKB; ++b) s[b] = at_mma(T(), at.rows(kt, kr + 32 * b, st), qf[st], s[b]);
+  };
+  auto largest = [&](const at_f16 (&s)[NKB]) {
     float mx = s[0][0];
 #pragma unroll
     for (int b = 0; b < NKB; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
-    mx = at_half_max(mx) * a.scale_log2;
+    return at_half_max(mx) * a.scale_log2;
+  };
+  auto raise = [&](float mx) {
     if (__any(mx > m + AT_SLACK)) {
       const float mn = fmaxf(m, mx);
       const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -115,15 +124,103 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
 #pragma unroll
       for (int i = 0; i < NDB; ++i) acc[i] *= f;
     }
+  };
+  auto probabilities = [&](at_f16 (&s)[NKB]) {
     const float mu = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-    for (int b = 0; b < NKB; ++b) {
+    for (int b = 0; b < NKB; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         s[b][i] = __builtin_amdgcn_exp2f(s[b][i] * a.scale_log2 - mu);
         l += s[b][i];
       }
-      at_mma_cols<T, DC>(at, vt, kr + 32 * b, s[b], acc);
+  };
+  auto values = [&](const at_f16 (&s)[NKB], const unsigned char* vt) {
+#pragma unroll
+    for (int b = 0; b < NKB; ++b) at_mma_cols<T, DC>(at, vt, kr + 32 * b, s[b], acc);
+  };
+
+  if constexpr (AHEAD) {
+    // The scores of the next tile are multiplied while this one's are exponentiated, so that the matrix and the vector
+    // pipe of a SIMD have work at the same time: the keys are fetched a tile ahead of the values.
+    at_f16 s0[NKB], s1[NKB];
+    if (tiles > 0) {
+      at_landed();
+      if (tiles > 1) kv.template fetch<true, false>(a, lds0 + C::TILE, 0u, wave, lane);
+      if (!idle) {
+        scores(s0, 0, smem);
+        raise(largest(s0));
+      }
+    }
+    // (behind the last tile, scores of whatever lies in LDS are multiplied; nothing looks at them)
+    auto step = [&](at_f16 (&s)[NKB], at_f16 (&next)[NKB], int j, int odd) {
+      at_landed();
+      if (j + 2 < tiles) kv.template fetch<true, false>(a, lds0 + odd * C::TILE, 0u, wave, lane);
+      if (j + 1 < tiles) kv.template fetch<false, true>(a, 0u, lds0 + (2 + (odd ^ 1)) * C::TILE, wave, lane);
+      if (idle) return;
+      const unsigned char* kt = smem + (odd ^ 1) * C::TILE;
+      const unsigned char* vt = smem + (2 + odd) * C::TILE;
+      start(next, j + 1);
+      const float mu = m == -INFINITY ? 0.0f : m;
+      at_u4 kf[2][NKB];
+#pragma unroll
+      for (int b = 0; b < NKB; ++b) kf[0][b] = at.rows(kt, kr + 32 * b, 0);
+#pragma unroll
+      for (int st = 0; st < R::STEPS; ++st) {
+#pragma unroll
+        for (int b = 0; b < NKB; ++b) {
+          if (st + 1 < R::STEPS) kf[(st + 1) & 1][b] = at.rows(kt, kr + 32 * b, st + 1);
+          next[b] = at_mma(T(), kf[st & 1][b], qf[st], next[b]);
+#pragma unroll
+          for (int i = 16 * st / R::STEPS; i < 16 * (st + 1) / R::STEPS; ++i) {
+            s[b][i] = __builtin_amdgcn_exp2f(s[b][i] * a.scale_log2 - mu);
+            l += s[b][i];
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      priority(1);
+      constexpr int U = NKB * 2 * NDB;  // products of the values: 16 keys by 32 elements each
+      float mx = next[0][0];
+      at_u4 vf[2];
+      at_u4 pf;
+      vf[0] = at.cols(vt, kr, 0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int b = u / (2 * NDB), hf = u / NDB % 2, db = u % NDB;
+        if (u + 1 < U) vf[(u + 1) & 1] = at.cols(vt, kr + 16 * ((u + 1) / NDB), (u + 1) % NDB);
+        if (db == 0) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) pf[x] = at_pack(T(), s[b][8 * hf + 2 * x], s[b][8 * hf + 2 * x + 1]);
+        }
+        acc[db] = at_mma(T(), vf[u & 1], pf, acc[db]);
+#pragma unroll
+        for (int i = 16 * NKB * u / U; i < 16 * NKB * (u + 1) / U; ++i) mx = fmaxf(mx, next[i / 16][i % 16]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      priority(0);
+      mx = at_half_max(mx) * a.scale_log2;
+      raise(mx);
+    };
+    for (int j = 0; j < tiles; j += 2) {
+      step(s0, s1, j, 0);
+      if (j + 1 < tiles) step(s1, s0, j + 1, 1);
+    }
+  } else {
+    for (int j = 0; j < tiles; ++j) {
+      at_landed();
+      if (j + 1 < tiles)
+        kv.template fetch<true, true>(a, lds0 + ((j + 1) & 1) * C::TILE, lds0 + (2 + ((j + 1) & 1)) * C::TILE, wave, lane);
+      if (idle) continue;
+      at_f16 s[NKB];
+      priority(1);
+      scores(s, j, smem + (j & 1) * C::TILE);
+      priority(0);
+      raise(largest(s));
+      probabilities(s);
+      priority(1);
+      values(s, smem + (2 + (j & 1)) * C::TILE);
+      priority(0);
     }
   }
   l = at_half_sum(l);
@@ -252,13 +349,13 @@ __global__ __launch_bounds__(256) void at_bits_kernel(const unsigned char* __res
   if ((threadIdx.x & 63) == 0) bits[w] = b;
 }
 
-template <typename T, int DC, int NWQ, int NWK, int NKB, int OCC>
+template <typename T, int DC, int NWQ, int NWK, int NKB, bool AHEAD, int OCC>
 int at_launch(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, void* out, float* lse,
               at_split sp, hipStream_t st) {
   using C = at_fwd_cfg<T, DC, NWQ, NWK, NKB>;
   constexpr int lds = NWK > 1 && C::WAVES * (64 + DC / 32 * 1024 + 4) * 4 > C::LDS ? C::WAVES * (64 + DC / 32 * 1024 + 4) * 4 : C::LDS;
   static_assert(lds <= 160 * 1024, "LDS");
-  auto kernel = at_fwd_kernel<T, DC, NWQ, NWK, NKB, OCC>;
+  auto kernel = at_fwd_kernel<T, DC, NWQ, NWK, NKB, AHEAD, OCC>;
   if (lds > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) {
@@ -267,9 +364,9 @@ int at_launch(const rc_attn* a, const at_args& d, const void* q, const void* k, 
     }
   }
   const int64_t rows = a->Tq * d.G, row_tiles = (rows + C::ROWS - 1) / C::ROWS;
-  const int64_t items = a->N * a->Hk * sp.n * row_tiles;
-  kernel<<<at_grid(items), 64 * C::WAVES, lds, st>>>((const T*)q, (const T*)k, (const T*)v, (T*)out, lse, sp, d,
-                                                     at_div((uint32_t)row_tiles), at_div((uint32_t)sp.n), (int)items);
+  const at_order order(a->N, a->Hk, sp.n * row_tiles);
+  kernel<<<order.grid(), 64 * C::WAVES, lds, st>>>((const T*)q, (const T*)k, (const T*)v, (T*)out, lse, sp, d,
+                                                order, at_div((uint32_t)row_tiles), at_div((uint32_t)sp.n));
   int rc = rc_check_launch("rc_cross_attn_fwd");
   if (rc || sp.n == 1) return rc;
   const int64_t all = a->N * a->Hk * rows;
@@ -317,8 +414,12 @@ int at_run(const rc_attn* a, const at_args& d, const void* q, const void* k, con
   constexpr int NWK = RB >= 1024 ? 1 : RB >= 512 ? 2 : 4;
   constexpr int NKB = RB >= 512 ? 1 : 2;
   constexpr int OCC = RB >= 1024 ? 1 : DC * (int)sizeof(T) >= 192 ? 2 : 3;
-  if (p.few) return at_launch<T, DC, 1, NWK, 1, 1>(a, d, q, k, v, out, lse, p.sp, st);
-  return at_launch<T, DC, 4, 1, NKB, OCC>(a, d, q, k, v, out, lse, p.sp, st);
+  // AHEAD: 16-bit heads of 96 and 128 (8 x 2047 x 4095, 16/4 heads of 128: 620 against 680 us, 800 x 800: 122 against
+  // 138).  Narrower heads are held up by the exponentials either way and have four waves per SIMD to hide them with
+  // (D 64: 332 against 328 us, 312 x 312: 167 against 148); wider ones have no registers for a second tile of scores.
+  constexpr bool AHEAD = sizeof(T) == 2 && DC > 64 && DC <= 128;
+  if (p.few) return at_launch<T, DC, 1, NWK, 1, false, 1>(a, d, q, k, v, out, lse, p.sp, st);
+  return at_launch<T, DC, 4, 1, NKB, AHEAD, (AHEAD ? 2 : OCC)>(a, d, q, k, v, out, lse, p.sp, st);
 }
 
 template <typename T>
