@@ -51,6 +51,10 @@ struct at_args {
   float scale, scale_log2;
 };
 
+// host side (attention_rows.hip): the backward pass in one kernel where a sequence's keys fit a workgroup
+bool at_rows_fit(const rc_attn* a);
+int at_rows_bwd(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, const void* out,
+                const float* lse, const void* dout, void* dq, void* dk, void* dv, hipStream_t st);
 // host side (attention_fwd.hip)
 int at_check(const rc_attn* a);
 int at_check_operand(const rc_attn* a, int64_t rows, const void* p);
@@ -100,13 +104,15 @@ __device__ __forceinline__ at_f16 at_mma(float, at_u4 a, at_u4 b, at_f16 c) {
 
 // What a block of 32 keys' scores start from: 0, or -inf for the keys whose bit in `take` is not set (the same for the
 // whole wave).  The mask costs a select and a product of one column by one row: -inf or 0 of this lane's key by 1.
-template <typename T> __device__ __forceinline__ at_f16 at_start(uint32_t take, int lane) {
+// COLS: the keys are the result's columns.
+template <typename T, bool COLS = false> __device__ __forceinline__ at_f16 at_start(uint32_t take, int lane) {
   at_f16 s = (at_f16)(0.0f);
   if (take != 0xffffffffu) {
     const bool out = lane < 32 && !((take >> lane) & 1);
     const uint32_t inf = sizeof(T) == 4 ? 0xff800000u : __is_same(T, rc_half) ? 0xfc00u : 0xff80u;
     const uint32_t one = sizeof(T) == 4 ? 0x3f800000u : __is_same(T, rc_half) ? 0x3c00u : 0x3f80u;
-    const at_u4 x = {out ? inf : 0u, 0u, 0u, 0u}, y = {lane < 32 ? one : 0u, 0u, 0u, 0u};
+    const at_u4 keys = {out ? inf : 0u, 0u, 0u, 0u}, ones = {lane < 32 ? one : 0u, 0u, 0u, 0u};
+    const at_u4 x = COLS ? ones : keys, y = COLS ? keys : ones;
     if constexpr (sizeof(T) == 4) {
       const at_f4 u = __builtin_bit_cast(at_f4, x), w = __builtin_bit_cast(at_f4, y);
       s = __builtin_amdgcn_mfma_f32_32x32x2f32(u[0], w[0], s, 0, 0, 0);
@@ -472,3 +478,31 @@ struct at_rows_of {
     for (int st = 0; st < at_row<T, DC>::STEPS; ++st) f[st] = chunk<T>(off, D, st, lane >> 5);
   }
 };
+
+// fp16 has no room for scores' gradients as they come (of a long row they lie below its smallest normal number, of a
+// scaled loss beyond its largest).  Each lane's column has a power of two of its own, that of the running largest, and
+// its sums are rescaled when a larger one comes along, like a softmax's.  (P is at most 1: 2^12 throughout.)
+template <typename T> struct at_fit {
+  static constexpr bool ON = sizeof(T) == 2 && __is_same(T, rc_half);
+  float s = ON ? 0.0f : 1.0f;
+  template <int NDB> __device__ __forceinline__ void fit(at_f16& x, at_f16* acc) {
+    if constexpr (ON) {
+      float mx = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(x[i]));
+      mx = at_half_max(mx);
+      const bool need = mx * s > 32768.0f || (s == 0.0f && mx > 0.0f);
+      if (__any(need)) {
+        const int e = max(__builtin_amdgcn_frexp_expf(mx), -110);
+        const float to = need ? ldexpf(1.0f, 11 - e) : s;
+        const float f = s == 0.0f ? 1.0f : to / s;
+#pragma unroll
+        for (int i = 0; i < NDB; ++i) acc[i] *= f;
+        s = to;
+      }
+      x *= s;
+    }
+  }
+  __device__ __forceinline__ float undo() const { return ON ? (s == 0.0f ? 1.0f : 1.0f / s) : 1.0f; }
+};
+template <typename T> constexpr float AT_P_LIFT = at_fit<T>::ON ? 12.0f : 0.0f;

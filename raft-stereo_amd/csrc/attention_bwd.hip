@@ -15,34 +15,6 @@
 
 namespace {
 
-// fp16 has no room for scores' gradients as they come (of a long row they lie below its smallest normal number, of a
-// scaled loss beyond its largest).  Each lane's column has a power of two of its own, that of the running largest, and
-// its sums are rescaled when a larger one comes along, like a softmax's.  (P is at most 1: 2^12 throughout.)
-template <typename T> struct at_fit {
-  static constexpr bool ON = sizeof(T) == 2 && __is_same(T, rc_half);
-  float s = ON ? 0.0f : 1.0f;
-  template <int NDB> __device__ __forceinline__ void fit(at_f16& x, at_f16* acc) {
-    if constexpr (ON) {
-      float mx = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(x[i]));
-      mx = at_half_max(mx);
-      const bool need = mx * s > 32768.0f || (s == 0.0f && mx > 0.0f);
-      if (__any(need)) {
-        const int e = max(__builtin_amdgcn_frexp_expf(mx), -110);
-        const float to = need ? ldexpf(1.0f, 11 - e) : s;
-        const float f = s == 0.0f ? 1.0f : to / s;
-#pragma unroll
-        for (int i = 0; i < NDB; ++i) acc[i] *= f;
-        s = to;
-      }
-      x *= s;
-    }
-  }
-  __device__ __forceinline__ float undo() const { return ON ? (s == 0.0f ? 1.0f : 1.0f / s) : 1.0f; }
-};
-template <typename T> constexpr float AT_P_LIFT = at_fit<T>::ON ? 12.0f : 0.0f;
-
 struct at_parts {
   float* p;       // [split][...]: fp32 parts in the result's layout; NULL: one split, the result itself is written
   int64_t part;   // elements of one split
@@ -487,6 +459,8 @@ extern "C" int rc_cross_attn_bwd(const rc_attn* a, const void* q, const void* k,
   c.st = (hipStream_t)stream;
   c.d = at_to_dev(a, work);
   if ((rc = at_launch_bits(a, work, c.st))) return rc;
+  if (dq && dk && a->N * a->Tq && a->N * a->Tk && at_rows_fit(a))
+    return at_rows_bwd(a, c.d, q, k, v, out, lse, dout, dq, dk, dv, c.st);
   if (a->dtype == RC_F32) return at_bwd_d<float>(c);
   if (a->dtype == RC_F16) return at_bwd_d<rc_half>(c);
   return at_bwd_d<rc_bf16>(c);

@@ -57,6 +57,18 @@ SHAPES = [  # N, Tq, Tk, Hq, Hk, D
     (3, 129, 200, 2, 2, 24),
 ]
 
+# enough sequences of few keys for the backward pass to take a workgroup for each (the rows of an image): every number
+# of waves, keys that end inside a wave's block, query tiles that end inside, heads that share
+SHAPES += [
+    (260, 20, 33, 1, 1, 32),
+    (130, 37, 100, 4, 2, 64),
+    (90, 70, 129, 6, 3, 40),
+    (128, 33, 190, 2, 2, 32),
+    (70, 5, 250, 4, 4, 64),
+    (64, 100, 380, 4, 4, 24),
+    (256, 1, 1, 2, 1, 8),
+]
+
 
 def masks(kind, N, Tk, rng):
     """(lengths, mask): lengths of nothing, one, more than there are and less than nothing; a mask that leaves a
