@@ -336,6 +336,16 @@ template <typename T, int DC, int ROWS, int WAVES> struct at_stage {
   }
 };
 
+// instruction i of the loads of 32 rows from `base` (bit r of take: row r takes part)
+template <typename T, int DC>
+__device__ __forceinline__ void at_fetch_rows(const void* base, uint32_t stride, int D, uint32_t take, uint32_t lds, int i, int lane) {
+  using R = at_row<T, DC>;
+  constexpr int PER = 1024 / R::RB;
+  const int r = i * PER + lane / R::CH, chunk = (lane % R::CH) ^ at_swizzle<R::CH>(r);
+  const uint32_t off = chunk * 16 < D * R::ES && ((take >> r) & 1) ? (uint32_t)r * stride + (uint32_t)chunk * 16u : AT_OUTSIDE;
+  at_load_lds(at_buffer(base), off, 0u, __builtin_amdgcn_readfirstlane(lds + (uint32_t)(i * 1024 + ((i * PER) >> 3) * R::PAD)));
+}
+
 // The key and value tiles of a work item, in the order that it goes through them.
 template <typename T, int DC, int KT, int WAVES> struct at_key_tiles {
   using S = at_stage<T, DC, KT, WAVES>;

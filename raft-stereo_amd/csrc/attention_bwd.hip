@@ -113,10 +113,14 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dq_kernel(const T* __restrict
   else at_store_rows<T, DC>(dq + orow, live, acc, f, a.D, lane);
 }
 
-template <typename T, int DC, int RT> struct at_dkv_lds {
+// HALVES = 2: two waves share 32 keys and take every other block of query rows; their values lie in LDS
+template <typename T, int DC, int RT, int NW, int HALVES> struct at_dkv_lds {
   static constexpr int TILE = at_row<T, DC>::tile(RT);
   static constexpr int STAT = 256;  // bytes of a tile's lse2 (delta): 64 floats, what one load moves
-  static constexpr int BYTES = 4 * TILE + 4 * STAT;
+  static constexpr int V = 4 * TILE + 4 * STAT;
+  static constexpr int K = V + at_row<T, DC>::tile(32 * NW);  // (fp16: its scaling takes the registers that K has in bf16)
+  static constexpr int BYTES = HALVES == 1 ? V : at_fit<T>::ON ? K + at_row<T, DC>::tile(32 * NW) : K;
+  static_assert(HALVES == 1 || NW * DC / 32 * 16 * 64 * 4 <= V, "a wave's sums pass through the tiles' place");
 };
 
 // rows t0 .. of one query head: Q, dO, lse2 and delta
@@ -152,15 +156,15 @@ template <typename T, int DC, int RT, int NW> struct at_query_tiles {
   }
 };
 
-template <typename T, int DC, int NW, int NRB, bool DO_K, bool DO_V, int OCC>
-__global__ __launch_bounds__(64 * NW, OCC) void at_dkv_kernel(const T* __restrict__ q, const T* __restrict__ k,
+template <typename T, int DC, int NW, int HALVES, int NRB, bool DO_K, bool DO_V, int OCC>
+__global__ __launch_bounds__(64 * NW * HALVES, OCC) void at_dkv_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                               const T* __restrict__ v, const float* __restrict__ lse,
                                                               const T* __restrict__ dout, const float* __restrict__ delta,
                                                               T* __restrict__ dk, T* __restrict__ dv, at_parts sp, at_args a,
                                                               at_order order, at_div by_tiles, at_div by_splits, at_div by_rows) {
   using R = at_row<T, DC>;
   constexpr int NDB = DC / 32, RT = 32 * NRB;
-  using L = at_dkv_lds<T, DC, RT>;
+  using L = at_dkv_lds<T, DC, RT, NW, HALVES>;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
   const int item = order.item();
   if (item < 0) return;
@@ -169,7 +173,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dkv_kernel(const T* __restric
   const int n = a.by_Hk.of(nh), hk = nh - n * a.Hk, row_tiles = (int)by_rows.d;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c = lane & 31, h = lane >> 5;
-  const int key0 = (kt * NW + wave) * 32, key = key0 + c;
+  const int kw = wave % NW, half = wave / NW;
+  const int key0 = (kt * NW + kw) * 32, key = key0 + c;
   const int len = at_length(a, n);
   const uint32_t mine = at_key_bits(a, n, len, key0);
   const bool live = key < a.Tk, takes = (mine >> c) & 1;
@@ -181,7 +186,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dkv_kernel(const T* __restric
   const int begin = split * sp.per, end = some ? min(a.G * row_tiles, begin + sp.per) : begin;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(at_lds)smem;
   const uint32_t stat0 = lds0 + 4 * L::TILE;
-  at_query_tiles<T, DC, RT, NW> qt;
+  at_query_tiles<T, DC, RT, NW * HALVES> qt;
   qt.init(a, wave, lane);
   int g = row_tiles ? by_rows.of(begin) : 0, t0 = (begin - g * row_tiles) * RT;  // of the tile that is fetched next
   auto fetch = [&](int buf) {
@@ -195,12 +200,20 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dkv_kernel(const T* __restric
   };
   if (begin < end) fetch(0);
 
-  at_u4 kf[R::STEPS], vf[DO_K ? R::STEPS : 1];
-  at_rows_of(k + (int64_t)n * a.ks[0] + (int64_t)key0 * a.ks[1] + (int64_t)hk * a.ks[2])
-      .row<T, DC>(takes ? (uint32_t)c * (uint32_t)(a.ks[1] * sizeof(T)) : AT_OUTSIDE, a.D, lane, kf);
-  if constexpr (DO_K)
-    at_rows_of(v + (int64_t)n * a.vs[0] + (int64_t)key0 * a.vs[1] + (int64_t)hk * a.vs[2])
-        .row<T, DC>(takes ? (uint32_t)c * (uint32_t)(a.vs[1] * sizeof(T)) : AT_OUTSIDE, a.D, lane, vf);
+  constexpr bool V_LDS = HALVES > 1, K_LDS = HALVES > 1 && at_fit<T>::ON;
+  at_u4 kf[K_LDS ? 1 : R::STEPS], vf[V_LDS ? 1 : R::STEPS];
+  const T* kp = k + (int64_t)n * a.ks[0] + (int64_t)key0 * a.ks[1] + (int64_t)hk * a.ks[2];
+  const T* vp = v + (int64_t)n * a.vs[0] + (int64_t)key0 * a.vs[1] + (int64_t)hk * a.vs[2];
+  const uint32_t kst = (uint32_t)(a.ks[1] * sizeof(T)), vst = (uint32_t)(a.vs[1] * sizeof(T));
+  const unsigned char *vs = smem + L::V + R::at(32) * kw, *ks = smem + L::K + R::at(32) * kw;
+#pragma unroll
+  for (int i = 0; i < 32 * R::RB / 1024; ++i) {
+    if (i % HALVES != half) continue;
+    if constexpr (V_LDS) at_fetch_rows<T, DC>(vp, vst, a.D, mine, lds0 + L::V + R::at(32) * kw, i, lane);
+    if constexpr (K_LDS) at_fetch_rows<T, DC>(kp, kst, a.D, mine, lds0 + L::K + R::at(32) * kw, i, lane);
+  }
+  if constexpr (!K_LDS) at_rows_of(kp).row<T, DC>(takes ? (uint32_t)c * kst : AT_OUTSIDE, a.D, lane, kf);
+  if constexpr (!V_LDS && DO_K) at_rows_of(vp).row<T, DC>(takes ? (uint32_t)c * vst : AT_OUTSIDE, a.D, lane, vf);
   at_places<T, DC> at;
   at.init(lane);
   at_f16 acck[DO_K ? NDB : 1], accv[DO_V ? NDB : 1];
@@ -221,10 +234,12 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dkv_kernel(const T* __restric
     const float* ds = reinterpret_cast<const float*>(smem + 4 * L::TILE + (2 + buf) * L::STAT);
     if (DC <= 64 && mine == 0) continue;  // (none of this wave's keys takes part: it only helps with the loads)
 #pragma unroll
-    for (int b = 0; b < NRB; ++b) {
-      at_f16 s = (at_f16)(0.0f);
+    for (int bb = 0; bb < NRB / HALVES; ++bb) {
+      const int b = bb + half * (NRB / HALVES);
+      // (a key that takes no part has the score -inf, so P = 0, and zeros for its value, so dP = 0)
+      at_f16 s = at_start<T, true>(mine, lane);
 #pragma unroll
-      for (int st = 0; st < R::STEPS; ++st) s = at_mma(T(), at.rows(qs, 32 * b, st), kf[st], s);
+      for (int st = 0; st < R::STEPS; ++st) s = at_mma(T(), at.rows(qs, 32 * b, st), K_LDS ? at.rows(ks, 0, st) : kf[K_LDS ? 0 : st], s);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const at_f4 l4 = *reinterpret_cast<const at_f4*>(ls + 32 * b + 8 * x + 4 * h);
@@ -235,7 +250,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dkv_kernel(const T* __restric
       if constexpr (DO_K) {
         at_f16 dp = (at_f16)(0.0f);
 #pragma unroll
-        for (int st = 0; st < R::STEPS; ++st) dp = at_mma(T(), at.rows(gs, 32 * b, st), vf[st], dp);
+        for (int st = 0; st < R::STEPS; ++st) dp = at_mma(T(), at.rows(gs, 32 * b, st), V_LDS ? at.rows(vs, 0, st) : vf[V_LDS ? 0 : st], dp);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const at_f4 d4 = *reinterpret_cast<const at_f4*>(ds + 32 * b + 8 * x + 4 * h);
@@ -247,17 +262,35 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dkv_kernel(const T* __restric
       }
     }
   }
-  // a key that takes no part has a column of its own, whatever it holds: it is not written
+  const int64_t o = (((int64_t)n * a.Tk + key) * a.Hk + hk) * a.D;
+  if constexpr (HALVES > 1) {
+    // the other wave's sums, one of the two at a time
+    float* meet = reinterpret_cast<float*>(smem) + kw * NDB * 1024 + lane;
+    const float uk = fit.undo();
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      at_f16* acc = x ? accv : acck;
+      const float u = x ? 1.0f : uk;
+      at_sync();
+      if (half == 1) {
+#pragma unroll
+        for (int i = 0; i < NDB; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) meet[(i * 16 + r) * 64] = acc[i][r] * u;
+      }
+      at_sync();
+      if (half == 0) {
+#pragma unroll
+        for (int i = 0; i < NDB; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][r] = acc[i][r] * u + meet[(i * 16 + r) * 64];
+      }
+    }
+    if (half == 1) return;
+    fit = at_fit<T>();
+  }
   const float unlift = at_fit<T>::ON ? 1.0f / 4096.0f : 1.0f;
   const float fk = a.scale * fit.undo() * unlift, fv = unlift;
-  const int64_t o = (((int64_t)n * a.Tk + key) * a.Hk + hk) * a.D;
-  if (!takes) {
-#pragma unroll
-    for (int i = 0; i < NDB; ++i) {
-      if constexpr (DO_K) acck[i] = (at_f16)(0.0f);
-      if constexpr (DO_V) accv[i] = (at_f16)(0.0f);
-    }
-  }
   if (sp.n > 1) {
     float* p = sp.p + (int64_t)split * 2 * sp.part + o;
     if constexpr (DO_K) at_store_rows<float, DC>(p, live, acck, fk, a.D, lane);
@@ -339,11 +372,11 @@ struct at_bwd_call {
   hipStream_t st;
 };
 
-template <typename T, int DC, int NRB, bool DO_K, bool DO_V, int OCC> int at_launch_dkv(const at_bwd_call& c) {
+template <typename T, int DC, int HALVES, int NRB, bool DO_K, bool DO_V, int OCC> int at_launch_dkv(const at_bwd_call& c) {
   constexpr int RT = 32 * NRB;
-  using L = at_dkv_lds<T, DC, RT>;
+  using L = at_dkv_lds<T, DC, RT, 4, HALVES>;
   static_assert(L::BYTES <= 160 * 1024, "LDS");
-  auto kernel = at_dkv_kernel<T, DC, 4, NRB, DO_K, DO_V, OCC>;
+  auto kernel = at_dkv_kernel<T, DC, 4, HALVES, NRB, DO_K, DO_V, OCC>;
   int rc = at_allow_lds(kernel, L::BYTES);
   if (rc) return rc;
   const int64_t row_tiles = (c.a->Tq + RT - 1) / RT, all = row_tiles * c.d.G;
@@ -354,7 +387,7 @@ template <typename T, int DC, int NRB, bool DO_K, bool DO_V, int OCC> int at_lau
   sp.p = c.parts;
   sp.part = c.a->N * c.a->Tk * c.a->Hk * c.a->D;
   const at_order order(c.a->N, c.a->Hk, c.p.k_tiles * sp.n);
-  kernel<<<order.grid(), 256, L::BYTES, c.st>>>((const T*)c.q, (const T*)c.k, (const T*)c.v, c.lse, (const T*)c.dout, c.delta,
+  kernel<<<order.grid(), 256 * HALVES, L::BYTES, c.st>>>((const T*)c.q, (const T*)c.k, (const T*)c.v, c.lse, (const T*)c.dout, c.delta,
                                                   (T*)c.dk, (T*)c.dv, sp, c.d, order,
                                                at_div((uint32_t)c.p.k_tiles), at_div((uint32_t)sp.n), at_div((uint32_t)row_tiles));
   return rc_check_launch("rc_cross_attn_bwd (keys)");
@@ -370,7 +403,8 @@ template <typename T, int DC> int at_bwd(const at_bwd_call& c) {
   constexpr int RB = at_row<T, DC>::RB;
   constexpr int NB = RB >= 512 ? 1 : 2;
   constexpr int OCC = RB >= 512 ? 1 : 2;
-  constexpr int KOCC = DC * sizeof(T) <= 128 ? 2 : 1;
+  constexpr int HALVES = sizeof(T) == 2 && DC > 64 && DC <= 128 ? 2 : 1;
+  constexpr int KOCC = HALVES == 2 || DC * sizeof(T) <= 128 ? 2 : 1;
   int rc = RC_OK;
   if (c.p.q_items) {  // (the gradients of keys and values need delta)
     constexpr int bytes = at_dq_lds<T, DC, 32 * NB, 4>::BYTES;
@@ -392,10 +426,10 @@ template <typename T, int DC> int at_bwd(const at_bwd_call& c) {
   if (!c.dk || !c.p.k_items) return RC_OK;
   // wide heads in fp32, and in fp16 with its scaling: registers for one of the two at a time
   if constexpr (RB >= 1024 || (at_fit<T>::ON && DC > 128)) {
-    if ((rc = at_launch_dkv<T, DC, 1, true, false, 1>(c))) return rc;
-    if ((rc = at_launch_dkv<T, DC, 1, false, true, 1>(c))) return rc;
+    if ((rc = at_launch_dkv<T, DC, 1, 1, true, false, 1>(c))) return rc;
+    if ((rc = at_launch_dkv<T, DC, 1, 1, false, true, 1>(c))) return rc;
   } else {
-    if ((rc = at_launch_dkv<T, DC, NB, true, true, KOCC>(c))) return rc;
+    if ((rc = at_launch_dkv<T, DC, HALVES, NB, true, true, KOCC>(c))) return rc;
   }
   if (c.p.k_splits > 1) {
     const int64_t part = c.a->N * c.a->Tk * c.a->Hk * c.a->D;

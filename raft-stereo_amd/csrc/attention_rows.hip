@@ -26,16 +26,6 @@ template <typename T, int DC, int NW> struct at_rows_lds {
   static constexpr int BYTES = NORM + 64;
 };
 
-// instruction i of the loads of 32 rows from `base` (bit r of take: row r takes part)
-template <typename T, int DC>
-__device__ __forceinline__ void at_fetch_rows(const void* base, uint32_t stride, int D, uint32_t take, uint32_t lds, int i, int lane) {
-  using R = at_row<T, DC>;
-  constexpr int PER = 1024 / R::RB;
-  const int r = i * PER + lane / R::CH, chunk = (lane % R::CH) ^ at_swizzle<R::CH>(r);
-  const uint32_t off = chunk * 16 < D * R::ES && ((take >> r) & 1) ? (uint32_t)r * stride + (uint32_t)chunk * 16u : AT_OUTSIDE;
-  at_load_lds(at_buffer(base), off, 0u, __builtin_amdgcn_readfirstlane(lds + (uint32_t)(i * 1024 + ((i * PER) >> 3) * R::PAD)));
-}
-
 // A lane's place of an operand of a 16 x 16 product across a tile's rows: 32 rows a step (16-bit types: rows 8 g + 0..3
 // and + 4..7 of column i, g = lane / 16), columns 16 ct ..; fp32: 8 rows a step, row g and 4 + g.
 template <typename T, int DC> struct at_cols16 {
