@@ -48,6 +48,10 @@ def _heads_view(t):
     """`t` as (tensor, strides of sequence, token and head) the kernels can address: dense heads, everything on 16-byte
     boundaries (slices of a wider projection qualify, and expanded dimensions).  Anything else is copied."""
     es = t.element_size()
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        _, T, H, D = t.shape
+        if H * D * es < _MAX_STRIDE_BYTES:
+            return t, (T * H * D, H * D, D)
     st = [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
     if t.stride(3) != 1 or t.data_ptr() % 16 or any(s * es % 16 for s in st) or max(st[1:]) * es >= _MAX_STRIDE_BYTES \
             or t.shape[2] * st[2] * es >= _MAX_SPAN_BYTES:
@@ -121,8 +125,8 @@ def _norm_rotate_raw(s):
     dev = s.q.device
     dq, dk, tail = s.describe()
     with _on_device(dev):
-        yq = torch.empty(s.q.shape, dtype=s.q.dtype, device=dev)
-        yk = None if s.k is None else torch.empty(s.k.shape, dtype=s.k.dtype, device=dev)
+        yq = torch.empty_like(s.q, memory_format=torch.contiguous_format)
+        yk = None if s.k is None else torch.empty_like(s.k, memory_format=torch.contiguous_format)
         rc = lib.rc_qk_norm_rotate_fwd(dq, dk, yq.data_ptr(), None if yk is None else yk.data_ptr(), s.q.shape[0],
                                        s.q.shape[3], *tail, _stream(dev))
         if rc:
@@ -250,7 +254,7 @@ def _attention_raw(q, k, v, strides, key_mask, key_lengths, scale, want_lse):
     N, Tq, Hq, _ = q.shape
     a = _attn_desc(q, k, v, strides, key_mask, key_lengths, scale)
     with _on_device(dev):
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = torch.empty((N, Hq, Tq), dtype=torch.float32, device=dev) if want_lse else None
         work = _work(lib.rc_cross_attn_fwd_work_bytes(a), "rc_cross_attn_fwd_work_bytes", dev)
         rc = lib.rc_cross_attn_fwd(a, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),

@@ -51,6 +51,22 @@ struct at_args {
   float scale, scale_log2;
 };
 
+// Raises KERNEL's limit of dynamic LDS, once per device (the call is idempotent, so racing first calls are harmless).
+template <auto KERNEL> int at_allow_lds(int bytes) {
+  static bool done[64];
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e == hipSuccess && dev >= 0 && dev < 64 && done[dev]) return RC_OK;
+  if (e == hipSuccess)
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) {
+    rc_set_error("rc_cross_attn: %d bytes of LDS refused: %s", bytes, hipGetErrorString(e));
+    return (int)e;
+  }
+  if (dev >= 0 && dev < 64) done[dev] = true;
+  return RC_OK;
+}
+
 // host side (attention_rows.hip): the backward pass in one kernel where a sequence's keys fit a workgroup
 bool at_rows_fit(const rc_attn* a);
 int at_rows_bwd(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, const void* out,
@@ -419,6 +435,8 @@ struct at_order {
   int32_t units;
   __host__ at_order(int64_t N, int64_t Hk, int64_t items_of_head)
       : subs((uint32_t)(N >= 16 ? Hk * items_of_head : items_of_head)), units((int32_t)(N >= 16 ? N : N * Hk)) {}
+  // units that are given
+  __host__ at_order(int64_t units_, int64_t subs_) : subs((uint32_t)subs_), units((int32_t)units_) {}
   __host__ uint32_t grid() const {
     return (uint32_t)(8 * ((int64_t)(units / 8) * subs.d + ((int64_t)(units % 8) * subs.d + 7) / 8));
   }

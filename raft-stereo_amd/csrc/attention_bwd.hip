@@ -353,14 +353,6 @@ at_bwd_plan at_make_bwd_plan(const rc_attn* a) {
   return p;
 }
 
-template <typename K> int at_allow_lds(K kernel, int bytes) {
-  if (bytes <= 64 * 1024) return RC_OK;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == hipSuccess) return RC_OK;
-  rc_set_error("rc_cross_attn_bwd: %d bytes of LDS refused: %s", bytes, hipGetErrorString(e));
-  return (int)e;
-}
-
 struct at_bwd_call {
   const rc_attn* a;
   at_args d;
@@ -376,8 +368,8 @@ template <typename T, int DC, int HALVES, int NRB, bool DO_K, bool DO_V, int OCC
   constexpr int RT = 32 * NRB;
   using L = at_dkv_lds<T, DC, RT, 4, HALVES>;
   static_assert(L::BYTES <= 160 * 1024, "LDS");
-  auto kernel = at_dkv_kernel<T, DC, 4, HALVES, NRB, DO_K, DO_V, OCC>;
-  int rc = at_allow_lds(kernel, L::BYTES);
+  constexpr auto kernel = at_dkv_kernel<T, DC, 4, HALVES, NRB, DO_K, DO_V, OCC>;
+  int rc = at_allow_lds<kernel>(L::BYTES);
   if (rc) return rc;
   const int64_t row_tiles = (c.a->Tq + RT - 1) / RT, all = row_tiles * c.d.G;
   at_parts sp = {};
@@ -409,8 +401,8 @@ template <typename T, int DC> int at_bwd(const at_bwd_call& c) {
   if (c.p.q_items) {  // (the gradients of keys and values need delta)
     constexpr int bytes = at_dq_lds<T, DC, 32 * NB, 4>::BYTES;
     static_assert(bytes <= 160 * 1024, "LDS");
-    auto kernel = at_dq_kernel<T, DC, 4, NB, OCC>;
-    if ((rc = at_allow_lds(kernel, bytes))) return rc;
+    constexpr auto kernel = at_dq_kernel<T, DC, 4, NB, OCC>;
+    if ((rc = at_allow_lds<kernel>(bytes))) return rc;
     at_parts sp = {};
     sp.n = c.p.q_splits;
     sp.per = c.p.q_per;

@@ -43,12 +43,24 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
   using R = at_row<T, DC>;
   constexpr int NDB = DC / 32;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-  // rows fastest, then splits, then heads and sequences
-  const int item = order.item();
+  int item = order.item();
   if (item < 0) return;
-  const int rest = by_tiles.of(item), rt = item - rest * (int)by_tiles.d;
-  const int nh = by_splits.of(rest), split = rest - nh * (int)by_splits.d;
-  const int n = a.by_Hk.of(nh), hk = nh - n * a.Hk;
+  int rt = 0, split, n, hk;
+  if constexpr (NWK > 1) {
+    // few rows: heads fastest, then splits, then sequences
+    const int rest = a.by_Hk.of(item);
+    hk = item - rest * a.Hk;
+    n = by_splits.of(rest);
+    split = rest - n * (int)by_splits.d;
+    item = (n * a.Hk + hk) * (int)by_splits.d + split;
+  } else {
+    // rows fastest, then splits, then heads and sequences
+    const int rest = by_tiles.of(item), nh = by_splits.of(rest);
+    rt = item - rest * (int)by_tiles.d;
+    split = rest - nh * (int)by_splits.d;
+    n = a.by_Hk.of(nh);
+    hk = nh - n * a.Hk;
+  }
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wq = wave % NWQ, wk = wave / NWQ;
@@ -304,37 +316,60 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
     lse[((int64_t)n * a.Hq + hq) * a.Tq + t] = any ? m + __builtin_amdgcn_logf(l) : INFINITY;
 }
 
-// Joins the splits: a wave per row, weights exp2(m_i - max).
+// Joins the splits: a wave per row.  The lanes take a split's maximum and sum each, the weights exp2(m_i - max) go to LDS;
+// then a group of D / 4 lanes takes four elements each of every (64 / group)th split, many loads in flight.
+constexpr int AT_MOST_SPLITS = 512;
+
 template <typename T>
 __global__ __launch_bounds__(256) void at_join_kernel(T* __restrict__ out, float* __restrict__ lse, at_split sp, at_args a,
-                                                      int row_tiles, int tile_rows, int64_t all_rows) {
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= all_rows) return;
-  const int lane = threadIdx.x & 63;
-  const int64_t nh = i / ((int64_t)a.Tq * a.G);
-  const int row = (int)(i - nh * ((int64_t)a.Tq * a.G));
-  const int rt = row / tile_rows, r = row - rt * tile_rows;
-  const int64_t item0 = nh * sp.n * row_tiles + rt;  // + split * row_tiles
-  float top = -INFINITY, l = 0.0f;
-  for (int s = 0; s < sp.n; ++s) top = fmaxf(top, sp.ml[(item0 + (int64_t)s * row_tiles) * 2 * tile_rows + r]);
-  float acc[4] = {0, 0, 0, 0};
-  for (int s = 0; s < sp.n; ++s) {
-    const int64_t item = item0 + (int64_t)s * row_tiles;
-    const float mi = sp.ml[item * 2 * tile_rows + r], li = sp.ml[item * 2 * tile_rows + tile_rows + r];
-    if (li == 0.0f) continue;  // no key in this split
-    const float w = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - top);
-    l += w * li;
-    const float* o = sp.o + (item * tile_rows + r) * a.D;
+                                                      at_div by_rows, at_div by_tile_rows, int row_tiles, int64_t all_rows) {
+  __shared__ float weights[4][AT_MOST_SPLITS];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t i = (int64_t)blockIdx.x * 4 + wave;
+  if (i >= all_rows) return;  // (a wave joins its row alone)
+  const int nh = by_rows.of((int)i), row = (int)i - nh * (int)by_rows.d;
+  const int tile_rows = (int)by_tile_rows.d, rt = by_tile_rows.of(row), r = row - rt * tile_rows;
+  const int64_t item0 = (int64_t)nh * sp.n * row_tiles + rt;  // + split * row_tiles
+  float top = -INFINITY;
+  for (int s = lane; s < sp.n; s += 64) top = fmaxf(top, sp.ml[(item0 + (int64_t)s * row_tiles) * 2 * tile_rows + r]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (lane * 4 + e < a.D) acc[e] += w * o[lane * 4 + e];
+  for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+  float l = 0.0f;
+  for (int s = lane; s < sp.n; s += 64) {
+    const float* ml = sp.ml + (item0 + (int64_t)s * row_tiles) * 2 * tile_rows + r;
+    const float mi = ml[0], li = ml[tile_rows];
+    // (sum 0: no key in this split)
+    const float w = li == 0.0f || mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - top);
+    weights[wave][s] = w;
+    l += li == 0.0f ? 0.0f : mi == -INFINITY ? li * 0.0f : w * li;  // (a NaN stays one)
   }
-  const int n = (int)(nh / a.Hk), hk = (int)(nh - (int64_t)n * a.Hk), t = row / a.G, hq = hk * a.G + row - t * a.G;
-  const bool none = l == 0.0f;
-  T* o = out + (((int64_t)n * a.Tq + t) * a.Hq + hq) * a.D + lane * 4;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (lane * 4 + e < a.D) o[e] = rc_from_float<T>(none ? 0.0f : acc[e] / l);
+  for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x);
+  const bool none = l == 0.0f;
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  int group = 2;  // lanes of a group: D / 4 rounded up to a power of two
+  while (group * 4 < a.D) group *= 2;
+  const int e = (lane & (group - 1)) * 4, part = lane / group, parts = 64 / group;
+  at_f4 acc = (at_f4)(0.0f);
+  if (e < a.D && !none) {
+    const float* o = sp.o + (item0 * tile_rows + r) * a.D + e;
+    const int64_t step = (int64_t)row_tiles * tile_rows * a.D;
+#pragma unroll 8
+    for (int s = part; s < sp.n; s += parts) {
+      const float w = weights[wave][s];
+      if (w != 0.0f) acc += w * *reinterpret_cast<const at_f4*>(o + s * step);
+    }
+  }
+  for (int x = group; x < 64; x <<= 1)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) acc[y] += __shfl_xor(acc[y], x);
+  const int n = a.by_Hk.of(nh), hk = nh - n * a.Hk, t = a.by_G.of(row), hq = hk * a.G + row - t * a.G;
+  if (e < a.D && part == 0) {
+    const float f = none ? 0.0f : 1.0f / l;
+    T* p = out + (((int64_t)n * a.Tq + t) * a.Hq + hq) * a.D + e;
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<at_u2*>(p) = at_u2{at_pack(T(), acc[0] * f, acc[1] * f), at_pack(T(), acc[2] * f, acc[3] * f)};
+    else *reinterpret_cast<at_f4*>(p) = acc * f;
+  }
   if (lse != nullptr && lane == 0) lse[((int64_t)n * a.Hq + hq) * a.Tq + t] = none ? INFINITY : top + __builtin_amdgcn_logf(l);
 }
 
@@ -355,22 +390,19 @@ int at_launch(const rc_attn* a, const at_args& d, const void* q, const void* k, 
   using C = at_fwd_cfg<T, DC, NWQ, NWK, NKB>;
   constexpr int lds = NWK > 1 && C::WAVES * (64 + DC / 32 * 1024 + 4) * 4 > C::LDS ? C::WAVES * (64 + DC / 32 * 1024 + 4) * 4 : C::LDS;
   static_assert(lds <= 160 * 1024, "LDS");
-  auto kernel = at_fwd_kernel<T, DC, NWQ, NWK, NKB, AHEAD, OCC>;
-  if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) {
-      rc_set_error("rc_cross_attn_fwd: %d bytes of LDS refused: %s", lds, hipGetErrorString(e));
-      return (int)e;
-    }
-  }
+  constexpr auto kernel = at_fwd_kernel<T, DC, NWQ, NWK, NKB, AHEAD, OCC>;
+  int rc = at_allow_lds<kernel>(lds);
+  if (rc) return rc;
   const int64_t rows = a->Tq * d.G, row_tiles = (rows + C::ROWS - 1) / C::ROWS;
-  const at_order order(a->N, a->Hk, sp.n * row_tiles);
+  // few rows: nothing is read twice, and the heads of a split, which may share cache lines, are all that stays together
+  const at_order order = NWK > 1 ? at_order(a->N * sp.n, a->Hk) : at_order(a->N, a->Hk, sp.n * row_tiles);
   kernel<<<order.grid(), 64 * C::WAVES, lds, st>>>((const T*)q, (const T*)k, (const T*)v, (T*)out, lse, sp, d,
                                                 order, at_div((uint32_t)row_tiles), at_div((uint32_t)sp.n));
-  int rc = rc_check_launch("rc_cross_attn_fwd");
+  rc = rc_check_launch("rc_cross_attn_fwd");
   if (rc || sp.n == 1) return rc;
   const int64_t all = a->N * a->Hk * rows;
-  at_join_kernel<T><<<(uint32_t)((all + 3) / 4), 256, 0, st>>>((T*)out, lse, sp, d, (int)row_tiles, C::ROWS, all);
+  at_join_kernel<T><<<(uint32_t)((all + 3) / 4), 256, 0, st>>>((T*)out, lse, sp, d, at_div((uint32_t)rows), at_div(C::ROWS),
+                                                               (int)row_tiles, all);
   return rc_check_launch("rc_cross_attn_fwd (join)");
 }
 
@@ -391,12 +423,15 @@ at_plan at_make_plan(const rc_attn* a) {
   p.tile_rows = p.few ? 32 : 128;
   p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   p.items = a->N * a->Hk * p.row_tiles;
-  // fewer work items than fill the card twice: the keys are divided too, down to 256 of them
+  // Fewer work items than fill the card twice: the keys are divided too, down to 256 of them.  (One token in each of 16
+  // sequences, 8192 ragged keys, 32/8 heads of 128: 84 us; one over 16384 keys, 8/1 heads: 21 us, in splits of 1024 keys
+  // 29.)  Up to 1024 keys few rows stay whole: joining is a launch more (1000 keys: 14.7 against 18.9 us a call).
   int64_t n = 1;
-  if (p.items > 0 && p.items < 512) {
+  if (p.items > 0 && p.items < 512 && !(p.few && a->Tk <= 1024)) {
     n = (512 + p.items - 1) / p.items;
     const int64_t most = (a->Tk + 255) / 256;
     n = n < most ? n : most;
+    n = n < AT_MOST_SPLITS ? n : AT_MOST_SPLITS;
     n = n < 1 ? 1 : n;
   }
   const int64_t keys = ((a->Tk + n - 1) / n + 255) / 256 * 256;
@@ -409,9 +444,11 @@ at_plan at_make_plan(const rc_attn* a) {
 template <typename T, int DC>
 int at_run(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, void* out, float* lse,
            const at_plan& p, hipStream_t st) {
-  // waves of an item's keys, keys of a wave in a tile, resident workgroups: what registers and 160 KiB of LDS allow
+  // waves of an item's keys, blocks of keys of a wave in a tile, resident workgroups: what registers and 160 KiB of LDS
+  // allow.  Few rows: two workgroups per CU, so that one streams while the other starts or ends (D 128: two waves a
+  // workgroup; with four, and one workgroup, 8192 ragged keys took 110 instead of 84 us)
   constexpr int RB = at_row<T, DC>::RB;
-  constexpr int NWK = RB >= 1024 ? 1 : RB >= 512 ? 2 : 4;
+  constexpr int NWK = RB >= 1024 ? 1 : RB >= 256 ? 2 : 4;
   constexpr int NKB = RB >= 512 ? 1 : 2;
   constexpr int OCC = RB >= 1024 ? 1 : DC * (int)sizeof(T) >= 192 ? 2 : 3;
   // AHEAD: 16-bit heads of 96 and 128 (8 x 2047 x 4095, 16/4 heads of 128: 620 against 680 us, 800 x 800: 122 against

@@ -229,14 +229,9 @@ int at_launch_rows(const rc_attn* a, const at_args& d, const void* q, const void
                    const float* lse, const void* dout, void* dq, void* dk, void* dv, hipStream_t st) {
   using L = at_rows_lds<T, DC, NW>;
   static_assert(L::BYTES <= 160 * 1024, "LDS");
-  auto kernel = at_rows_kernel<T, DC, NW, OCC>;
-  if (L::BYTES > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
-    if (e != hipSuccess) {
-      rc_set_error("rc_cross_attn_bwd: %d bytes of LDS refused: %s", L::BYTES, hipGetErrorString(e));
-      return (int)e;
-    }
-  }
+  constexpr auto kernel = at_rows_kernel<T, DC, NW, OCC>;
+  const int rc = at_allow_lds<kernel>(L::BYTES);
+  if (rc) return rc;
   const at_order order(a->N, a->Hk, 1);
   kernel<<<order.grid(), 64 * NW, L::BYTES, st>>>((const T*)q, (const T*)k, (const T*)v, (const T*)out, lse, (const T*)dout, (T*)dq,
                                                   (T*)dk, (T*)dv, d, order, at_div((uint32_t)((a->Tq + 32 * NW - 1) / (32 * NW))));
