@@ -31,7 +31,7 @@ template <typename T, int DC, int NW> struct at_rows_lds {
 template <typename T, int DC> struct at_cols16 {
   using R = at_row<T, DC>;
   uint32_t lo, hi;
-  __device__ __forceinline__ at_cols16(int ct, int lane) {
+  __device__ __forceinline__ void init(int ct, int lane) {
     const int i = lane & 15, g = lane >> 4;
     if constexpr (sizeof(T) == 2) {
       const int chunk = 2 * ct + ((i >> 1) & 1);
@@ -189,11 +189,16 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_rows_kernel(const T* __restri
       fit.template fit<NDB>(s, acck);
       at_mma_cols<T, DC>(at, qs, 0, s, acck);
       at_sync();
-      // dQ of these rows: blocks of 16 elements by 16 rows, in turn over the waves
-      for (int x = (wave + j) % NW; x < 4 * NDB; x += NW) {
+      // dQ of these rows: blocks of 16 elements by 16 rows.  (Their places are worked out here each time: there are no
+      // registers to keep them in.)
+      int ln = lane;
+      asm volatile("" : "+v"(ln));
+      for (int x = wave; x < 4 * NDB; x += NW) {
         if (16 * (x >> 1) >= a.D) break;
-        const at_cols16<T, DC> ka(x >> 1, lane);
-        const at_cols16<T, 32> sb(x & 1, lane);
+        at_cols16<T, DC> ka;
+        at_cols16<T, 32> sb;
+        ka.init(x >> 1, ln);
+        sb.init(x & 1, ln);
         at_f4 acc = (at_f4)(0.0f);
         if constexpr (sizeof(T) == 2) {
 #pragma unroll 2
@@ -206,7 +211,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_rows_kernel(const T* __restri
             acc = __builtin_amdgcn_mfma_f32_16x16x4f32(u[1], w[1], acc, 0, 0, 0);
           }
         }
-        const int r = 16 * (x & 1) + (lane & 15), d = 16 * (x >> 1) + 4 * (lane >> 4), t = t0 + 32 * j + r;
+        const int r = 16 * (x & 1) + (ln & 15), d = 16 * (x >> 1) + 4 * (ln >> 4), t = t0 + 32 * j + r;
         float f = a.scale;
         if constexpr (FIT) f = f / (fr[r] * fv) * (1.0f / 4096.0f);
         T* o = dq + (((int64_t)n * a.Tq + t) * a.Hq + hq) * a.D + d;
@@ -248,14 +253,16 @@ int at_rows_waves(const rc_attn* a) {
 }
 
 template <typename T, int DC, typename... Args> int at_rows_nw(int waves, Args... args) {
-  constexpr bool WIDE = sizeof(T) == 4 && DC > 32;
-  if constexpr (!WIDE)
-    if (waves == 6) return at_launch_rows<T, DC, 6, 2>(args...);
+  // Waves per SIMD.  16-bit heads of 32: four, 128 registers.  (Six waves spread over the SIMDs as 2, 2, 1, 1: with room
+  // for three on each, a second workgroup often found no place, and 640 sequences of 180 took 215 instead of 155 us.)
+  constexpr int OCC = sizeof(T) == 2 && DC == 32 ? 4 : sizeof(T) == 4 && DC > 32 ? 1 : 2;
+  if constexpr (sizeof(T) == 2 || DC == 32)
+    if (waves == 6) return at_launch_rows<T, DC, 6, OCC>(args...);
   if constexpr (sizeof(T) == 2)
-    if (waves == 8) return at_launch_rows<T, DC, 8, 2>(args...);
+    if (waves == 8) return at_launch_rows<T, DC, 8, 2>(args...);  // (one workgroup per CU: LDS)
   if constexpr (sizeof(T) == 2 && DC == 32)
     if (waves == 12) return at_launch_rows<T, DC, 12, 3>(args...);
-  return at_launch_rows<T, DC, 4, WIDE ? 1 : 2>(args...);
+  return at_launch_rows<T, DC, 4, OCC>(args...);
 }
 
 }  // namespace

@@ -287,10 +287,17 @@ __global__ __launch_bounds__(NR_THREADS) void nr_weight_sum_kernel(const float* 
   const int e = threadIdx.x % 8, r0 = threadIdx.x / 8;
   const int d = ((int)blockIdx.x - (is_k ? slices : 0)) * 8 + e;
   double sum = 0.0;
-  for (uint32_t r = r0; r < rows; r += 32) sum += (double)p[(int64_t)r * D + d];
+  for (uint32_t r = r0; r < rows; r += 32 * 16) {  // sixteen loads in flight
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = r + 32 * i < rows ? p[(int64_t)(r + 32 * i) * D + d] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += (double)v[i];
+  }
   part[r0][e] = sum;
   __syncthreads();
   if (r0 == 0) {
+#pragma unroll
     for (int i = 1; i < 32; ++i) sum += part[i][e];
     out[d] = (float)sum;
   }
@@ -427,7 +434,9 @@ extern "C" int rc_qk_norm_rotate_bwd(const rc_heads* q, const rc_heads* k, const
   RC_REQUIRE((dwq == nullptr && dwk == nullptr) || (work != nullptr && (uintptr_t)work % 16 == 0), RC_EINVAL,
              "rc_qk_norm_rotate_bwd: work is null or not aligned to 16 bytes");
   RC_REQUIRE(k != nullptr || dwk == nullptr, RC_EINVAL, "rc_qk_norm_rotate_bwd: dwk without keys");
-  const nr_side sq = nr_plan(q, dq, gq, N, D, NR_MAX_BLOCKS), sk = nr_plan(k, dk, gk, N, D, NR_MAX_BLOCKS);
+  // (two sides share the card: half the blocks each, so that both are resident at once, and half the rows to add up)
+  const uint32_t most = k == nullptr ? NR_MAX_BLOCKS : NR_MAX_BLOCKS / 2;
+  const nr_side sq = nr_plan(q, dq, gq, N, D, most), sk = nr_plan(k, dk, gk, N, D, most);
   const nr_common c = {freqs, freqs_f64, n_freqs, D, eps};
   float* pq = dwq ? reinterpret_cast<float*>(work) : nullptr;
   float* pk = dwk ? reinterpret_cast<float*>(work) + (int64_t)NR_MAX_BLOCKS * D : nullptr;
