@@ -9,8 +9,6 @@ the reference: f1^T f2 / sqrt(D), the rows of one image wider than the other's a
 half.  The reference has no counterpart.  Operands are sequences of heads [N, T, H, D]; the projections around them are
 torch's, like the convolutions of the update block.  There is no CPU or eager fallback: tensors must live on a GPU.
 """
-import ctypes
-
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -81,9 +79,9 @@ def _check_weight(w, x, what):
 
 
 def _check_pos(pos, x, what):
-    """Positions as (tensor, elements between two sequences)."""
+    """Positions whose tokens lie side by side."""
     if pos is None:
-        return None, 0
+        return None
     if pos.dtype not in _POS:
         raise TypeError(f"{what} must be int32, int64 or float32, got {pos.dtype}")
     if pos.device != x.device:
@@ -91,12 +89,10 @@ def _check_pos(pos, x, what):
     N, T = x.shape[:2]
     if tuple(pos.shape) not in ((T,), (N, T)):
         raise ValueError(f"{what} must be [{T}] or [{N}, {T}], got {tuple(pos.shape)}")
-    if T > 1 and pos.stride(-1) != 1:
-        pos = pos.contiguous()
-    return pos, (pos.stride(0) if pos.dim() == 2 and N > 1 else 0)
+    return pos.contiguous() if T > 1 and pos.stride(-1) != 1 else pos
 
 
-def _heads_desc(x, st, weight, pos, pos_stride):
+def _heads_desc(x, st, weight, pos):
     d = Heads()
     d.x = x.data_ptr()
     d.T, d.H = x.shape[1], x.shape[2]
@@ -104,77 +100,78 @@ def _heads_desc(x, st, weight, pos, pos_stride):
     if weight is not None:
         d.weight, d.weight_dtype = weight.data_ptr(), _DT[weight.dtype]
     if pos is not None:
-        d.pos, d.pos_dtype, d.pos_stride = pos.data_ptr(), _POS[pos.dtype], pos_stride
+        d.pos, d.pos_dtype = pos.data_ptr(), _POS[pos.dtype]
+        d.pos_stride = pos.stride(0) if pos.dim() == 2 and x.shape[0] > 1 else 0
     return d
 
 
-class _Sides:
-    """The checked operands of one norm + rotation call, as the library takes them."""
-    __slots__ = ("q", "k", "q_st", "k_st", "qw", "kw", "q_pos", "k_pos", "q_ps", "k_ps", "freqs", "eps", "interleaved")
+def _norm_rotate_desc(q, k, q_weight, k_weight, freqs, q_pos, k_pos, rest):
+    """The operands as the library takes them, and q and k as they are described (copies, where they have to be)."""
+    eps, interleaved = rest
+    q, st = _heads_view(q)
+    desc_q = _heads_desc(q, st, q_weight, q_pos)
+    desc_k = None
+    if k is not None:
+        k, st = _heads_view(k)
+        desc_k = _heads_desc(k, st, k_weight, k_pos)
+    tail = (_DT[q.dtype], None if freqs is None else freqs.data_ptr(), int(freqs is not None and freqs.dtype is torch.float64),
+            0 if freqs is None else freqs.shape[0], interleaved, eps)
+    return q, k, desc_q, desc_k, tail
 
-    def describe(self):
-        dq = _heads_desc(self.q, self.q_st, self.qw, self.q_pos, self.q_ps)
-        dk = None if self.k is None else _heads_desc(self.k, self.k_st, self.kw, self.k_pos, self.k_ps)
-        fr = self.freqs
-        tail = (_DT[self.q.dtype], None if fr is None else fr.data_ptr(), int(fr is not None and fr.dtype is torch.float64),
-                0 if fr is None else fr.shape[0], int(self.interleaved), self.eps)
-        return dq, dk, tail
 
-
-def _norm_rotate_raw(s):
-    dev = s.q.device
-    dq, dk, tail = s.describe()
+def _norm_rotate_raw(q, k, desc_q, desc_k, tail):
+    dev = q.device
     with _on_device(dev):
-        yq = torch.empty_like(s.q, memory_format=torch.contiguous_format)
-        yk = None if s.k is None else torch.empty_like(s.k, memory_format=torch.contiguous_format)
-        rc = lib.rc_qk_norm_rotate_fwd(dq, dk, yq.data_ptr(), None if yk is None else yk.data_ptr(), s.q.shape[0],
-                                       s.q.shape[3], *tail, _stream(dev))
+        yq = torch.empty_like(q, memory_format=torch.contiguous_format)
+        yk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
+        rc = lib.rc_qk_norm_rotate_fwd(desc_q, desc_k, yq.data_ptr(), None if yk is None else yk.data_ptr(), q.shape[0],
+                                       q.shape[3], *tail, _stream(dev))
         if rc:
             check(rc, "rc_qk_norm_rotate_fwd")
     return yq, yk
 
 
 class _NormRotateFn(torch.autograd.Function):
-    """Keeps its inputs for the backward pass, which works the norm out again."""
+    """Keeps its inputs for the backward pass, which works the norm out again.  (They are described again there: a hook
+    on saved tensors may have moved them.)"""
 
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, s):
-        s.q, s.k, s.qw, s.kw = q, k, q_weight, k_weight
-        yq, yk = _norm_rotate_raw(s)
-        ctx.save_for_backward(q, k, q_weight, k_weight, s.freqs, s.q_pos, s.k_pos)
-        ctx.rest = (s.q_st, s.k_st, s.q_ps, s.k_ps, s.eps, s.interleaved)
-        s.q = s.k = s.qw = s.kw = s.freqs = s.q_pos = s.k_pos = None
+    def forward(ctx, q, k, q_weight, k_weight, freqs, q_pos, k_pos, rest):
+        ctx.save_for_backward(q, k, q_weight, k_weight, freqs, q_pos, k_pos)
+        ctx.rest = rest
         ctx.set_materialize_grads(False)
-        return yq, yk
+        return _norm_rotate_raw(*_norm_rotate_desc(q, k, q_weight, k_weight, freqs, q_pos, k_pos, rest))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
-        s = _Sides()
-        s.q, s.k, s.qw, s.kw, s.freqs, s.q_pos, s.k_pos = ctx.saved_tensors
-        s.q_st, s.k_st, s.q_ps, s.k_ps, s.eps, s.interleaved = ctx.rest
         if gq is None and gk is None:
-            return None, None, None, None, None
-        dev, D = s.q.device, s.q.shape[3]
+            return (None,) * 8
+        q, k, qw, kw, freqs, q_pos, k_pos = ctx.saved_tensors
+        q, k, desc_q, desc_k, tail = _norm_rotate_desc(q, k, qw, kw, freqs, q_pos, k_pos, ctx.rest)
+        dev, D = q.device, q.shape[3]
         want = ctx.needs_input_grad
-        gq = torch.zeros(s.q.shape, dtype=s.q.dtype, device=dev) if gq is None else _dense(gq)
-        if s.k is not None:
-            gk = torch.zeros(s.k.shape, dtype=s.k.dtype, device=dev) if gk is None else _dense(gk)
-        dq_desc, dk_desc, tail = s.describe()
         with _on_device(dev):
-            dq = torch.empty(s.q.shape, dtype=s.q.dtype, device=dev)
-            dk = None if s.k is None else torch.empty(s.k.shape, dtype=s.k.dtype, device=dev)
-            dwq = torch.empty(D, dtype=torch.float32, device=dev) if s.qw is not None and want[2] else None
-            dwk = torch.empty(D, dtype=torch.float32, device=dev) if s.kw is not None and want[3] else None
-            work = None
+            gq = torch.zeros(q.shape, dtype=q.dtype, device=dev) if gq is None else _dense(gq)
+            dq = torch.empty_like(gq)
+            gk_ptr = dk = dk_ptr = dwq = dwk = dwq_ptr = dwk_ptr = work_ptr = None
+            if k is not None:
+                gk = torch.zeros(k.shape, dtype=k.dtype, device=dev) if gk is None else _dense(gk)
+                dk = torch.empty_like(gk)
+                gk_ptr, dk_ptr = gk.data_ptr(), dk.data_ptr()
+            if qw is not None and want[2]:
+                dwq = torch.empty(D, dtype=torch.float32, device=dev)
+                dwq_ptr = dwq.data_ptr()
+            if kw is not None and want[3]:
+                dwk = torch.empty(D, dtype=torch.float32, device=dev)
+                dwk_ptr = dwk.data_ptr()
             if dwq is not None or dwk is not None:
                 work = torch.empty(int(lib.rc_qk_norm_rotate_bwd_work_bytes(D)), dtype=torch.uint8, device=dev)
-            ptr = lambda t: None if t is None else t.data_ptr()
-            check(lib.rc_qk_norm_rotate_bwd(dq_desc, dk_desc, gq.data_ptr(), ptr(gk), dq.data_ptr(), ptr(dk), ptr(dwq),
-                                            ptr(dwk), ptr(work), s.q.shape[0], D, *tail, _stream(dev)),
-                  "rc_qk_norm_rotate_bwd")
-        cast = lambda d, w: None if d is None else d.to(w.dtype)
-        return dq, dk, cast(dwq, s.qw), cast(dwk, s.kw), None
+                work_ptr = work.data_ptr()
+            check(lib.rc_qk_norm_rotate_bwd(desc_q, desc_k, gq.data_ptr(), gk_ptr, dq.data_ptr(), dk_ptr, dwq_ptr, dwk_ptr,
+                                            work_ptr, q.shape[0], D, *tail, _stream(dev)), "rc_qk_norm_rotate_bwd")
+        return (dq, dk, None if dwq is None else dwq.to(qw.dtype), None if dwk is None else dwk.to(kw.dtype),
+                None, None, None, None)
 
 
 def qk_norm_rotate_hip(q, k=None, q_weight=None, k_weight=None, freqs=None, q_pos=None, k_pos=None, eps=1e-6,
@@ -211,36 +208,33 @@ def qk_norm_rotate_hip(q, k=None, q_weight=None, k_weight=None, freqs=None, q_po
         raise ValueError("positions need freqs")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    s = _Sides()
-    s.freqs, s.eps, s.interleaved = freqs, float(eps), bool(interleaved)
-    s.q_pos, s.q_ps = _check_pos(q_pos, q, "q_pos")
-    s.k_pos, s.k_ps = (None, 0) if k is None else _check_pos(k_pos, k, "k_pos")
-    # views are taken here, so that autograd carries the gradient of a copy back through torch's own clone
-    q, s.q_st = _heads_view(q)
-    k, s.k_st = (None, None) if k is None else _heads_view(k)
+    q_pos = _check_pos(q_pos, q, "q_pos")
+    k_pos = None if k is None else _check_pos(k_pos, k, "k_pos")
     q_weight = None if q_weight is None else q_weight.contiguous()
     k_weight = None if k_weight is None else k_weight.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        yq, yk = _NormRotateFn.apply(q, k, q_weight, k_weight, s)
+    args = (q, k, q_weight, k_weight, freqs, q_pos, k_pos, (float(eps), int(bool(interleaved))))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+        yq, yk = _NormRotateFn.apply(*args)
     else:
-        s.q, s.k, s.qw, s.kw = q, k, q_weight, k_weight
-        yq, yk = _norm_rotate_raw(s)
+        yq, yk = _norm_rotate_raw(*_norm_rotate_desc(*args))
     return yq if k is None else (yq, yk)
 
 
 # ------------------------------------------------------------------------------------------------ cross attention
-def _attn_desc(q, k, v, strides, key_mask, key_lengths, scale):
+def _attn_desc(q, k, v, key_mask, key_lengths, scale):
+    """The operands as the library takes them, and q, k and v as they are described (copies, where they have to be)."""
+    (q, qs), (k, ks), (v, vs) = _heads_view(q), _heads_view(k), _heads_view(v)
     a = Attn()
     N, a.Tq, a.Hq, a.D = q.shape
     a.N, a.Tk, a.Hk = N, k.shape[1], k.shape[2]
     a.dtype, a.scale = _DT[q.dtype], scale
-    for dst, st in zip((a.q_stride, a.k_stride, a.v_stride), strides):
+    for dst, st in ((a.q_stride, qs), (a.k_stride, ks), (a.v_stride, vs)):
         dst[0], dst[1], dst[2] = st
     if key_mask is not None:
         a.key_mask, a.mask_stride = key_mask.data_ptr(), key_mask.stride(0) if N > 1 else 0
     if key_lengths is not None:
         a.key_lengths, a.lengths_i64 = key_lengths.data_ptr(), int(key_lengths.dtype is torch.int64)
-    return a
+    return a, q, k, v
 
 
 def _work(nbytes, what, dev):
@@ -249,10 +243,9 @@ def _work(nbytes, what, dev):
     return torch.empty(int(nbytes), dtype=torch.uint8, device=dev) if nbytes else None
 
 
-def _attention_raw(q, k, v, strides, key_mask, key_lengths, scale, want_lse):
+def _attention_raw(a, q, k, v, want_lse):
     dev = q.device
     N, Tq, Hq, _ = q.shape
-    a = _attn_desc(q, k, v, strides, key_mask, key_lengths, scale)
     with _on_device(dev):
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = torch.empty((N, Hq, Tq), dtype=torch.float32, device=dev) if want_lse else None
@@ -266,33 +259,34 @@ def _attention_raw(q, k, v, strides, key_mask, key_lengths, scale, want_lse):
 
 
 class _CrossAttentionFn(torch.autograd.Function):
-    """Keeps the operands, the result and each row's log-sum-exp; the backward pass works the scores out again."""
+    """Keeps the operands, the result and each row's log-sum-exp; the backward pass works the scores out again.  (The
+    operands are described again there: a hook on saved tensors may have moved them.)"""
 
     @staticmethod
-    def forward(ctx, q, k, v, strides, key_mask, key_lengths, scale):
-        out, lse = _attention_raw(q, k, v, strides, key_mask, key_lengths, scale, True)
+    def forward(ctx, q, k, v, key_mask, key_lengths, scale):
+        out, lse = _attention_raw(*_attn_desc(q, k, v, key_mask, key_lengths, scale), True)
         ctx.save_for_backward(q, k, v, out, lse, key_mask, key_lengths)
-        ctx.strides, ctx.scale = strides, scale
+        ctx.scale = scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
         q, k, v, out, lse, key_mask, key_lengths = ctx.saved_tensors
+        a, q, k, v = _attn_desc(q, k, v, key_mask, key_lengths, ctx.scale)
         dev = q.device
         g = _dense(grad_out)
-        a = _attn_desc(q, k, v, ctx.strides, key_mask, key_lengths, ctx.scale)
         want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         with _on_device(dev):
-            dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if want_q else None
-            dk = torch.empty(k.shape, dtype=k.dtype, device=dev) if want_kv else None
-            dv = torch.empty(v.shape, dtype=v.dtype, device=dev) if want_kv else None
+            dq = torch.empty_like(g) if want_q else None
+            dk = torch.empty_like(k, memory_format=torch.contiguous_format) if want_kv else None
+            dv = torch.empty_like(v, memory_format=torch.contiguous_format) if want_kv else None
             work = _work(lib.rc_cross_attn_bwd_work_bytes(a), "rc_cross_attn_bwd_work_bytes", dev)
             ptr = lambda t: None if t is None else t.data_ptr()
             check(lib.rc_cross_attn_bwd(a, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
                                         g.data_ptr(), ptr(dq), ptr(dk), ptr(dv), ptr(work), _stream(dev)),
                   "rc_cross_attn_bwd")
-        return dq, dk, dv, None, None, None, None
+        return dq, dk, dv, None, None, None
 
 
 def cross_attention_hip(q, k, v, key_mask=None, key_lengths=None, scale=None):
@@ -335,11 +329,9 @@ def cross_attention_hip(q, k, v, key_mask=None, key_lengths=None, scale=None):
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    # views are taken here, so that autograd carries the gradient of a copy back through torch's own clone
-    (q, qs), (k, ks), (v, vs) = _heads_view(q), _heads_view(k), _heads_view(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _CrossAttentionFn.apply(q, k, v, (qs, ks, vs), key_mask, key_lengths, scale)
-    return _attention_raw(q, k, v, (qs, ks, vs), key_mask, key_lengths, scale, False)[0]
+        return _CrossAttentionFn.apply(q, k, v, key_mask, key_lengths, scale)
+    return _attention_raw(*_attn_desc(q, k, v, key_mask, key_lengths, scale), False)[0]
 
 
 # ------------------------------------------------------------------------------------------- rows of feature maps

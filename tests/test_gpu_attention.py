@@ -279,6 +279,29 @@ def test_attention_repeats_bit_for_bit_and_skips_unwanted_gradients(R):
         torch.autograd.grad(d.sum(), t)
 
 
+def test_gradients_where_saved_tensors_were_moved(R):
+    """Saved tensors that a hook has put elsewhere, with other strides, give the same gradients."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    wide = torch.randn((2, 40, 12, 64), generator=g, device="cuda").half()
+    pos = torch.randint(0, 1000, (2, 80), generator=g, device="cuda")[:, ::2]
+    mask = torch.rand((40, 2), generator=g, device="cuda").t() > 0.3
+    freqs, w = torch.linspace(0.01, 1.0, 32, device="cuda"), torch.ones(128, device="cuda")[::2]
+    go = torch.randn((2, 40, 4, 64), generator=g, device="cuda").half()
+
+    def grads(hooks):
+        leaf, wl = wide.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        with hooks:
+            q, k = R.qk_norm_rotate_hip(leaf[:, :, :4], leaf[:, :, 4:8], wl, wl, freqs, pos, pos)
+            out = R.cross_attention_hip(q, k, leaf[:, :, 8:], key_mask=mask)
+        junk = torch.full((64 << 20,), 7, dtype=torch.uint8, device="cuda")   # takes what the hooks have freed
+        res = torch.autograd.grad(out, (leaf, wl), go)
+        del junk
+        return res
+    import contextlib
+    for a, b in zip(grads(contextlib.nullcontext()), grads(torch.autograd.graph.save_on_cpu())):
+        assert torch.equal(a, b)
+
+
 def test_attention_refuses(R):
     x = torch.randn(2, 8, 4, 32, device="cuda")
     f = R.cross_attention_hip
