@@ -506,20 +506,22 @@ typedef struct rc_attn {
   float scale;                      /* positive and finite */
 } rc_attn;
 
-/* out [N, Tq, Hq, D]; lse float [N, Hq, Tq]: log-sum-exp of each row's scores in base 2 (scores times log2 e; +inf
- * for a row without a key), what the backward pass needs; NULL in inference.  work: rc_cross_attn_fwd_work_bytes()
+/* out [N, Tq, Hq, D].  For the backward pass, NULL in inference: lse float [N, Hq, Tq], the log-sum-exp of each row's
+ * scores in base 2 (scores times log2 e; +inf for a row without a key), and out_rest, of out's shape and type (16-bit
+ * types; may be NULL): what rounding took from out.  work: rc_cross_attn_fwd_work_bytes()
  * of scratch (0 in most cases: only a few query rows over many keys are split over workgroups); negative: *a is
  * invalid. */
 int64_t rc_cross_attn_fwd_work_bytes(const rc_attn* a);
-int rc_cross_attn_fwd(const rc_attn* a, const void* q, const void* k, const void* v, void* out, float* lse,
-                      void* work, void* stream);
-/* The adjoint: out and lse of the forward call, dout contiguous like out; dq [N, Tq, Hq, D], dk, dv [N, Tk, Hk, D]
+int rc_cross_attn_fwd(const rc_attn* a, const void* q, const void* k, const void* v, void* out,
+                      void* out_rest, float* lse, void* work, void* stream);
+/* The adjoint: out, out_rest and lse of the forward call (without out_rest the sum of dout * out that every score's
+ * gradient is taken against has out's rounding in it), dout contiguous like out; dq [N, Tq, Hq, D], dk, dv [N, Tk, Hk, D]
  * contiguous of `dtype`.  Gradients of a shared head are summed over its group in fp32; no atomics, reproducible run
  * to run.  dq may be NULL, and dk and dv together, where no gradient is wanted.  work: rc_cross_attn_bwd_work_bytes()
  * of scratch. */
 int64_t rc_cross_attn_bwd_work_bytes(const rc_attn* a);
 int rc_cross_attn_bwd(const rc_attn* a, const void* q, const void* k, const void* v, const void* out,
-                      const float* lse, const void* dout, void* dq, void* dk, void* dv, void* work,
+                      const void* out_rest, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* work,
                       void* stream);
 
 #ifdef __cplusplus

@@ -116,9 +116,9 @@ SIGNATURES = {
     "rc_qk_norm_rotate_bwd_work_bytes": (_L, [_I]),
     "rc_qk_norm_rotate_bwd": (_I, [_HP, _HP, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _P, _I, _I, _I, _F, _P]),
     "rc_cross_attn_fwd_work_bytes": (_L, [_ATP]),
-    "rc_cross_attn_fwd": (_I, [_ATP, _P, _P, _P, _P, _P, _P, _P]),
+    "rc_cross_attn_fwd": (_I, [_ATP, _P, _P, _P, _P, _P, _P, _P, _P]),
     "rc_cross_attn_bwd_work_bytes": (_L, [_ATP]),
-    "rc_cross_attn_bwd": (_I, [_ATP, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "rc_cross_attn_bwd": (_I, [_ATP, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
 }
 
 

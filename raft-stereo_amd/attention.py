@@ -243,36 +243,37 @@ def _work(nbytes, what, dev):
     return torch.empty(int(nbytes), dtype=torch.uint8, device=dev) if nbytes else None
 
 
-def _attention_raw(a, q, k, v, want_lse):
+def _attention_raw(a, q, k, v, train):
     dev = q.device
     N, Tq, Hq, _ = q.shape
     with _on_device(dev):
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        lse = torch.empty((N, Hq, Tq), dtype=torch.float32, device=dev) if want_lse else None
+        lse = torch.empty((N, Hq, Tq), dtype=torch.float32, device=dev) if train else None
+        rest = torch.empty_like(out) if train and out.dtype is not torch.float32 else None
         work = _work(lib.rc_cross_attn_fwd_work_bytes(a), "rc_cross_attn_fwd_work_bytes", dev)
         rc = lib.rc_cross_attn_fwd(a, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                   None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(),
+                                   None if rest is None else rest.data_ptr(), None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(),
                                    _stream(dev))
         if rc:
             check(rc, "rc_cross_attn_fwd")
-    return out, lse
+    return out, rest, lse
 
 
 class _CrossAttentionFn(torch.autograd.Function):
-    """Keeps the operands, the result and each row's log-sum-exp; the backward pass works the scores out again.  (The
-    operands are described again there: a hook on saved tensors may have moved them.)"""
+    """Keeps the operands, the result (16-bit: with what rounding took from it) and each row's log-sum-exp; the backward
+    pass works the scores out again.  (The operands are described again there: a hook on saved tensors may have moved them.)"""
 
     @staticmethod
     def forward(ctx, q, k, v, key_mask, key_lengths, scale):
-        out, lse = _attention_raw(*_attn_desc(q, k, v, key_mask, key_lengths, scale), True)
-        ctx.save_for_backward(q, k, v, out, lse, key_mask, key_lengths)
+        out, rest, lse = _attention_raw(*_attn_desc(q, k, v, key_mask, key_lengths, scale), True)
+        ctx.save_for_backward(q, k, v, out, rest, lse, key_mask, key_lengths)
         ctx.scale = scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        q, k, v, out, lse, key_mask, key_lengths = ctx.saved_tensors
+        q, k, v, out, rest, lse, key_mask, key_lengths = ctx.saved_tensors
         a, q, k, v = _attn_desc(q, k, v, key_mask, key_lengths, ctx.scale)
         dev = q.device
         g = _dense(grad_out)
@@ -283,8 +284,8 @@ class _CrossAttentionFn(torch.autograd.Function):
             dv = torch.empty_like(v, memory_format=torch.contiguous_format) if want_kv else None
             work = _work(lib.rc_cross_attn_bwd_work_bytes(a), "rc_cross_attn_bwd_work_bytes", dev)
             ptr = lambda t: None if t is None else t.data_ptr()
-            check(lib.rc_cross_attn_bwd(a, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
-                                        g.data_ptr(), ptr(dq), ptr(dk), ptr(dv), ptr(work), _stream(dev)),
+            check(lib.rc_cross_attn_bwd(a, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr(rest),
+                                        lse.data_ptr(), g.data_ptr(), ptr(dq), ptr(dk), ptr(dv), ptr(work), _stream(dev)),
                   "rc_cross_attn_bwd")
         return dq, dk, dv, None, None, None
 

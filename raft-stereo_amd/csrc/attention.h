@@ -70,7 +70,7 @@ template <auto KERNEL> int at_allow_lds(int bytes) {
 // host side (attention_rows.hip): the backward pass in one kernel where a sequence's keys fit a workgroup
 bool at_rows_fit(const rc_attn* a);
 int at_rows_bwd(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, const void* out,
-                const float* lse, const void* dout, void* dq, void* dk, void* dv, hipStream_t st);
+                const void* rest, const float* lse, const void* dout, void* dq, void* dk, void* dv, hipStream_t st);
 // host side (attention_fwd.hip)
 int at_check(const rc_attn* a);
 int at_check_operand(const rc_attn* a, int64_t rows, const void* p);
@@ -175,6 +175,15 @@ __device__ __forceinline__ void at_swap(uint32_t& a, uint32_t& b) {
   a = r[0];
   b = r[1];
 }
+__device__ __forceinline__ at_f2 at_unpack(rc_half, uint32_t x) {
+  const at_h2 v = __builtin_bit_cast(at_h2, x);
+  return at_f2{(float)v[0], (float)v[1]};
+}
+__device__ __forceinline__ at_f2 at_unpack(rc_bf16, uint32_t x) {
+  const at_b2 v = __builtin_bit_cast(at_b2, x);
+  return at_f2{(float)v[0], (float)v[1]};
+}
+
 // both halves see their two values
 __device__ __forceinline__ void at_both(float x, float& lo, float& hi) {
   uint32_t a = __builtin_bit_cast(uint32_t, x), b = a;
@@ -452,9 +461,10 @@ struct at_order {
   }
 };
 
-// Writes a result (rows: elements 32 db .. of the head, column: this lane's row of memory at p) times f.
-template <typename T, int DC>
-__device__ __forceinline__ void at_store_rows(T* p, bool live, const at_f16* acc, float f, int D, int lane) {
+// Writes a result (rows: elements 32 db .. of the head, column: this lane's row of memory at p) times f; REST: and what
+// rounding took from it.
+template <typename T, int DC, bool REST = false>
+__device__ __forceinline__ void at_store_rows(T* p, bool live, const at_f16* acc, float f, int D, int lane, T* rest = nullptr) {
   const int h = lane >> 5;
 #pragma unroll
   for (int db = 0; db < DC / 32; ++db) {
@@ -463,17 +473,28 @@ __device__ __forceinline__ void at_store_rows(T* p, bool live, const at_f16* acc
       for (int b = 0; b < 2; ++b) {
         // registers 8 b .. + 3 hold elements 4 h + 0..3 of 16, the next four 8 + 4 h + 0..3: the halves swap, and each
         // lane has eight in a row
-        at_u4 w;
+        at_u4 w, r;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          uint32_t x = at_pack(T(), acc[db][8 * b + 2 * j] * f, acc[db][8 * b + 2 * j + 1] * f);
-          uint32_t y = at_pack(T(), acc[db][8 * b + 4 + 2 * j] * f, acc[db][8 * b + 5 + 2 * j] * f);
+          const at_f2 u = {acc[db][8 * b + 2 * j] * f, acc[db][8 * b + 2 * j + 1] * f};
+          const at_f2 v = {acc[db][8 * b + 4 + 2 * j] * f, acc[db][8 * b + 5 + 2 * j] * f};
+          uint32_t x = at_pack(T(), u[0], u[1]), y = at_pack(T(), v[0], v[1]);
+          if constexpr (REST) {
+            const at_f2 a = u - at_unpack(T(), x), c = v - at_unpack(T(), y);
+            uint32_t ra = at_pack(T(), a[0], a[1]), rc = at_pack(T(), c[0], c[1]);
+            at_swap(ra, rc);
+            r[j] = ra;
+            r[2 + j] = rc;
+          }
           at_swap(x, y);
           w[j] = x;
           w[2 + j] = y;
         }
         const int d = 32 * db + 16 * b + 8 * h;
-        if (live && d < D) *reinterpret_cast<at_u4*>(p + d) = w;
+        if (live && d < D) {
+          *reinterpret_cast<at_u4*>(p + d) = w;
+          if constexpr (REST) *reinterpret_cast<at_u4*>(rest + d) = r;
+        }
       }
     } else {
 #pragma unroll

@@ -30,7 +30,7 @@ template <typename T, int DC, int KT, int WAVES> struct at_dq_lds {
 template <typename T, int DC, int NW, int NKB, int OCC>
 __global__ __launch_bounds__(64 * NW, OCC) void at_dq_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                              const T* __restrict__ v, const T* __restrict__ out,
-                                                             const float* __restrict__ lse, const T* __restrict__ dout,
+                                                             const T* __restrict__ rest_out, const float* __restrict__ lse, const T* __restrict__ dout,
                                                              float* __restrict__ delta, T* __restrict__ dq, at_parts sp,
                                                              at_args a, at_order order, at_div by_tiles, at_div by_splits) {
   using R = at_row<T, DC>;
@@ -74,6 +74,14 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dq_kernel(const T* __restrict
     for (int s = 0; s < R::STEPS; ++s) {
       dl += at_dot(T(), of.chunk<T>(ooff, a.D, s, h), gf[s]);
       if (s % 8 == 7) asm volatile("" ::: "memory");  // (not all of the row at once: registers)
+    }
+    if (sizeof(T) == 2 && rest_out != nullptr) {
+      const at_rows_of rf(rest_out + obase);
+#pragma unroll
+      for (int s = 0; s < R::STEPS; ++s) {
+        dl += at_dot(T(), rf.chunk<T>(ooff, a.D, s, h), gf[s]);
+        if (s % 8 == 7) asm volatile("" ::: "memory");
+      }
     }
     dl = at_half_sum(dl);
     if (live && h == 0 && split == 0) delta[srow] = dl;
@@ -357,7 +365,7 @@ struct at_bwd_call {
   const rc_attn* a;
   at_args d;
   at_bwd_plan p;
-  const void *q, *k, *v, *out, *dout;
+  const void *q, *k, *v, *out, *rest, *dout;
   const float* lse;
   void *dq, *dk, *dv;
   float *delta, *parts;
@@ -409,7 +417,8 @@ template <typename T, int DC> int at_bwd(const at_bwd_call& c) {
     sp.p = c.parts;
     sp.part = c.a->N * c.a->Tq * c.a->Hq * c.a->D;
     const at_order order(c.a->N, c.a->Hk, c.p.q_tiles * sp.n);
-    kernel<<<order.grid(), 256, bytes, c.st>>>((const T*)c.q, (const T*)c.k, (const T*)c.v, (const T*)c.out, c.lse,
+    kernel<<<order.grid(), 256, bytes, c.st>>>((const T*)c.q, (const T*)c.k, (const T*)c.v, (const T*)c.out,
+                                                 (const T*)c.rest, c.lse,
                                                  (const T*)c.dout, c.delta, (T*)c.dq, sp, c.d, order,
                                                  at_div((uint32_t)c.p.q_tiles), at_div((uint32_t)sp.n));
     if ((rc = rc_check_launch("rc_cross_attn_bwd (queries)"))) return rc;
@@ -451,7 +460,7 @@ extern "C" int64_t rc_cross_attn_bwd_work_bytes(const rc_attn* a) {
 }
 
 extern "C" int rc_cross_attn_bwd(const rc_attn* a, const void* q, const void* k, const void* v, const void* out,
-                                 const float* lse, const void* dout, void* dq, void* dk, void* dv, void* work,
+                                 const void* rest, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* work,
                                  void* stream) {
   int rc = at_check(a);
   if (rc) return rc;
@@ -460,7 +469,7 @@ extern "C" int rc_cross_attn_bwd(const rc_attn* a, const void* q, const void* k,
   for (const void* p : {k, v})
     if ((rc = at_check_operand(a, a->N * a->Tk, p))) return rc;
   RC_REQUIRE((dk == nullptr) == (dv == nullptr), RC_EINVAL, "rc_cross_attn_bwd: dk and dv are wanted together or not at all");
-  RC_REQUIRE(((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) % 16 == 0, RC_EINVAL,
+  RC_REQUIRE(((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)rest) % 16 == 0, RC_EINVAL,
              "rc_cross_attn_bwd: a gradient is not aligned to 16 bytes");
   if (a->N == 0) return RC_OK;
   at_bwd_call c = {};
@@ -475,6 +484,7 @@ extern "C" int rc_cross_attn_bwd(const rc_attn* a, const void* q, const void* k,
   c.k = k;
   c.v = v;
   c.out = out;
+  c.rest = rest;
   c.dout = dout;
   c.lse = lse;
   c.dq = dq;
@@ -486,7 +496,7 @@ extern "C" int rc_cross_attn_bwd(const rc_attn* a, const void* q, const void* k,
   c.d = at_to_dev(a, work);
   if ((rc = at_launch_bits(a, work, c.st))) return rc;
   if (dq && dk && a->N * a->Tq && a->N * a->Tk && at_rows_fit(a))
-    return at_rows_bwd(a, c.d, q, k, v, out, lse, dout, dq, dk, dv, c.st);
+    return at_rows_bwd(a, c.d, q, k, v, out, rest, lse, dout, dq, dk, dv, c.st);
   if (a->dtype == RC_F32) return at_bwd_d<float>(c);
   if (a->dtype == RC_F16) return at_bwd_d<rc_half>(c);
   return at_bwd_d<rc_bf16>(c);

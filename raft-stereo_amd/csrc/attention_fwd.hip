@@ -37,7 +37,7 @@ template <typename T, int DC, int NWQ, int NWK, int NKB> struct at_fwd_cfg {
 template <typename T, int DC, int NWQ, int NWK, int NKB, bool AHEAD, int OCC>
 __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                                      const T* __restrict__ v, T* __restrict__ out,
-                                                                     float* __restrict__ lse, at_split sp, at_args a,
+                                                                     T* __restrict__ rest_out, float* __restrict__ lse, at_split sp, at_args a,
                                                                      at_order order, at_div by_tiles, at_div by_splits) {
   using C = at_fwd_cfg<T, DC, NWQ, NWK, NKB>;
   using R = at_row<T, DC>;
@@ -305,12 +305,12 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
   const float f = any ? 1.0f / l : 0.0f;  // (without a key the sums are 0)
   const int hq = hk * a.G + g;
   T* o = out + ((int64_t)((int64_t)n * a.Tq + t) * a.Hq + hq) * a.D;
-  if constexpr (NWK == 1) {
-    at_store_rows<T, DC>(o, live, acc, f, a.D, lane);
-  } else {
+  T* r = rest_out + (o - out);
 #pragma unroll
-    for (int i = 0; i < NDB; ++i)
-      if (i % NWK == wk) at_store_rows<T, 32>(o + 32 * i, live, acc + i, f, a.D - 32 * i, lane);
+  for (int i = 0; i < NDB; ++i) {
+    if (NWK > 1 && i % NWK != wk) continue;
+    if (sizeof(T) == 2 && rest_out != nullptr) at_store_rows<T, 32, true>(o + 32 * i, live, acc + i, f, a.D - 32 * i, lane, r + 32 * i);
+    else at_store_rows<T, 32>(o + 32 * i, live, acc + i, f, a.D - 32 * i, lane);
   }
   if (lse != nullptr && live && h == 0 && wk == 0)
     lse[((int64_t)n * a.Hq + hq) * a.Tq + t] = any ? m + __builtin_amdgcn_logf(l) : INFINITY;
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
 constexpr int AT_MOST_SPLITS = 512;
 
 template <typename T>
-__global__ __launch_bounds__(256) void at_join_kernel(T* __restrict__ out, float* __restrict__ lse, at_split sp, at_args a,
+__global__ __launch_bounds__(256) void at_join_kernel(T* __restrict__ out, T* __restrict__ rest, float* __restrict__ lse, at_split sp, at_args a,
                                                       at_div by_rows, at_div by_tile_rows, int row_tiles, int64_t all_rows) {
   __shared__ float weights[4][AT_MOST_SPLITS];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -366,9 +366,18 @@ __global__ __launch_bounds__(256) void at_join_kernel(T* __restrict__ out, float
   const int n = a.by_Hk.of(nh), hk = nh - n * a.Hk, t = a.by_G.of(row), hq = hk * a.G + row - t * a.G;
   if (e < a.D && part == 0) {
     const float f = none ? 0.0f : 1.0f / l;
-    T* p = out + (((int64_t)n * a.Tq + t) * a.Hq + hq) * a.D + e;
-    if constexpr (sizeof(T) == 2) *reinterpret_cast<at_u2*>(p) = at_u2{at_pack(T(), acc[0] * f, acc[1] * f), at_pack(T(), acc[2] * f, acc[3] * f)};
-    else *reinterpret_cast<at_f4*>(p) = acc * f;
+    const int64_t at = (((int64_t)n * a.Tq + t) * a.Hq + hq) * a.D + e;
+    if constexpr (sizeof(T) == 2) {
+      const at_u2 w = {at_pack(T(), acc[0] * f, acc[1] * f), at_pack(T(), acc[2] * f, acc[3] * f)};
+      *reinterpret_cast<at_u2*>(out + at) = w;
+      if (rest != nullptr) {
+        const at_f2 x = at_unpack(T(), w[0]), y = at_unpack(T(), w[1]);
+        *reinterpret_cast<at_u2*>(rest + at) = at_u2{at_pack(T(), acc[0] * f - x[0], acc[1] * f - x[1]),
+                                                     at_pack(T(), acc[2] * f - y[0], acc[3] * f - y[1])};
+      }
+    } else {
+      *reinterpret_cast<at_f4*>(out + at) = acc * f;
+    }
   }
   if (lse != nullptr && lane == 0) lse[((int64_t)n * a.Hq + hq) * a.Tq + t] = none ? INFINITY : top + __builtin_amdgcn_logf(l);
 }
@@ -385,7 +394,7 @@ __global__ __launch_bounds__(256) void at_bits_kernel(const unsigned char* __res
 }
 
 template <typename T, int DC, int NWQ, int NWK, int NKB, bool AHEAD, int OCC>
-int at_launch(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, void* out, float* lse,
+int at_launch(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, void* out, void* rest, float* lse,
               at_split sp, hipStream_t st) {
   using C = at_fwd_cfg<T, DC, NWQ, NWK, NKB>;
   constexpr int lds = NWK > 1 && C::WAVES * (64 + DC / 32 * 1024 + 4) * 4 > C::LDS ? C::WAVES * (64 + DC / 32 * 1024 + 4) * 4 : C::LDS;
@@ -396,12 +405,12 @@ int at_launch(const rc_attn* a, const at_args& d, const void* q, const void* k, 
   const int64_t rows = a->Tq * d.G, row_tiles = (rows + C::ROWS - 1) / C::ROWS;
   // few rows: nothing is read twice, and the heads of a split, which may share cache lines, are all that stays together
   const at_order order = NWK > 1 ? at_order(a->N * sp.n, a->Hk) : at_order(a->N, a->Hk, sp.n * row_tiles);
-  kernel<<<order.grid(), 64 * C::WAVES, lds, st>>>((const T*)q, (const T*)k, (const T*)v, (T*)out, lse, sp, d,
+  kernel<<<order.grid(), 64 * C::WAVES, lds, st>>>((const T*)q, (const T*)k, (const T*)v, (T*)out, (T*)rest, lse, sp, d,
                                                 order, at_div((uint32_t)row_tiles), at_div((uint32_t)sp.n));
   rc = rc_check_launch("rc_cross_attn_fwd");
   if (rc || sp.n == 1) return rc;
   const int64_t all = a->N * a->Hk * rows;
-  at_join_kernel<T><<<(uint32_t)((all + 3) / 4), 256, 0, st>>>((T*)out, lse, sp, d, at_div((uint32_t)rows), at_div(C::ROWS),
+  at_join_kernel<T><<<(uint32_t)((all + 3) / 4), 256, 0, st>>>((T*)out, (T*)rest, lse, sp, d, at_div((uint32_t)rows), at_div(C::ROWS),
                                                                (int)row_tiles, all);
   return rc_check_launch("rc_cross_attn_fwd (join)");
 }
@@ -442,7 +451,7 @@ at_plan at_make_plan(const rc_attn* a) {
 }
 
 template <typename T, int DC>
-int at_run(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, void* out, float* lse,
+int at_run(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, void* out, void* rest, float* lse,
            const at_plan& p, hipStream_t st) {
   // waves of an item's keys, blocks of keys of a wave in a tile, resident workgroups: what registers and 160 KiB of LDS
   // allow.  Few rows: two workgroups per CU, so that one streams while the other starts or ends (D 128: two waves a
@@ -455,20 +464,20 @@ int at_run(const rc_attn* a, const at_args& d, const void* q, const void* k, con
   // 138).  Narrower heads are held up by the exponentials either way and have four waves per SIMD to hide them with
   // (D 64: 332 against 328 us, 312 x 312: 167 against 148); wider ones have no registers for a second tile of scores.
   constexpr bool AHEAD = sizeof(T) == 2 && DC > 64 && DC <= 128;
-  if (p.few) return at_launch<T, DC, 1, NWK, 1, false, 1>(a, d, q, k, v, out, lse, p.sp, st);
-  return at_launch<T, DC, 4, 1, NKB, AHEAD, (AHEAD ? 2 : OCC)>(a, d, q, k, v, out, lse, p.sp, st);
+  if (p.few) return at_launch<T, DC, 1, NWK, 1, false, 1>(a, d, q, k, v, out, rest, lse, p.sp, st);
+  return at_launch<T, DC, 4, 1, NKB, AHEAD, (AHEAD ? 2 : OCC)>(a, d, q, k, v, out, rest, lse, p.sp, st);
 }
 
 template <typename T>
-int at_run_d(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, void* out, float* lse,
+int at_run_d(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, void* out, void* rest, float* lse,
              const at_plan& p, hipStream_t st) {
   switch (at_padded(a->D)) {
-    case 32: return at_run<T, 32>(a, d, q, k, v, out, lse, p, st);
-    case 64: return at_run<T, 64>(a, d, q, k, v, out, lse, p, st);
-    case 96: return at_run<T, 96>(a, d, q, k, v, out, lse, p, st);
-    case 128: return at_run<T, 128>(a, d, q, k, v, out, lse, p, st);
-    case 192: return at_run<T, 192>(a, d, q, k, v, out, lse, p, st);
-    default: return at_run<T, 256>(a, d, q, k, v, out, lse, p, st);
+    case 32: return at_run<T, 32>(a, d, q, k, v, out, rest, lse, p, st);
+    case 64: return at_run<T, 64>(a, d, q, k, v, out, rest, lse, p, st);
+    case 96: return at_run<T, 96>(a, d, q, k, v, out, rest, lse, p, st);
+    case 128: return at_run<T, 128>(a, d, q, k, v, out, rest, lse, p, st);
+    case 192: return at_run<T, 192>(a, d, q, k, v, out, rest, lse, p, st);
+    default: return at_run<T, 256>(a, d, q, k, v, out, rest, lse, p, st);
   }
 }
 
@@ -550,12 +559,13 @@ extern "C" int64_t rc_cross_attn_fwd_work_bytes(const rc_attn* a) {
   return at_bits_bytes(a) + parts;
 }
 
-extern "C" int rc_cross_attn_fwd(const rc_attn* a, const void* q, const void* k, const void* v, void* out, float* lse,
+extern "C" int rc_cross_attn_fwd(const rc_attn* a, const void* q, const void* k, const void* v, void* out, void* rest, float* lse,
                                  void* work, void* stream) {
   int rc = at_check(a);
   if (rc) return rc;
   for (const void* p : {q, (const void*)out})
     if ((rc = at_check_operand(a, a->N * a->Tq, p))) return rc;
+  RC_REQUIRE((uintptr_t)rest % 16 == 0, RC_EINVAL, "rc_cross_attn_fwd: rest is not aligned to 16 bytes");
   for (const void* p : {k, v})
     if ((rc = at_check_operand(a, a->N * a->Tk, p))) return rc;
   if (a->N * a->Tq == 0) return RC_OK;
@@ -568,7 +578,7 @@ extern "C" int rc_cross_attn_fwd(const rc_attn* a, const void* q, const void* k,
   p.sp.o = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + at_bits_bytes(a));
   p.sp.ml = p.sp.o + p.items * p.sp.n * p.tile_rows * a->D;
   const at_args d = at_to_dev(a, work);
-  if (a->dtype == RC_F32) return at_run_d<float>(a, d, q, k, v, out, lse, p, st);
-  if (a->dtype == RC_F16) return at_run_d<rc_half>(a, d, q, k, v, out, lse, p, st);
-  return at_run_d<rc_bf16>(a, d, q, k, v, out, lse, p, st);
+  if (a->dtype == RC_F32) return at_run_d<float>(a, d, q, k, v, out, rest, lse, p, st);
+  if (a->dtype == RC_F16) return at_run_d<rc_half>(a, d, q, k, v, out, rest, lse, p, st);
+  return at_run_d<rc_bf16>(a, d, q, k, v, out, rest, lse, p, st);
 }

@@ -23,7 +23,10 @@ template <typename T, int DC, int NW> struct at_rows_lds {
   static constexpr int DELTA = LSE + NW * STAT;        // [NW][32]
   static constexpr int FACTOR = DELTA + NW * STAT / 2; // [NW][32]; fp16: what a row of dS is scaled by
   static constexpr int NORM = FACTOR + NW * STAT / 2;  // fp16: each wave's largest |V|^2
-  static constexpr int BYTES = NORM + 64;
+  // fp16 heads of 32: V too, its scaling takes V's registers
+  static constexpr bool V_LDS = at_fit<T>::ON && DC == 32;
+  static constexpr int V = (NORM + 64 + 1023) / 1024 * 1024;
+  static constexpr int BYTES = V_LDS ? V + KEYS : NORM + 64;
 };
 
 // A lane's place of an operand of a 16 x 16 product across a tile's rows: 32 rows a step (16-bit types: rows 8 g + 0..3
@@ -63,7 +66,7 @@ __device__ __forceinline__ at_f4 at_mma16(rc_bf16, at_u4 a, at_u4 b, at_f4 c) {
 template <typename T, int DC, int NW, int OCC>
 __global__ __launch_bounds__(64 * NW, OCC) void at_rows_kernel(const T* __restrict__ q, const T* __restrict__ k,
                                                                const T* __restrict__ v, const T* __restrict__ out,
-                                                               const float* __restrict__ lse, const T* __restrict__ dout,
+                                                               const T* __restrict__ rest_out, const float* __restrict__ lse, const T* __restrict__ dout,
                                                                T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv,
                                                                at_args a, at_order order, at_div by_batches) {
   using R = at_row<T, DC>;
@@ -88,9 +91,14 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_rows_kernel(const T* __restri
     at_fetch_rows<T, DC>(k + (int64_t)n * a.ks[0] + (int64_t)key0 * a.ks[1] + (int64_t)hk * a.ks[2], (uint32_t)(a.ks[1] * sizeof(T)), a.D,
                          mine, lds0 + R::at(32) * wave, i, lane);
   at_u4 vf[R::STEPS];
-  at_rows_of(v + (int64_t)n * a.vs[0] + (int64_t)key0 * a.vs[1] + (int64_t)hk * a.vs[2])
-      .row<T, DC>(takes ? (uint32_t)c * (uint32_t)(a.vs[1] * sizeof(T)) : AT_OUTSIDE, a.D, lane, vf);
-  const unsigned char* ks = smem + R::at(32) * wave;
+  const T* vp = v + (int64_t)n * a.vs[0] + (int64_t)key0 * a.vs[1] + (int64_t)hk * a.vs[2];
+  const uint32_t vst = (uint32_t)(a.vs[1] * sizeof(T));
+  at_rows_of(vp).row<T, DC>(takes ? (uint32_t)c * vst : AT_OUTSIDE, a.D, lane, vf);
+  if constexpr (L::V_LDS) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) at_fetch_rows<T, DC>(vp, vst, a.D, mine, lds0 + L::V + R::at(32) * wave, i, lane);
+  }
+  const unsigned char *ks = smem + R::at(32) * wave, *vs = smem + L::V + R::at(32) * wave;
   at_places<T, DC> at;
   at.init(lane);
   at_f16 acck[NDB], accv[NDB];
@@ -130,12 +138,17 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_rows_kernel(const T* __restri
       at_fetch_floats(lse + ((int64_t)n * a.Hq + hq) * a.Tq + t, left, lds0 + L::LSE + L::STAT * wave, lane);
       at_u4 of[R::STEPS];
       at_rows_of(out + o).row<T, DC>(c < left ? (uint32_t)c * ost : AT_OUTSIDE, a.D, lane, of);
+      constexpr int RESTS = sizeof(T) == 2 ? R::STEPS : 1;
+      at_u4 rf[RESTS];
+      const bool both = sizeof(T) == 2 && rest_out != nullptr;
+      if (both) at_rows_of(rest_out + o).row<T, sizeof(T) == 2 ? DC : 8>(c < left ? (uint32_t)c * ost : AT_OUTSIDE, a.D, lane, rf);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       float s = 0.0f, n2 = 0.0f;
 #pragma unroll
       for (int st = 0; st < R::STEPS; ++st) {
         const at_u4 x = at.rows(smem + L::G + R::at(32) * wave, 0, st);
         s += at_dot(T(), x, of[st]);
+        if (both) s += at_dot(T(), x, rf[sizeof(T) == 2 ? st : 0]);
         if constexpr (FIT) n2 += at_dot(T(), x, x);
       }
       s = at_half_sum(s);
@@ -172,7 +185,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_rows_kernel(const T* __restri
       at_mma_cols<T, DC>(at, gs, 0, s, accv);
       at_f16 dp = (at_f16)(0.0f);
 #pragma unroll
-      for (int st = 0; st < R::STEPS; ++st) dp = at_mma(T(), at.rows(gs, 0, st), vf[st], dp);
+      for (int st = 0; st < R::STEPS; ++st) dp = at_mma(T(), at.rows(gs, 0, st), L::V_LDS ? at.rows(vs, 0, st) : vf[st], dp);
       unsigned char* dss = smem + L::DSS + (j & 1) * L::DS;
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -231,14 +244,14 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_rows_kernel(const T* __restri
 
 template <typename T, int DC, int NW, int OCC>
 int at_launch_rows(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, const void* out,
-                   const float* lse, const void* dout, void* dq, void* dk, void* dv, hipStream_t st) {
+                   const void* rest, const float* lse, const void* dout, void* dq, void* dk, void* dv, hipStream_t st) {
   using L = at_rows_lds<T, DC, NW>;
   static_assert(L::BYTES <= 160 * 1024, "LDS");
   constexpr auto kernel = at_rows_kernel<T, DC, NW, OCC>;
   const int rc = at_allow_lds<kernel>(L::BYTES);
   if (rc) return rc;
   const at_order order(a->N, a->Hk, 1);
-  kernel<<<order.grid(), 64 * NW, L::BYTES, st>>>((const T*)q, (const T*)k, (const T*)v, (const T*)out, lse, (const T*)dout, (T*)dq,
+  kernel<<<order.grid(), 64 * NW, L::BYTES, st>>>((const T*)q, (const T*)k, (const T*)v, (const T*)out, (const T*)rest, lse, (const T*)dout, (T*)dq,
                                                   (T*)dk, (T*)dv, d, order, at_div((uint32_t)((a->Tq + 32 * NW - 1) / (32 * NW))));
   return rc_check_launch("rc_cross_attn_bwd (rows)");
 }
@@ -269,15 +282,15 @@ template <typename T, int DC, typename... Args> int at_rows_nw(int waves, Args..
 
 bool at_rows_fit(const rc_attn* a) { return at_rows_waves(a) > 0 && a->N * a->Hk >= 256; }
 
-int at_rows_bwd(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, const void* out, const float* lse,
-                const void* dout, void* dq, void* dk, void* dv, hipStream_t st) {
+int at_rows_bwd(const rc_attn* a, const at_args& d, const void* q, const void* k, const void* v, const void* out, const void* rest,
+                const float* lse, const void* dout, void* dq, void* dk, void* dv, hipStream_t st) {
   const int w = at_rows_waves(a);
   if (a->dtype == RC_F32)
-    return a->D <= 32 ? at_rows_nw<float, 32>(w, a, d, q, k, v, out, lse, dout, dq, dk, dv, st)
-                      : at_rows_nw<float, 64>(w, a, d, q, k, v, out, lse, dout, dq, dk, dv, st);
+    return a->D <= 32 ? at_rows_nw<float, 32>(w, a, d, q, k, v, out, rest, lse, dout, dq, dk, dv, st)
+                      : at_rows_nw<float, 64>(w, a, d, q, k, v, out, rest, lse, dout, dq, dk, dv, st);
   if (a->dtype == RC_F16)
-    return a->D <= 32 ? at_rows_nw<rc_half, 32>(w, a, d, q, k, v, out, lse, dout, dq, dk, dv, st)
-                      : at_rows_nw<rc_half, 64>(w, a, d, q, k, v, out, lse, dout, dq, dk, dv, st);
-  return a->D <= 32 ? at_rows_nw<rc_bf16, 32>(w, a, d, q, k, v, out, lse, dout, dq, dk, dv, st)
-                    : at_rows_nw<rc_bf16, 64>(w, a, d, q, k, v, out, lse, dout, dq, dk, dv, st);
+    return a->D <= 32 ? at_rows_nw<rc_half, 32>(w, a, d, q, k, v, out, rest, lse, dout, dq, dk, dv, st)
+                      : at_rows_nw<rc_half, 64>(w, a, d, q, k, v, out, rest, lse, dout, dq, dk, dv, st);
+  return a->D <= 32 ? at_rows_nw<rc_bf16, 32>(w, a, d, q, k, v, out, rest, lse, dout, dq, dk, dv, st)
+                    : at_rows_nw<rc_bf16, 64>(w, a, d, q, k, v, out, rest, lse, dout, dq, dk, dv, st);
 }

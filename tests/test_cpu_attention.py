@@ -31,8 +31,8 @@ def test_attention_descriptions_are_checked(kw, rc):
     from raft_stereo_amd._lib import lib
     a = attn(**kw)
     assert lib.rc_cross_attn_fwd_work_bytes(a) == rc and lib.rc_cross_attn_bwd_work_bytes(a) == rc
-    assert lib.rc_cross_attn_fwd(a, 16, 16, 16, 16, None, 16, None) == rc
-    assert lib.rc_cross_attn_bwd(a, 16, 16, 16, 16, 16, 16, 16, 16, 16, 16, None) == rc
+    assert lib.rc_cross_attn_fwd(a, 16, 16, 16, 16, None, None, 16, None) == rc
+    assert lib.rc_cross_attn_bwd(a, 16, 16, 16, 16, None, 16, 16, 16, 16, 16, 16, None) == rc
     assert lib.rc_last_error_string()
 
 
@@ -44,19 +44,22 @@ def test_attention_operands_are_checked():
         for bad in (None, 8):
             p = [16] * 4
             p[i] = bad
-            assert lib.rc_cross_attn_fwd(a, *p, None, 16, None) == -1
-    for i in (0, 1, 2, 3, 4, 5, 9):
-        p = [16] * 10
+            assert lib.rc_cross_attn_fwd(a, *p, None, None, 16, None) == -1
+    assert lib.rc_cross_attn_fwd(a, 16, 16, 16, 16, 24, None, 16, None) == -1        # misaligned rest
+    for i in (0, 1, 2, 3, 5, 6, 10):                  # (4, the rest, may be left out)
+        p = [16] * 11
         p[i] = None
         assert lib.rc_cross_attn_bwd(a, *p, None) == -1
-    p = [16] * 10
-    p[7] = None                                       # dk without dv
+    p = [16] * 11
+    p[8] = None                                       # dk without dv
     assert lib.rc_cross_attn_bwd(a, *p, None) == -1
-    p[7] = 24                                         # misaligned
-    assert lib.rc_cross_attn_bwd(a, *p, None) == -1
-    assert lib.rc_cross_attn_fwd(None, 16, 16, 16, 16, None, 16, None) == -1
-    assert lib.rc_cross_attn_fwd(attn(N=0), None, None, None, None, None, None, None) == 0      # nothing to do
-    assert lib.rc_cross_attn_fwd(attn(Tq=0), None, 16, 16, None, None, None, None) == 0
+    for i in (4, 8):
+        p = [16] * 11
+        p[i] = 24                                     # misaligned
+        assert lib.rc_cross_attn_bwd(a, *p, None) == -1
+    assert lib.rc_cross_attn_fwd(None, 16, 16, 16, 16, None, None, 16, None) == -1
+    assert lib.rc_cross_attn_fwd(attn(N=0), None, None, None, None, None, None, None, None) == 0      # nothing to do
+    assert lib.rc_cross_attn_fwd(attn(Tq=0), None, 16, 16, None, None, None, None, None) == 0
 
 
 def heads(**kw):
