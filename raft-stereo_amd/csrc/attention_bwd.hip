@@ -333,7 +333,6 @@ struct at_bwd_plan {
 
 constexpr int AT_TILE_ROWS = 128;  // query rows, or keys, of a work item
 constexpr int AT_Q_TILE = 32;      // smallest tile of query rows in at_dkv_kernel
-constexpr int64_t AT_FILL = 512;   // work items that fill the card twice
 
 at_bwd_plan at_make_bwd_plan(const rc_attn* a) {
   at_bwd_plan p = {};
@@ -342,17 +341,20 @@ at_bwd_plan at_make_bwd_plan(const rc_attn* a) {
   p.k_tiles = (a->Tk + AT_TILE_ROWS - 1) / AT_TILE_ROWS;
   p.q_items = groups * p.q_tiles;
   p.k_items = groups * p.k_tiles;
-  auto splits = [](int64_t items, int64_t most) {
-    if (items == 0 || items >= AT_FILL) return 1;
-    const int64_t n = (AT_FILL + items - 1) / items;
+  // work items that fill the card: narrow heads have two workgroups or more per CU (2048 x 4096, 16/4 heads of 128 with
+  // ragged keys, a training step: 622 us, filled twice 641; 4096 x 2048, 8 heads of 64: 155 us, filled twice 142)
+  const int64_t fill = a->D * (a->dtype == RC_F32 ? 4 : 2) > 128 ? 256 : 512;
+  auto splits = [fill](int64_t items, int64_t most) {
+    if (items == 0 || items >= fill) return 1;
+    const int64_t n = (fill + items - 1) / items;
     return (int)(n < most ? n : most < 1 ? 1 : most);
   };
-  // a split has 512 keys at least, or 512 query rows
-  const int qs = splits(p.q_items, a->Tk / 512);
+  // a split has 256 keys at least, or 256 query rows
+  const int qs = splits(p.q_items, a->Tk / 256);
   p.q_per = (int)(((a->Tk + qs - 1) / qs + 63) / 64 * 64);
   if (p.q_per < 64) p.q_per = 64;
   p.q_splits = a->Tk ? (int)((a->Tk + p.q_per - 1) / p.q_per) : 1;
-  p.k_splits = splits(p.k_items, rows / 512);
+  p.k_splits = splits(p.k_items, rows / 256);
   p.bits = at_bits_bytes(a);
   p.delta = (a->N * a->Tq * a->Hq * 4 + 255) / 256 * 256;
   const int64_t pq = p.q_splits > 1 ? (int64_t)p.q_splits * a->N * a->Tq * a->Hq * a->D * 4 : 0;
