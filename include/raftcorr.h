@@ -451,7 +451,7 @@ int rc_sequence_loss_bwd(const float* const* preds, float* const* grad_preds, co
  * Attention operators.  Operands are sequences of heads, [N, T, H, D] of `dtype` with D the fastest dimension:
  * element (n, t, h, d) lives at n*stride[0] + t*stride[1] + h*stride[2] + d.  D is a multiple of 8 up to
  * RC_HEAD_DIM_MAX; base pointers and strides are multiples of 16 bytes (a stride of 0 repeats an operand).  Results
- * are contiguous.  Sizes of zero are allowed.
+ * are contiguous.  Sizes of zero are allowed.  rc_cross_attn_* takes strides under 8 MiB between tokens and heads.
  *
  * rc_qk_norm_rotate: RMS norm of every head and its rotation by position, queries and keys in one launch:
  *     r = 1 / sqrt(mean_d x_d^2 + eps),   y_d = x_d r w_d,

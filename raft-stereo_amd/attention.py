@@ -19,7 +19,7 @@ from raft_stereo_amd._lib import lib, check, Attn, Heads
 from raft_stereo_amd.corr import _DT, _stream, _on_device
 
 _POS = {torch.int32: _lib.RC_POS_I32, torch.int64: _lib.RC_POS_I64, torch.float32: _lib.RC_POS_F32}
-_MAX_STRIDE_BYTES = 1 << 24     # between tokens or heads: a tile's rows are addressed with 32 bits
+_MAX_STRIDE_BYTES = 1 << 23     # between tokens or heads: a tile's rows are addressed with 32 bits
 _MAX_SPAN_BYTES = 1 << 30       # from a token's first head to its last
 
 
@@ -56,7 +56,7 @@ def _heads_view(t):
         t = t.clone(memory_format=torch.contiguous_format)
         st = list(t.stride()[:3])
         if max(s if n > 1 else 0 for n, s in zip(t.shape[1:3], st[1:])) * es >= _MAX_STRIDE_BYTES:
-            raise ValueError(f"heads of {tuple(t.shape)} are too wide: a token has to stay under 16 MiB")
+            raise ValueError(f"heads of {tuple(t.shape)} are too wide: a token has to stay under 8 MiB")
     return t, st
 
 

@@ -296,7 +296,7 @@ __device__ __forceinline__ void at_mma_cols(const at_places<T, DC>& at, const un
 // the swizzle is applied to the addresses that the lanes fetch from.  Chunks behind the head's end and rows that do
 // not take part are fetched from beyond the buffer's range, which gives zeros (so whatever those rows hold, NaN
 // included, never meets a product).
-// (an offset, a row's length and the scalar offset, together under 2^31, leave AT_OUTSIDE outside without a wrap)
+// (128 rows under 8 MiB apart: offsets and scalar offsets stay under 2^30, and AT_OUTSIDE outside without a wrap)
 constexpr uint32_t AT_RANGE = 0x80010000u, AT_OUTSIDE = 0xc0000000u;
 
 typedef int at_i4 __attribute__((ext_vector_type(4)));
@@ -332,7 +332,7 @@ template <typename T, int DC, int ROWS, int WAVES> struct at_stage {
   uint32_t off[PD];
   uint32_t ahead;  // bytes from one group of PD instructions to the next
 
-  // D: elements of a head; stride: bytes between rows (under 16 MiB)
+  // D: elements of a head; stride: bytes between rows (under 8 MiB)
   __device__ __forceinline__ void init(int wave, int lane, int D, uint32_t stride) {
     ahead = PD * STEP * stride;
 #pragma unroll

@@ -499,12 +499,12 @@ int at_check(const rc_attn* a) {
   const int64_t* st[3] = {a->q_stride, a->k_stride, a->v_stride};
   for (int o = 0; o < 3; ++o)
     for (int i = 0; i < 3; ++i)
-      RC_REQUIRE(st[o][i] >= 0 && st[o][i] * es % 16 == 0 && (i == 0 || st[o][i] * es < (1ll << 24)), RC_EINVAL,
-                 "rc_cross_attn: stride %lld of %c is negative, no multiple of 16 bytes, or 16 MiB or more between tokens "
+      RC_REQUIRE(st[o][i] >= 0 && st[o][i] * es % 16 == 0 && (i == 0 || st[o][i] * es < (1ll << 23)), RC_EINVAL,
+                 "rc_cross_attn: stride %lld of %c is negative, no multiple of 16 bytes, or 8 MiB or more between tokens "
                  "or heads", (long long)st[o][i], "qkv"[o]);
   RC_REQUIRE((int64_t)a->Hq * a->q_stride[2] * es < (1ll << 30), RC_EINVAL,
              "rc_cross_attn: the heads of a query token span 1 GiB or more");
-  RC_REQUIRE((int64_t)a->Hq * a->D * es < (1ll << 24), RC_EINVAL, "rc_cross_attn: a query token of 16 MiB or more");
+  RC_REQUIRE((int64_t)a->Hq * a->D * es < (1ll << 23), RC_EINVAL, "rc_cross_attn: a query token of 8 MiB or more");
   RC_REQUIRE(a->key_mask == nullptr || a->mask_stride >= 0, RC_EINVAL, "rc_cross_attn: negative mask stride");
   return RC_OK;
 }

@@ -25,7 +25,8 @@ def attn(**kw):
     (dict(D=12), -2), (dict(D=264), -2), (dict(D=0), -2), (dict(dtype=3), -2), (dict(N=-1), -1), (dict(Tq=-1), -1),
     (dict(Hk=3), -1), (dict(Hk=0), -1), (dict(Hq=0), -1), (dict(scale=0.0), -1), (dict(scale=float("nan")), -1),
     (dict(scale=float("inf")), -1), (dict(q_stride=(1, 4)), -1), (dict(k_stride=(0, -64)), -1),
-    (dict(v_stride=(1, 1 << 24)), -1), (dict(Tk=1 << 31), -1), (dict(N=1 << 30, Tk=1 << 20), -1),
+    (dict(v_stride=(1, 1 << 24)), -1), (dict(v_stride=(1, 1 << 22)), -1), (dict(k_stride=(2, 1 << 22)), -1),
+    (dict(Tk=1 << 31), -1), (dict(N=1 << 30, Tk=1 << 20), -1),
     (dict(key_mask=16, mask_stride=-1), -1)])
 def test_attention_descriptions_are_checked(kw, rc):
     from raft_stereo_amd._lib import lib

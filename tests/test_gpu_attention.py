@@ -69,6 +69,18 @@ SHAPES += [
     (256, 1, 1, 2, 1, 8),
 ]
 
+# lengths that are divided: keys over workgroups with rows that fill a tile and more, query rows in the backward pass,
+# an even and an odd count of key tiles for the heads whose loads run ahead, more sequences than the card has dies
+SHAPES += [
+    (2, 70, 1500, 2, 1, 64),
+    (1, 600, 300, 2, 1, 128),
+    (1, 520, 70, 2, 1, 256),
+    (1, 300, 1100, 1, 1, 96),
+    (2, 40, 577, 3, 3, 128),
+    (20, 40, 70, 2, 2, 64),
+    (1, 90, 600, 1, 1, 160),
+]
+
 
 def masks(kind, N, Tk, rng):
     """(lengths, mask): lengths of nothing, one, more than there are and less than nothing; a mask that leaves a
@@ -139,6 +151,31 @@ def test_masked_places_may_hold_anything(R, shape, dtype):
         dirty = run_attention(R, q, kb, vb, g, lengths, mask, dtype)
         for name in clean:
             assert torch.equal(clean[name], dirty[name]), (name, bad)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D, Tq, Hq", [(64, 200, 1), (128, 150, 2), (256, 140, 1), (64, 1, 4)])
+def test_the_widest_strides(R, dtype, D, Tq, Hq):
+    """Tokens 16 bytes short of 8 MiB apart: every tile's rows stay in reach, and the rows behind the last give nothing."""
+    Tk, wide = 141, ((8 << 20) - 16) // DT[dtype].itemsize
+    rng = np.random.default_rng(D + Tq)
+    q, k, v, g = (rand(rng, (1, T, H, D), dtype) for T, H in ((Tq, Hq), (Tk, 1), (Tk, 1), (Tq, Hq)))
+    ok = A.allowed_keys(1, Tk, None, None)
+    want = A.attention(*(host(x) for x in (q, k, v, g)), ok, dtype=dtype)
+
+    def spread(x):
+        T, H = x.shape[1:3]
+        base = torch.empty(T * wide + H * D, dtype=x.dtype, device="cuda")
+        y = base.as_strided((1, T, H, D), (T * wide, wide, D, 1))
+        y.copy_(x)
+        return y.detach().requires_grad_()
+
+    t = [spread(x) for x in (q, k, v)]
+    assert all(x.stride(1) * x.element_size() == (8 << 20) - 16 for x in t)
+    out = R.cross_attention_hip(*t)
+    got = dict(zip(("out", "dq", "dk", "dv"), (out,) + torch.autograd.grad(out, t, g.cuda())))
+    for name in want.keys() & got.keys():
+        assert_within(got[name], want[name], name)
 
 
 def test_what_is_not_finite_in_allowed_places_shows(R):
