@@ -462,9 +462,10 @@ struct at_order {
 };
 
 // Writes a result (rows: elements 32 db .. of the head, column: this lane's row of memory at p) times f; REST: and what
-// rounding took from it.
+// rounding took from it.  Without `keep`, zeros: where no key takes part, the sums may hold 0 times an infinity or NaN.
 template <typename T, int DC, bool REST = false>
-__device__ __forceinline__ void at_store_rows(T* p, bool live, const at_f16* acc, float f, int D, int lane, T* rest = nullptr) {
+__device__ __forceinline__ void at_store_rows(T* p, bool live, bool keep, const at_f16* acc, float f, int D, int lane,
+                                              T* rest = nullptr) {
   const int h = lane >> 5;
 #pragma unroll
   for (int db = 0; db < DC / 32; ++db) {
@@ -483,12 +484,12 @@ __device__ __forceinline__ void at_store_rows(T* p, bool live, const at_f16* acc
             const at_f2 a = u - at_unpack(T(), x), c = v - at_unpack(T(), y);
             uint32_t ra = at_pack(T(), a[0], a[1]), rc = at_pack(T(), c[0], c[1]);
             at_swap(ra, rc);
-            r[j] = ra;
-            r[2 + j] = rc;
+            r[j] = keep ? ra : 0u;
+            r[2 + j] = keep ? rc : 0u;
           }
           at_swap(x, y);
-          w[j] = x;
-          w[2 + j] = y;
+          w[j] = keep ? x : 0u;
+          w[2 + j] = keep ? y : 0u;
         }
         const int d = 32 * db + 16 * b + 8 * h;
         if (live && d < D) {
@@ -500,7 +501,9 @@ __device__ __forceinline__ void at_store_rows(T* p, bool live, const at_f16* acc
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const int d = 32 * db + 8 * b + 4 * h;
-        const at_f4 w = {acc[db][4 * b] * f, acc[db][4 * b + 1] * f, acc[db][4 * b + 2] * f, acc[db][4 * b + 3] * f};
+        at_f4 w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = keep ? acc[db][4 * b + j] * f : 0.0f;
         if (live && d < D) *reinterpret_cast<at_f4*>(p + d) = w;
       }
     }

@@ -92,6 +92,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dq_kernel(const T* __restrict
 #pragma unroll
   for (int i = 0; i < NDB; ++i) acc[i] = (at_f16)(0.0f);
   at_fit<T> fit;
+  uint32_t any = 0;
 
   for (int j = 0; j < tiles; ++j) {
     at_landed();
@@ -102,7 +103,9 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dq_kernel(const T* __restrict
 #pragma unroll
     for (int b = 0; b < NKB; ++b) {
       // (a key that takes no part has the score -inf, so P = 0, and zeros for its value, so dP = 0)
-      at_f16 s = at_start<T>(at_key_bits(a, n, k_end, k_begin + j * KT + 32 * b), lane), dp = (at_f16)(0.0f);
+      const uint32_t take = at_key_bits(a, n, k_end, k_begin + j * KT + 32 * b);
+      any |= take;
+      at_f16 s = at_start<T>(take, lane), dp = (at_f16)(0.0f);
 #pragma unroll
       for (int st = 0; st < R::STEPS; ++st) {
         s = at_mma(T(), at.rows(kt, 32 * b, st), qf[st], s);
@@ -117,8 +120,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dq_kernel(const T* __restrict
   }
   if (dq == nullptr) return;
   const float f = a.scale * fit.undo();
-  if (sp.n > 1) at_store_rows<float, DC>(sp.p + split * sp.part + orow, live, acc, f, a.D, lane);
-  else at_store_rows<T, DC>(dq + orow, live, acc, f, a.D, lane);
+  if (sp.n > 1) at_store_rows<float, DC>(sp.p + split * sp.part + orow, live, any != 0, acc, f, a.D, lane);
+  else at_store_rows<T, DC>(dq + orow, live, any != 0, acc, f, a.D, lane);
 }
 
 // HALVES = 2: two waves share 32 keys and take every other block of query rows; their values lie in LDS
@@ -271,6 +274,7 @@ __global__ __launch_bounds__(64 * NW * HALVES, OCC) void at_dkv_kernel(const T* 
     }
   }
   const int64_t o = (((int64_t)n * a.Tk + key) * a.Hk + hk) * a.D;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the values' loads to LDS, where no row has waited for them)
   if constexpr (HALVES > 1) {
     // the other wave's sums, one of the two at a time
     float* meet = reinterpret_cast<float*>(smem) + kw * NDB * 1024 + lane;
@@ -299,13 +303,14 @@ __global__ __launch_bounds__(64 * NW * HALVES, OCC) void at_dkv_kernel(const T* 
   }
   const float unlift = at_fit<T>::ON ? 1.0f / 4096.0f : 1.0f;
   const float fk = a.scale * fit.undo() * unlift, fv = unlift;
+  const bool keep = (mine >> c) & 1;
   if (sp.n > 1) {
     float* p = sp.p + (int64_t)split * 2 * sp.part + o;
-    if constexpr (DO_K) at_store_rows<float, DC>(p, live, acck, fk, a.D, lane);
-    if constexpr (DO_V) at_store_rows<float, DC>(p + sp.part, live, accv, fv, a.D, lane);
+    if constexpr (DO_K) at_store_rows<float, DC>(p, live, keep, acck, fk, a.D, lane);
+    if constexpr (DO_V) at_store_rows<float, DC>(p + sp.part, live, keep, accv, fv, a.D, lane);
   } else {
-    if constexpr (DO_K) at_store_rows<T, DC>(dk + o, live, acck, fk, a.D, lane);
-    if constexpr (DO_V) at_store_rows<T, DC>(dv + o, live, accv, fv, a.D, lane);
+    if constexpr (DO_K) at_store_rows<T, DC>(dk + o, live, keep, acck, fk, a.D, lane);
+    if constexpr (DO_V) at_store_rows<T, DC>(dv + o, live, keep, accv, fv, a.D, lane);
   }
 }
 
@@ -332,7 +337,6 @@ struct at_bwd_plan {
 };
 
 constexpr int AT_TILE_ROWS = 128;  // query rows, or keys, of a work item
-constexpr int AT_Q_TILE = 32;      // smallest tile of query rows in at_dkv_kernel
 
 at_bwd_plan at_make_bwd_plan(const rc_attn* a) {
   at_bwd_plan p = {};

@@ -302,15 +302,15 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
     }
     return;
   }
-  const float f = any ? 1.0f / l : 0.0f;  // (without a key the sums are 0)
+  const float f = 1.0f / l;
   const int hq = hk * a.G + g;
   T* o = out + ((int64_t)((int64_t)n * a.Tq + t) * a.Hq + hq) * a.D;
   T* r = rest_out + (o - out);
 #pragma unroll
   for (int i = 0; i < NDB; ++i) {
     if (NWK > 1 && i % NWK != wk) continue;
-    if (sizeof(T) == 2 && rest_out != nullptr) at_store_rows<T, 32, true>(o + 32 * i, live, acc + i, f, a.D - 32 * i, lane, r + 32 * i);
-    else at_store_rows<T, 32>(o + 32 * i, live, acc + i, f, a.D - 32 * i, lane);
+    if (sizeof(T) == 2 && rest_out != nullptr) at_store_rows<T, 32, true>(o + 32 * i, live, any != 0, acc + i, f, a.D - 32 * i, lane, r + 32 * i);
+    else at_store_rows<T, 32>(o + 32 * i, live, any != 0, acc + i, f, a.D - 32 * i, lane);
   }
   if (lse != nullptr && live && h == 0 && wk == 0)
     lse[((int64_t)n * a.Hq + hq) * a.Tq + t] = any ? m + __builtin_amdgcn_logf(l) : INFINITY;

@@ -82,6 +82,9 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_rows_kernel(const T* __restri
   const int key0 = wave * 32, key = key0 + c;
   const uint32_t mine = at_key_bits(a, n, at_length(a, n), key0);
   const bool live = key < a.Tk, takes = (mine >> c) & 1;
+  uint32_t some = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) some |= at_key_bits(a, n, at_length(a, n), 32 * w);
   const int batches = (int)by_batches.d;  // of one head's query rows
   const uint32_t lds0 = (uint32_t)(uintptr_t)(at_lds)smem;
 
@@ -224,6 +227,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_rows_kernel(const T* __restri
             acc = __builtin_amdgcn_mfma_f32_16x16x4f32(u[1], w[1], acc, 0, 0, 0);
           }
         }
+        if (!some) acc = (at_f4)(0.0f);  // (no key at all: not even what 0 times NaN leaves)
         const int r = 16 * (x & 1) + (ln & 15), d = 16 * (x >> 1) + 4 * (ln >> 4), t = t0 + 32 * j + r;
         float f = a.scale;
         if constexpr (FIT) f = f / (fr[r] * fv) * (1.0f / 4096.0f);
@@ -237,9 +241,10 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_rows_kernel(const T* __restri
   }
 
   const float unlift = FIT ? 1.0f / 4096.0f : 1.0f;
+  const bool keep = (mine >> c) & 1;
   const int64_t o = (((int64_t)n * a.Tk + key) * a.Hk + hk) * a.D;
-  at_store_rows<T, DC>(dk + o, live, acck, a.scale * fit.undo() * unlift, a.D, lane);
-  at_store_rows<T, DC>(dv + o, live, accv, unlift, a.D, lane);
+  at_store_rows<T, DC>(dk + o, live, keep, acck, a.scale * fit.undo() * unlift, a.D, lane);
+  at_store_rows<T, DC>(dv + o, live, keep, accv, unlift, a.D, lane);
 }
 
 template <typename T, int DC, int NW, int OCC>

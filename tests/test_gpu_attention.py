@@ -178,6 +178,31 @@ def test_the_widest_strides(R, dtype, D, Tq, Hq):
         assert_within(got[name], want[name], name)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 40, 100, 4, 2, 64), (3, 1, 300, 8, 2, 128), (2, 70, 1500, 1, 1, 256), (90, 70, 129, 6, 3, 40)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_keys_that_take_no_part_get_nothing_from_bad_queries(R, shape, dtype):
+    """NaN and infinities in queries and incoming gradients stay away from the gradients of masked keys, and a sequence
+    without a key gives zeros whatever its queries hold."""
+    N, Tq, Tk, Hq, Hk, D = shape
+    rng = np.random.default_rng(6)
+    q, k, v = rand(rng, (N, Tq, Hq, D), dtype), rand(rng, (N, Tk, Hk, D), dtype), rand(rng, (N, Tk, Hk, D), dtype)
+    g = rand(rng, (N, Tq, Hq, D), dtype)
+    mask = rng.random((N, Tk)) < 0.6
+    mask[N - 1] = False
+    off = torch.from_numpy(~mask)
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        for where in ("q", "g"):
+            x = {"q": q.clone(), "g": g.clone()}
+            x[where][:, Tq // 2] = bad
+            got = run_attention(R, x["q"], k, v, x["g"], None, mask, dtype)
+            for name in ("dk", "dv"):
+                assert not got[name].cpu()[off].any(), (name, bad, where)
+            for name in ("out", "dq"):
+                assert not got[name][N - 1].any(), (name, bad, where)
+            assert not run_attention(R, x["q"], k, v, None, None, mask, dtype)["out"][N - 1].any()
+
+
 def test_what_is_not_finite_in_allowed_places_shows(R):
     q, k, v = (torch.randn(1, 4, 1, 32, device="cuda") for _ in range(3))
     k[0, 2] = float("nan")
