@@ -40,6 +40,13 @@ struct at_div {
   __device__ __forceinline__ int of(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n, m) >> (s - 1)); }
 };
 
+// A launch holds fewer than 2^32 threads along x: larger grids go along y too, in rows of 2^22 blocks (a multiple of the
+// XCDs that block ids go round).
+inline dim3 at_grid(int64_t blocks) {
+  return blocks <= 1 << 22 ? dim3((uint32_t)blocks) : dim3(1u << 22, (uint32_t)((blocks + (1 << 22) - 1) >> 22));
+}
+__device__ __forceinline__ uint32_t at_block() { return (blockIdx.y << 22) + blockIdx.x; }
+
 struct at_args {
   int64_t qs[3], ks[3], vs[3];  // elements between sequences, tokens, heads
   const void* lengths;
@@ -446,12 +453,11 @@ struct at_order {
       : subs((uint32_t)(N >= 16 ? Hk * items_of_head : items_of_head)), units((int32_t)(N >= 16 ? N : N * Hk)) {}
   // units that are given
   __host__ at_order(int64_t units_, int64_t subs_) : subs((uint32_t)subs_), units((int32_t)units_) {}
-  __host__ uint32_t grid() const {
-    return (uint32_t)(8 * ((int64_t)(units / 8) * subs.d + ((int64_t)(units % 8) * subs.d + 7) / 8));
-  }
+  __host__ dim3 grid() const { return at_grid(8 * ((int64_t)(units / 8) * subs.d + ((int64_t)(units % 8) * subs.d + 7) / 8)); }
   // -1: none
   __device__ __forceinline__ int item() const {
-    const int xcd = blockIdx.x & 7, pos = blockIdx.x >> 3, whole = (units >> 3) * (int)subs.d;
+    const uint32_t id = at_block();
+    const int xcd = id & 7, pos = id >> 3, whole = (units >> 3) * (int)subs.d;
     if (pos < whole) {
       const int u = subs.of(pos);
       return (u * 8 + xcd) * (int)subs.d + pos - u * (int)subs.d;

@@ -385,7 +385,7 @@ __global__ __launch_bounds__(256) void at_join_kernel(T* __restrict__ out, T* __
 // The mask and the lengths as one bit per key: a scalar load tells a tile what it may skip.
 __global__ __launch_bounds__(256) void at_bits_kernel(const unsigned char* __restrict__ mask, int64_t stride,
                                                       uint64_t* __restrict__ bits, int64_t words, int Tk, int64_t total) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // a wave per word
+  const int64_t w = (int64_t)at_block() * 4 + (threadIdx.x >> 6);  // a wave per word
   if (w >= total) return;
   const int64_t n = w / words, key = (w - n * words) * 64 + (threadIdx.x & 63);
   const bool on = key < Tk && mask[n * stride + key] != 0;
@@ -547,7 +547,7 @@ int64_t at_bits_bytes(const rc_attn* a) {
 int at_launch_bits(const rc_attn* a, void* bits, hipStream_t st) {
   const int64_t words = (a->Tk + 63) / 64, total = a->N * words;
   if (a->key_mask == nullptr || total == 0) return RC_OK;
-  at_bits_kernel<<<(uint32_t)((total + 3) / 4), 256, 0, st>>>(a->key_mask, a->mask_stride, (uint64_t*)bits, words, (int)a->Tk, total);
+  at_bits_kernel<<<at_grid((total + 3) / 4), 256, 0, st>>>(a->key_mask, a->mask_stride, (uint64_t*)bits, words, (int)a->Tk, total);
   return rc_check_launch("rc_cross_attn (mask)");
 }
 

@@ -18,6 +18,7 @@ namespace {
 
 constexpr int NR_THREADS = 256;
 constexpr int NR_MAX_BLOCKS = 1024;  // of one side's backward pass: rows of partial weight gradients
+constexpr uint32_t NR_GRID_X = 1u << 22;  // a launch holds fewer than 2^32 threads along x
 constexpr int NR_UNROLL = 4;         // heads whose loads are in flight together
 
 struct nr_side {
@@ -179,8 +180,9 @@ __device__ __forceinline__ void nr_fwd_body(const nr_side& s, const nr_common& c
 
 template <typename T, int G, bool IL>
 __global__ __launch_bounds__(NR_THREADS) void nr_fwd_kernel(nr_side q, nr_side k, nr_common c) {
-  if (blockIdx.x < q.blocks) nr_fwd_body<T, G, IL>(q, c, blockIdx.x);
-  else nr_fwd_body<T, G, IL>(k, c, blockIdx.x - q.blocks);
+  const uint32_t block = blockIdx.y * NR_GRID_X + blockIdx.x;
+  if (block < q.blocks) nr_fwd_body<T, G, IL>(q, c, block);
+  else if (block - q.blocks < k.blocks) nr_fwd_body<T, G, IL>(k, c, block - q.blocks);
 }
 
 // A group goes through many tokens, so that its lanes' weight gradients are summed in registers; the groups of a block
@@ -373,7 +375,11 @@ nr_side nr_plan(const rc_heads* s, void* y, const void* g, int64_t N, int D, uin
 template <typename T, int G, bool IL>
 void nr_launch(const nr_side& q, const nr_side& k, const nr_common& c, bool bwd, float* pq, float* pk, hipStream_t st) {
   if (bwd) nr_bwd_kernel<T, G, IL><<<q.blocks + k.blocks, NR_THREADS, 0, st>>>(q, k, c, pq, pk);
-  else nr_fwd_kernel<T, G, IL><<<q.blocks + k.blocks, NR_THREADS, 0, st>>>(q, k, c);
+  else {
+    const uint32_t blocks = q.blocks + k.blocks;
+    const dim3 grid = blocks <= NR_GRID_X ? dim3(blocks) : dim3(NR_GRID_X, (blocks - 1) / NR_GRID_X + 1);
+    nr_fwd_kernel<T, G, IL><<<grid, NR_THREADS, 0, st>>>(q, k, c);
+  }
 }
 
 template <typename T, bool IL>

@@ -203,6 +203,27 @@ def test_keys_that_take_no_part_get_nothing_from_bad_queries(R, shape, dtype):
             assert not run_attention(R, x["q"], k, v, None, None, mask, dtype)["out"][N - 1].any()
 
 
+@pytest.mark.parametrize("D, Tq", [(8, 1), (8, 5), (72, 1)])
+def test_more_sequences_than_a_launch_holds_threads(R, D, Tq):
+    """2^24 sequences and some: a workgroup for each is 2^32 threads.  The whole agrees with its parts, forward and back."""
+    N, Tk = (1 << 24) + 37, 2
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(1, Tq, 1, D, generator=gen, device="cuda", dtype=torch.bfloat16).expand(N, -1, -1, -1)
+    kv = torch.randn(N, Tk, 1, 8, generator=gen, device="cuda", dtype=torch.bfloat16).repeat(1, 1, 1, D // 8)
+    mask = torch.rand(N, Tk, generator=gen, device="cuda") < 0.7
+    parts = [slice(0, 300), slice((1 << 22) - 9, (1 << 22) + 300), slice((1 << 24) - 270, N)]   # (as many as take the same way)
+
+    def run(n):
+        t = [x[n].detach().requires_grad_() for x in (q, kv, kv)]
+        out = R.cross_attention_hip(*t, key_mask=mask[n])
+        return (out,) + torch.autograd.grad(out, t, out.detach())
+
+    whole = run(slice(None))
+    for n in parts:
+        for a, b in zip(whole, run(n)):
+            assert torch.isfinite(b).all() and b.any() and torch.equal(a[n], b), n
+
+
 def test_what_is_not_finite_in_allowed_places_shows(R):
     q, k, v = (torch.randn(1, 4, 1, 32, device="cuda") for _ in range(3))
     k[0, 2] = float("nan")
@@ -493,6 +514,19 @@ def test_norm_rotate_weights_of_other_types_and_slices(R, wdtype):
     assert torch.equal(y2, y)
     d2, = torch.autograd.grad(y2.float().sum(), qt)
     assert torch.equal(d2, qt.grad)
+
+
+def test_norm_rotate_of_more_tokens_than_a_launch_holds_threads(R):
+    T, D = (1 << 27) + 11, 256       # 32 lanes each
+    x = torch.randn(1, 1, 1, D, device="cuda", dtype=torch.bfloat16)
+    freqs = 1e4 ** (-torch.arange(4, device="cuda", dtype=torch.float64) / 4)
+    y = R.qk_norm_rotate_hip(x.expand(1, T, 1, D), freqs=freqs)
+    for t in (0, 1, (1 << 25) - 1, 1 << 25, (1 << 27) - 1, 1 << 27, T - 1):
+        pos = torch.tensor([t], device="cuda")
+        assert torch.equal(y[:, t:t + 1], R.qk_norm_rotate_hip(x, freqs=freqs, q_pos=pos)), t
+    y = y.view(-1, D)
+    for t in range(0, T, 1 << 25):      # no token was left out: the rest of the head is the same in all of them
+        assert (y[t:t + (1 << 25), 8:] == y[0, 8:]).all()
 
 
 @pytest.mark.parametrize("shape", [(0, 3, 2), (2, 0, 2), (2, 3, 0)])
