@@ -350,15 +350,16 @@ at_bwd_plan at_make_bwd_plan(const rc_attn* a) {
   const int64_t fill = a->D * (a->dtype == RC_F32 ? 4 : 2) > 128 ? 256 : 512;
   auto splits = [fill](int64_t items, int64_t most) {
     if (items == 0 || items >= fill) return 1;
-    const int64_t n = (fill + items - 1) / items;
+    const int64_t n = fill / items;  // (no more than fill the card: the rest would be a second turn)
     return (int)(n < most ? n : most < 1 ? 1 : most);
   };
-  // a split has 256 keys at least, or 256 query rows
-  const int qs = splits(p.q_items, a->Tk / 256);
+  // a split has 256 keys at least, or 256 query rows; 64 in fp32, whose products take sixteen times as long
+  const int64_t least = a->dtype == RC_F32 ? 64 : 256;
+  const int qs = splits(p.q_items, a->Tk / least);
   p.q_per = (int)(((a->Tk + qs - 1) / qs + 63) / 64 * 64);
   if (p.q_per < 64) p.q_per = 64;
   p.q_splits = a->Tk ? (int)((a->Tk + p.q_per - 1) / p.q_per) : 1;
-  p.k_splits = splits(p.k_items, rows / 256);
+  p.k_splits = splits(p.k_items, rows / least);
   p.bits = at_bits_bytes(a);
   p.delta = (a->N * a->Tq * a->Hq * 4 + 255) / 256 * 256;
   const int64_t pq = p.q_splits > 1 ? (int64_t)p.q_splits * a->N * a->Tq * a->Hq * a->D * 4 : 0;

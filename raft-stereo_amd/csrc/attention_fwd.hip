@@ -432,21 +432,24 @@ at_plan at_make_plan(const rc_attn* a) {
   p.tile_rows = p.few ? 32 : 128;
   p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   p.items = a->N * a->Hk * p.row_tiles;
-  // Fewer work items than fill the card twice: the keys are divided too, down to 256 of them.  (One token in each of 16
+  // Fewer work items than fill the card twice: the keys are divided too, down to 256 of them; in fp32, whose products
+  // take sixteen times as long, down to 64 (128 for narrow heads, where that is the tile).  (One token in each of 16
   // sequences, 8192 ragged keys, 32/8 heads of 128: 84 us; one over 16384 keys, 8/1 heads: 21 us, in splits of 1024 keys
-  // 29.)  Up to 1024 keys few rows stay whole: joining is a launch more (1000 keys: 14.7 against 18.9 us a call).
+  // 29.)  Up to four such parts few rows stay whole: joining is a launch more (1000 keys in bf16: 14.7
+  // against 18.9 us a call); fp32 heads beyond 128, which one wave goes through alone, up to one.
+  const int64_t unit = a->dtype != RC_F32 ? 256 : a->D > 32 ? 64 : 128;
   int64_t n = 1;
-  if (p.items > 0 && p.items < 512 && !(p.few && a->Tk <= 1024)) {
+  if (p.items > 0 && p.items < 512 && !(p.few && a->Tk <= (a->dtype == RC_F32 && a->D > 128 ? 1 : 4) * unit)) {
     n = (512 + p.items - 1) / p.items;
-    const int64_t most = (a->Tk + 255) / 256;
+    const int64_t most = (a->Tk + unit - 1) / unit;
     n = n < most ? n : most;
     n = n < AT_MOST_SPLITS ? n : AT_MOST_SPLITS;
     n = n < 1 ? 1 : n;
   }
-  const int64_t keys = ((a->Tk + n - 1) / n + 255) / 256 * 256;
+  const int64_t keys = ((a->Tk + n - 1) / n + unit - 1) / unit * unit;
   p.sp.n = (int)(keys ? (a->Tk + keys - 1) / keys : 1);
   if (p.sp.n < 1) p.sp.n = 1;
-  p.sp.keys = (int)(keys ? keys : 256);
+  p.sp.keys = (int)(keys ? keys : unit);
   return p;
 }
 

@@ -79,6 +79,8 @@ SHAPES += [
     (2, 40, 577, 3, 3, 128),
     (20, 40, 70, 2, 2, 64),
     (1, 90, 600, 1, 1, 160),
+    (4, 1, 1124, 4, 2, 256),
+    (2, 3, 515, 2, 1, 32),
 ]
 
 
