@@ -9,6 +9,10 @@
 // after a barrier the waves take blocks of 16 x 16 of dQ = dS K, each over all keys.  Everything is read once and written
 // once, and S and dP are worked out once (the two kernels for long sequences read the operands twice and multiply 7
 // products instead of 5).
+//
+// 640 x 180 x 180, 8 heads of 32, bf16: 185 us, 2.2 TB/s (the two kernels: 225); the matrix pipe is busy 14 % of the time
+// and LDS 40 %: the waves of a workgroup wait for each other at each 32 query rows, and two or three workgroups on a CU
+// fill each other's gaps.  96 x 128 x 117, 4 heads of 64, fp32: 84 us, matrix pipe 29 %.
 #include "attention.h"
 
 namespace {

@@ -9,7 +9,13 @@
 // one head, 8 elements per lane; the sum of squares is a butterfly over the group.  A lane owns BOTH elements of each
 // of its four pairs -- elements 4 j .. 4 j + 3 and the ones n_freqs further on (or 8 j .. 8 j + 7 when neighbours are
 // paired) -- so the rotation needs no exchange between lanes, and its four angles are worked out once and serve all
-// heads of the token that the group goes through.
+// heads of the token that the group goes through.  Lanes of 8 elements rather than 16 bytes each: one form for all
+// types, and 8-byte loads of neighbouring lanes fill their cache lines together.
+//
+// Measured (a large copy reaches 4.8 TB/s; what the 256 MiB cache still holds comes faster): forward, 768 x 312 fp16
+// queries and keys, 4 heads of 64 each: 107 us, 4.6 TB/s.  640 x 180 fp32, 8 and 8 heads of 32: forward 85 us, 5.5 TB/s,
+// backward 141 us, 5.0 TB/s.  8 x 2047 and 4095 bf16, 16 and 4 heads of 128: 48 us, 4.2 TB/s, and 68 us, 4.4 TB/s, and
+// 6 us for the sum of the weights' gradients.  One token in 16 sequences, 32 heads of 128: 5.4 us, in 12.5 of the call.
 #include "rc_common.h"
 
 #include <math.h>
@@ -186,7 +192,8 @@ __global__ __launch_bounds__(NR_THREADS) void nr_fwd_kernel(nr_side q, nr_side k
 }
 
 // A group goes through many tokens, so that its lanes' weight gradients are summed in registers; the groups of a block
-// are then added in LDS, and the block's row goes to `partial`.
+// are then added in LDS, and the block's row goes to `partial`.  Bound by memory; two heads' loads in flight are what the
+// registers of four waves per SIMD hold.
 template <typename T, int G, bool IL>
 __device__ __forceinline__ void nr_bwd_body(const nr_side& s, const nr_common& c, uint32_t block, float* partial,
                                             float* lds) {
