@@ -323,18 +323,19 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
     lse[((int64_t)n * a.Hq + hq) * a.Tq + t] = any ? m + __builtin_amdgcn_logf(l) : INFINITY;
 }
 
-// Joins the splits: a wave per row.  The lanes take a split's maximum and sum each, the weights exp2(m_i - max) go to LDS;
+// Joins the splits: a wave per row, or four.  The lanes take a split's maximum and sum each, the weights exp2(m_i - max) go to LDS;
 // then a group of D / 4 lanes takes four elements each of every (64 / group)th split, many loads in flight.
 // Bound by latency: 512 rows of 128 in 4 splits take 4.5 us.
 constexpr int AT_MOST_SPLITS = 512;
 
-template <typename T>
+template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void at_join_kernel(T* __restrict__ out, T* __restrict__ rest, float* __restrict__ lse, at_split sp, at_args a,
                                                       at_div by_rows, at_div by_tile_rows, int row_tiles, int64_t all_rows) {
   __shared__ float weights[4][AT_MOST_SPLITS];
+  __shared__ at_f4 sums[4][64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t i = (int64_t)blockIdx.x * 4 + wave;
-  if (i >= all_rows) return;  // (a wave joins its row alone)
+  const int64_t i = (int64_t)blockIdx.x * (4 / WAVES) + wave / WAVES;
+  if (WAVES == 1 && i >= all_rows) return;  // (a wave joins its row alone; four share a workgroup's)
   const int nh = by_rows.of((int)i), row = (int)i - nh * (int)by_rows.d;
   const int tile_rows = (int)by_tile_rows.d, rt = by_tile_rows.of(row), r = row - rt * tile_rows;
   const int64_t item0 = (int64_t)nh * sp.n * row_tiles + rt;  // + split * row_tiles
@@ -357,13 +358,13 @@ __global__ __launch_bounds__(256) void at_join_kernel(T* __restrict__ out, T* __
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   int group = 2;  // lanes of a group: D / 4 rounded up to a power of two
   while (group * 4 < a.D) group *= 2;
-  const int e = (lane & (group - 1)) * 4, part = lane / group, parts = 64 / group;
+  const int e = (lane & (group - 1)) * 4, part = lane / group, parts = 64 / group, share = wave % WAVES;
   at_f4 acc = (at_f4)(0.0f);
   if (e < a.D && !none) {
     const float* o = sp.o + (item0 * tile_rows + r) * a.D + e;
     const int64_t step = (int64_t)row_tiles * tile_rows * a.D;
 #pragma unroll 8
-    for (int s = part; s < sp.n; s += parts) {
+    for (int s = share * parts + part; s < sp.n; s += parts * WAVES) {
       const float w = weights[wave][s];
       if (w != 0.0f) acc += w * *reinterpret_cast<const at_f4*>(o + s * step);
     }
@@ -371,6 +372,13 @@ __global__ __launch_bounds__(256) void at_join_kernel(T* __restrict__ out, T* __
   for (int x = group; x < 64; x <<= 1)
 #pragma unroll
     for (int y = 0; y < 4; ++y) acc[y] += __shfl_xor(acc[y], x);
+  if constexpr (WAVES > 1) {
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (share > 0) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) acc += sums[w][lane];
+  }
   const int n = a.by_Hk.of(nh), hk = nh - n * a.Hk, t = a.by_G.of(row), hq = hk * a.G + row - t * a.G;
   if (e < a.D && part == 0) {
     const float f = none ? 0.0f : 1.0f / l;
@@ -418,8 +426,12 @@ int at_launch(const rc_attn* a, const at_args& d, const void* q, const void* k, 
   rc = rc_check_launch("rc_cross_attn_fwd");
   if (rc || sp.n == 1) return rc;
   const int64_t all = a->N * a->Hk * rows;
-  at_join_kernel<T><<<(uint32_t)((all + 3) / 4), 256, 0, st>>>((T*)out, (T*)rest, lse, sp, d, at_div((uint32_t)rows), at_div(C::ROWS),
-                                                               (int)row_tiles, all);
+  // many splits: four waves to a row (8 rows of 128 in 64 splits: a call 21.3 -> 18.6 us)
+  auto join = [&](auto kernel, int64_t blocks) {
+    kernel<<<(uint32_t)blocks, 256, 0, st>>>((T*)out, (T*)rest, lse, sp, d, at_div((uint32_t)rows), at_div(C::ROWS), (int)row_tiles, all);
+  };
+  if (sp.n > 8) join(at_join_kernel<T, 4>, all);
+  else join(at_join_kernel<T, 1>, (all + 3) / 4);
   return rc_check_launch("rc_cross_attn_fwd (join)");
 }
 
@@ -440,12 +452,14 @@ at_plan at_make_plan(const rc_attn* a) {
   p.tile_rows = p.few ? 32 : 128;
   p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   p.items = a->N * a->Hk * p.row_tiles;
-  // Fewer work items than fill the card twice: the keys are divided too, down to 256 of them; in fp32, whose products
-  // take sixteen times as long, down to 64 (128 for narrow heads, where that is the tile).  (One token in each of 16
-  // sequences, 8192 ragged keys, 32/8 heads of 128: 84 us; one over 16384 keys, 8/1 heads: 21 us, in splits of 1024 keys
+  // Fewer work items than fill the card twice: the keys are divided too, down to 256 of them, or 128 where there are
+  // rows enough (3 x 1157 x 1102, 8/4 heads of 96 in fp16: 53 us with 256, 49 with 128; one token over 3426 keys, 4 heads
+  // of 192: 22 and 27); in fp32, whose products take sixteen times as long, down to 64 (128 for narrow heads, where that
+  // is the tile; 4 x 1124 keys, 4/2 heads of 256: 38 us, 90 with 256).  (One token in each of 16
+  // sequences, 8192 ragged keys, 32/8 heads of 128: 84 us; one over 16384 keys, 8/1 heads: 19 us, in splits of 1024 keys
   // 29.)  Up to four such parts few rows stay whole: joining is a launch more (1000 keys in bf16: 14.7
   // against 18.9 us a call); fp32 heads beyond 128, which one wave goes through alone, up to one.
-  const int64_t unit = a->dtype != RC_F32 ? 256 : a->D > 32 ? 64 : 128;
+  const int64_t unit = a->dtype != RC_F32 ? (p.few ? 256 : 128) : a->D > 32 ? 64 : 128;
   int64_t n = 1;
   if (p.items > 0 && p.items < 512 && !(p.few && a->Tk <= (a->dtype == RC_F32 && a->D > 128 ? 1 : 4) * unit)) {
     n = (512 + p.items - 1) / p.items;
