@@ -15,6 +15,7 @@
 #pragma once
 #include "rc_common.h"
 
+#include <atomic>
 #include <math.h>
 
 typedef short at_s4 __attribute__((ext_vector_type(4)));
@@ -58,9 +59,9 @@ struct at_args {
   float scale, scale_log2;
 };
 
-// Raises KERNEL's limit of dynamic LDS, once per device (the call is idempotent, so racing first calls are harmless).
+// Raises KERNEL's limit of dynamic LDS, once per device (the call is idempotent: two first calls at once do it twice).
 template <auto KERNEL> int at_allow_lds(int bytes) {
-  static bool done[64];
+  static std::atomic<bool> done[64];
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e == hipSuccess && dev >= 0 && dev < 64 && done[dev]) return RC_OK;

@@ -576,6 +576,64 @@ def test_on_another_stream(R):
     assert torch.equal(got, ref)
 
 
+@pytest.mark.parametrize("Tq,Tk,D", [(1, 3000, 128), (70, 900, 64), (5, 1100, 256)])
+def test_graphs_with_masks_and_divided_keys(R, Tq, Tk, D):
+    """The mask's bits and the splits' parts are scratch of each graph; the mask is read again at every replay."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    mk = lambda *s: torch.randn(s, generator=g, device="cuda").half()
+    sets = [[mk(2, Tq, 4, D), mk(2, Tk, 2, D), mk(2, Tk, 2, D), torch.rand(2, Tk, generator=g, device="cuda") < 0.5] for _ in range(2)]
+    call = lambda x: R.cross_attention_hip(*x[:3], key_mask=x[3])
+    call(sets[0])
+    torch.cuda.synchronize()
+    graphs = []
+    for x in sets:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = call(x)
+        graphs.append((gr, out))
+    for r in range(5):
+        for x, (gr, out) in zip(sets, graphs):
+            x[0].copy_(mk(*x[0].shape))
+            x[3].copy_(torch.rand(x[3].shape, generator=g, device="cuda") < 0.2 * r)     # none at all the first time
+            want = call(x)
+            gr.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            assert r or not out.any()
+
+
+def test_two_threads_at_once(R):
+    """Each thread on a stream of its own, forward and back, against the same calls one after the other."""
+    from concurrent.futures import ThreadPoolExecutor
+    shapes = [(3, 1, 3000, 4, 2, 128), (300, 40, 60, 2, 2, 32), (2, 300, 700, 4, 2, 96), (2, 90, 130, 2, 1, 256)]
+    sets = []
+    for n, (N, Tq, Tk, Hq, Hk, D) in enumerate(shapes):
+        g = torch.Generator(device="cuda").manual_seed(n)
+        mk = lambda *s: torch.randn(s, generator=g, device="cuda").bfloat16()
+        sets.append((mk(N, Tq, Hq, D), mk(N, Tk, Hk, D), mk(N, Tk, Hk, D), torch.rand(N, Tk, generator=g, device="cuda") < 0.7))
+
+    def run(x):
+        t = [y.detach().requires_grad_() for y in x[:3]]
+        q, k = R.qk_norm_rotate_hip(t[0], t[1])
+        out = R.cross_attention_hip(q, k, t[2], key_mask=x[3])
+        return (out.detach(),) + torch.autograd.grad(out, t, out.detach())
+
+    want = [run(x) for x in sets]
+    torch.cuda.synchronize()
+
+    def worker(order):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            got = [(i, run(sets[i])) for _ in range(4) for i in order]
+        st.synchronize()
+        return got
+
+    with ThreadPoolExecutor(2) as pool:
+        for got in pool.map(worker, ([0, 1, 2, 3], [3, 2, 1, 0])):
+            for i, tensors in got:
+                assert all(torch.equal(a, b) for a, b in zip(tensors, want[i])), shapes[i]
+
+
 @pytest.mark.parametrize("Tq,Tk", [(1, 900), (70, 90)])
 def test_inference_graphs(R, Tq, Tk):
     """Two graphs captured side by side, replayed in turn with eager calls between them."""
