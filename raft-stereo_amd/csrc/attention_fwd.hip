@@ -289,8 +289,8 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
   any = __builtin_amdgcn_readfirstlane(any);
 
   if (sp.n > 1) {
-    // no key at all: sum 0; keys, but every score -inf: NaN, as 0 / 0 is
-    l = any ? (l == 0.0f ? NAN : l) : 0.0f;
+    // no key at all: sum 0; keys, but every score -inf: sum -1, which the join counts as nothing (a sum is positive or NaN)
+    l = any ? (l == 0.0f ? -1.0f : l) : 0.0f;
     float* ml = sp.ml + (int64_t)item * 2 * C::ROWS + wq * 32;
     if (wk == 0 && h == 0) {
       ml[c] = m;
@@ -344,17 +344,19 @@ __global__ __launch_bounds__(256) void at_join_kernel(T* __restrict__ out, T* __
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
   float l = 0.0f;
+  bool keys = false;
   for (int s = lane; s < sp.n; s += 64) {
     const float* ml = sp.ml + (item0 + (int64_t)s * row_tiles) * 2 * tile_rows + r;
     const float mi = ml[0], li = ml[tile_rows];
-    // (sum 0: no key in this split)
-    const float w = li == 0.0f || mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - top);
+    // a weight of -1: no key in this split.  A split of -inf alone has the weight 0: its values count if they are not finite
+    const float w = li == 0.0f ? -1.0f : mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - top);
     weights[wave][s] = w;
-    l += li == 0.0f ? 0.0f : mi == -INFINITY ? li * 0.0f : w * li;  // (a NaN stays one)
+    keys |= li != 0.0f;
+    l += li == 0.0f ? 0.0f : mi == -INFINITY ? (li < 0.0f ? 0.0f : li) : w * li;  // (a NaN stays one)
   }
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x);
-  const bool none = l == 0.0f;
+  const bool none = !__any(keys);  // (keys, but a sum of 0: 0 / 0)
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   int group = 2;  // lanes of a group: D / 4 rounded up to a power of two
   while (group * 4 < a.D) group *= 2;
@@ -366,7 +368,7 @@ __global__ __launch_bounds__(256) void at_join_kernel(T* __restrict__ out, T* __
 #pragma unroll 8
     for (int s = share * parts + part; s < sp.n; s += parts * WAVES) {
       const float w = weights[wave][s];
-      if (w != 0.0f) acc += w * *reinterpret_cast<const at_f4*>(o + s * step);
+      if (!(w < 0.0f)) acc += w * *reinterpret_cast<const at_f4*>(o + s * step);
     }
   }
   for (int x = group; x < 64; x <<= 1)

@@ -1,0 +1,71 @@
+"""GPU tests of the attention operators where the way that the library takes decides: infinite scores in parts of divided
+keys, many parts, rows that end inside a tile, long rows in fp16, norms of more tokens than one block's share.  Expected
+values and bounds are the oracle's (64-bit formulas; element by element the roundings that the operators document)."""
+import numpy as np
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from oracle import attention_oracle as A
+from test_gpu_attention import DT, assert_within, host, norm_inputs, rand, run_attention
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+
+
+@pytest.fixture(scope="module")
+def R():
+    import raft_stereo_amd
+    assert torch.cuda.is_available(), "these tests need a GPU"
+    return raft_stereo_amd
+
+
+# ---------------------------------------------------------------------------------- allowed keys with infinite scores
+def with_bias_column(rng, shape, dtype, out):
+    """Operands whose last key element is a bias (the queries have a one there), -inf for the keys in `out`."""
+    N, Tq, Tk, Hq, Hk, D = shape
+    q, k, v = rand(rng, (N, Tq, Hq, D), dtype), rand(rng, (N, Tk, Hk, D), dtype), rand(rng, (N, Tk, Hk, D), dtype)
+    g = rand(rng, (N, Tq, Hq, D), dtype)
+    q[..., -1] = 1.0
+    k[..., -1] = torch.where(torch.from_numpy(out)[:, :, None], -INF, k[..., -1])
+    return q, k, v, g
+
+
+DIVIDED = [(1, 1, 3000, 4, 2, 64), (2, 3, 1500, 4, 1, 128), (1, 2, 1500, 2, 1, 256), (2, 70, 1500, 2, 1, 64),
+           (1, 40, 700, 1, 1, 256), (1, 5, 2600, 2, 1, 24)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", DIVIDED, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("where", ["first", "middle", "all but the last"])
+def test_minus_infinity_in_a_part_of_divided_keys(R, shape, dtype, where):
+    """A score of -inf is a probability of zero, wherever the keys are cut."""
+    N, Tk = shape[0], shape[2]
+    out = np.zeros((N, Tk), bool)
+    out[:, {"first": slice(0, 513), "middle": slice(Tk // 3, Tk - 64), "all but the last": slice(0, Tk - 1)}[where]] = True
+    q, k, v, g = with_bias_column(np.random.default_rng(len(where)), shape, dtype, out)
+    want = A.attention(host(q), np.nan_to_num(host(k), neginf=0.0), host(v), host(g), ~out, dtype=dtype)
+    got = run_attention(R, q, k, v, g, None, None, dtype)
+    assert_within(got["out"], want["out"], "out")
+    assert_within(run_attention(R, q, k, v, None, None, None, dtype)["out"], want["out"], "out (inference)")
+    # (the last element of dq is 0 times -inf)
+    assert_within(got["dq"][..., :-1], [x[..., :-1] for x in want["dq"]], "dq")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(3, 1, 3000, 4, 2, 64), (3, 70, 1500, 2, 1, 64), (3, 1, 40, 4, 2, 64)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_rows_without_a_finite_score(R, shape, dtype):
+    """Keys, but every score -inf: NaN, as 0 / 0 is.  No key: zeros.  A value that is not finite shows, however small its
+    probability.  The same where the keys are divided and where they are not."""
+    N, Tk = shape[0], shape[2]
+    out = np.zeros((N, Tk), bool)
+    out[0] = True
+    out[2, Tk // 2:] = True
+    q, k, v, _ = with_bias_column(np.random.default_rng(1), shape, dtype, out)
+    v[2, -1, :, 5] = INF
+    got = run_attention(R, q, k, v, None, [Tk, 0, Tk], None, dtype)["out"]
+    assert got[0].isnan().all() and not got[1].any()
+    assert got[2, ..., 5].isnan().all() and got[2, ..., :5].isfinite().all() and got[2, ..., 6:].isfinite().all()
+    k[2, 7] = float("nan")
+    assert run_attention(R, q, k, v, None, [Tk, 0, Tk], None, dtype)["out"][2].isnan().all()
