@@ -304,6 +304,8 @@ __device__ __forceinline__ void at_mma_cols(const at_places<T, DC>& at, const un
 // the swizzle is applied to the addresses that the lanes fetch from.  Chunks behind the head's end and rows that do
 // not take part are fetched from beyond the buffer's range, which gives zeros (so whatever those rows hold, NaN
 // included, never meets a product).
+// Behind the last query row it is that row, and its lse2, that the backward pass's tiles repeat, beside zeros for dO and
+// delta: P is then the row's own, and adds P times zero.  (Zeros for the query would make P NaN at an infinite key.)
 // (128 rows under 8 MiB apart: offsets and scalar offsets stay under 2^30, and AT_OUTSIDE outside without a wrap)
 constexpr uint32_t AT_RANGE = 0x80010000u, AT_OUTSIDE = 0xc0000000u;
 
@@ -359,6 +361,18 @@ template <typename T, int DC, int ROWS, int WAVES> struct at_stage {
       outside[p] = (uint32_t)__builtin_amdgcn_sbfe((int)~w, (p * STEP + wave * PER + lane / R::CH) & 31, 1) & AT_OUTSIDE;
     }
   }
+  // base: the tile's first row; in place of the rows behind `last`, that row again
+  __device__ __forceinline__ void issue_repeat(const char* base, uint32_t lds, int wave, int lane, int last) const {
+    const at_i4 rs = at_buffer(base);
+    const uint32_t stride = ahead / (PD * STEP);
+#pragma unroll
+    for (int p = 0; p < N; ++p) {
+      const int behind = max(p * STEP + wave * PER + lane / R::CH - last, 0);
+      const uint32_t at = off[p % PD] + (uint32_t)(p / PD) * ahead - (uint32_t)behind * stride;
+      at_load_lds(rs, off[p % PD] == AT_OUTSIDE ? AT_OUTSIDE : at, 0u,
+                  __builtin_amdgcn_readfirstlane(lds + (uint32_t)((p * WAVES + wave) * 1024 + (((p * WAVES + wave) * PER) >> 3) * R::PAD)));
+    }
+  }
   // base: the tile's first row; FULL: every row takes part
   template <bool FULL> __device__ __forceinline__ void issue(const char* base, uint32_t lds, int wave, const uint32_t (&outside)[N]) const {
     const at_i4 rs = at_buffer(base);
@@ -369,13 +383,14 @@ template <typename T, int DC, int ROWS, int WAVES> struct at_stage {
   }
 };
 
-// instruction i of the loads of 32 rows from `base` (bit r of take: row r takes part)
+// instruction i of the loads of 32 rows from `base` (bit r of take: row r takes part; behind `last`, that row again)
 template <typename T, int DC>
-__device__ __forceinline__ void at_fetch_rows(const void* base, uint32_t stride, int D, uint32_t take, uint32_t lds, int i, int lane) {
+__device__ __forceinline__ void at_fetch_rows(const void* base, uint32_t stride, int D, uint32_t take, uint32_t lds, int i, int lane,
+                                              int last = 31) {
   using R = at_row<T, DC>;
   constexpr int PER = 1024 / R::RB;
   const int r = i * PER + lane / R::CH, chunk = (lane % R::CH) ^ at_swizzle<R::CH>(r);
-  const uint32_t off = chunk * 16 < D * R::ES && ((take >> r) & 1) ? (uint32_t)r * stride + (uint32_t)chunk * 16u : AT_OUTSIDE;
+  const uint32_t off = chunk * 16 < D * R::ES && ((take >> r) & 1) ? (uint32_t)min(r, last) * stride + (uint32_t)chunk * 16u : AT_OUTSIDE;
   at_load_lds(at_buffer(base), off, 0u, __builtin_amdgcn_readfirstlane(lds + (uint32_t)(i * 1024 + ((i * PER) >> 3) * R::PAD)));
 }
 
@@ -437,9 +452,10 @@ __device__ __forceinline__ void at_sync() {
   asm volatile("" ::: "memory");
 }
 
-// up to 64 floats to LDS, zeros behind the first `left`
-__device__ __forceinline__ void at_fetch_floats(const float* base, int left, uint32_t lds, int lane) {
-  at_load_lds<true>(at_buffer(base), lane < left ? (uint32_t)lane * 4u : AT_OUTSIDE, 0u, __builtin_amdgcn_readfirstlane(lds));
+// up to 64 floats to LDS; behind the first `left`, zeros, or (REPEAT) the last of them
+template <bool REPEAT = false> __device__ __forceinline__ void at_fetch_floats(const float* base, int left, uint32_t lds, int lane) {
+  const uint32_t off = REPEAT ? (uint32_t)min(lane, left - 1) * 4u : lane < left ? (uint32_t)lane * 4u : AT_OUTSIDE;
+  at_load_lds<true>(at_buffer(base), off, 0u, __builtin_amdgcn_readfirstlane(lds));
 }
 
 // Block id -> work item.  Ids go round the 8 XCDs; items that share keys stay on one XCD and its L2, and units of them

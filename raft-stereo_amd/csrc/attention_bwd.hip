@@ -140,7 +140,7 @@ template <typename T, int DC, int RT, int NW, int HALVES> struct at_dkv_lds {
   static_assert(HALVES == 1 || NW * DC / 32 * 16 * 64 * 4 <= V, "a wave's sums pass through the tiles' place");
 };
 
-// rows t0 .. of one query head: Q, dO, lse2 and delta
+// rows t0 .. of one query head: Q, dO, lse2 and delta (behind the last row: its Q and lse2 again, zeros for the others)
 template <typename T, int DC, int RT, int NW> struct at_query_tiles {
   using S = at_stage<T, DC, RT, NW>;
   S sq, sg;
@@ -164,11 +164,11 @@ template <typename T, int DC, int RT, int NW> struct at_query_tiles {
 #pragma unroll
       for (int i = 0; i < RT / 32; ++i) words[i] = at_first_bits(left - 32 * i);
       S::spread(words, wave, lane, outside);
-      sq.template issue<false>(qp, lds_q, wave, outside);
+      sq.issue_repeat(qp, lds_q, wave, lane, left - 1);
       sg.template issue<false>(gp, lds_g, wave, outside);
     }
     const int64_t srow = ((int64_t)n * a.Hq + hq) * a.Tq + t0;
-    if (wave == 0) at_fetch_floats(lse + srow, left, lds_l, lane);
+    if (wave == 0) at_fetch_floats<true>(lse + srow, left, lds_l, lane);
     if (wave == NW - 1) at_fetch_floats(delta + srow, left, lds_d, lane);
   }
 };

@@ -130,7 +130,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_rows_kernel(const T* __restri
     const int g = by_batches.of(b), hq = hk * a.G + g, t0 = (b - g * batches) * 32 * NW;
     const int tiles = min(NW, (a.Tq - t0 + 31) >> 5);
     if (b > 0) at_sync();  // nobody reads the last batch any more
-    // 32 rows a wave: Q, dO and lse2 to LDS; delta, as soon as the wave's own loads have landed
+    // 32 rows a wave: Q, dO and lse2 to LDS (behind the last row: its Q and lse2 again); delta, as soon as the wave's own
+    // loads have landed
     if (wave < tiles) {
       const int t = t0 + 32 * wave, left = a.Tq - t;
       const uint32_t take = at_first_bits(left);
@@ -139,10 +140,10 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_rows_kernel(const T* __restri
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         at_fetch_rows<T, DC>(q + (int64_t)n * a.qs[0] + (int64_t)t * a.qs[1] + (int64_t)hq * a.qs[2], (uint32_t)(a.qs[1] * sizeof(T)), a.D,
-                             take, lds0 + L::Q + R::at(32) * wave, i, lane);
+                             0xffffffffu, lds0 + L::Q + R::at(32) * wave, i, lane, left - 1);
         at_fetch_rows<T, DC>(dout + o, ost, a.D, take, lds0 + L::G + R::at(32) * wave, i, lane);
       }
-      at_fetch_floats(lse + ((int64_t)n * a.Hq + hq) * a.Tq + t, left, lds0 + L::LSE + L::STAT * wave, lane);
+      at_fetch_floats<true>(lse + ((int64_t)n * a.Hq + hq) * a.Tq + t, left, lds0 + L::LSE + L::STAT * wave, lane);
       at_u4 of[R::STEPS];
       at_rows_of(out + o).row<T, DC>(c < left ? (uint32_t)c * ost : AT_OUTSIDE, a.D, lane, of);
       constexpr int RESTS = sizeof(T) == 2 ? R::STEPS : 1;

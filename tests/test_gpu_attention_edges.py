@@ -69,3 +69,21 @@ def test_rows_without_a_finite_score(R, shape, dtype):
     assert got[2, ..., 5].isnan().all() and got[2, ..., :5].isfinite().all() and got[2, ..., 6:].isfinite().all()
     k[2, 7] = float("nan")
     assert run_attention(R, q, k, v, None, [Tk, 0, Tk], None, dtype)["out"][2].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(260, 20, 33, 1, 1, 32), (130, 37, 100, 4, 2, 64), (64, 100, 380, 4, 4, 24), (2, 70, 150, 2, 1, 64),
+                                   (1, 90, 300, 4, 2, 96), (2, 130, 129, 2, 2, 128), (1, 33, 70, 2, 1, 160), (1, 65, 90, 1, 1, 256)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_infinite_keys_beside_query_rows_that_end_inside_a_tile(R, shape, dtype):
+    """Keys with scores of -inf have gradients of zero; the places behind the last query row add nothing to them."""
+    N, Tq, Tk = shape[:3]
+    rng = np.random.default_rng(2)
+    out = rng.random((N, Tk)) < 0.3
+    out[:, 0] = False
+    q, k, v, g = with_bias_column(rng, shape, dtype, out)
+    want = A.attention(host(q), np.nan_to_num(host(k), neginf=0.0), host(v), host(g), ~out, dtype=dtype)
+    got = run_attention(R, q, k, v, g, None, None, dtype)
+    for name in ("out", "dk", "dv"):
+        assert_within(got[name], want[name], name)
+    assert not got["dk"].cpu()[torch.from_numpy(out)].any() and not got["dv"].cpu()[torch.from_numpy(out)].any()
