@@ -58,7 +58,10 @@ def attention(q, k, v, g=None, ok=None, scale=None, dtype="f32"):
     # exp2 gives zero for what is below fp32's smallest normal number: a probability, its sum being at least 1, may be off
     # by that much however small it is
     flush = 2.0 ** -126
-    tiny = flush + 2.0 ** -25 if dtype == "f16" else flush       # (half a step of fp16's smallest numbers)
+    # fp16: half a step of its smallest numbers, 2^-25, of probabilities that are multiplied by 2^7 at least (2^12 in the
+    # gradients' pass)
+    tiny = flush + 2.0 ** -32 if dtype == "f16" else flush
+    tiny_back = flush + 2.0 ** -37 if dtype == "f16" else flush
     rnd = 0.0 if dtype == "f32" else u
     A = P @ np.abs(V)
     o_err = (rnd + rel + Tk * F32) * A + tiny * np.abs(V).sum(axis=2, keepdims=True)
@@ -85,7 +88,7 @@ def attention(q, k, v, g=None, ok=None, scale=None, dtype="f32"):
     dK = np.swapaxes(dS, 2, 3) @ Q * scale
     k_err = np.swapaxes(cols_err + G * Tq * F32 * np.abs(dS), 2, 3) @ np.abs(Q) * scale
     dV = np.swapaxes(P, 2, 3) @ Gr
-    p_err = P * (rnd + rel + G * Tq * F32) + flush + (tiny - flush) * 2.0 ** -8
+    p_err = P * (rnd + rel + G * Tq * F32) + tiny_back
     v_err = np.swapaxes(p_err * np.ones_like(P), 2, 3) @ np.abs(Gr)
     res["dq"] = (back(dQ), back(q_err + u * np.abs(dQ) + 1e-37))
     for name, d, e in (("dk", dK, k_err), ("dv", dV, v_err)):

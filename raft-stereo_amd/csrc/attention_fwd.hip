@@ -21,12 +21,15 @@
 namespace {
 
 // Scores are compared and exponentiated in units of log2: p = exp2(s c - m), c = scale log2 e.  The accumulators are
-// rescaled only when a maximum grows by more than this (p stays under 2^8, where fp16 and fp32 have range to spare).
+// rescaled only when a maximum grows by more than AT_SLACK.  In fp16, p is rounded to numbers that end at 2^-24, and a long
+// row's small probabilities, each lost, would be missed together (8192 of 2^-26 are 1.2e-4 of the row): m lies AT_LIFT below
+// the maximum, so that p ends at 2^-31 of it and stays under 2^15.
 constexpr float AT_SLACK = 8.0f;
+template <typename T> constexpr float AT_LIFT = at_fit<T>::ON ? 7.0f : 0.0f;
 
 struct at_split {
   float* o;     // [item][split][rows][D]: unnormalised sums
-  float* ml;    // [item][split][2][rows]: maxima, sums
+  float* ml;    // [item][split][2][rows]: maxima (in fp16 AT_LIFT below), sums
   int32_t n;    // splits of the keys
   int32_t keys; // of one split, a multiple of the tile
 };
@@ -132,7 +135,7 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
     for (int b = 0; b < NKB; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
-    return at_half_max(mx) * a.scale_log2;
+    return at_half_max(mx) * a.scale_log2 - AT_LIFT<T>;
   };
   auto raise = [&](float mx) {
     if (__any(mx > m + AT_SLACK)) {
@@ -218,7 +221,7 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
         __builtin_amdgcn_sched_barrier(0);
       }
       priority(0);
-      mx = at_half_max(mx) * a.scale_log2;
+      mx = at_half_max(mx) * a.scale_log2 - AT_LIFT<T>;
       raise(mx);
     };
     for (int j = 0; j < tiles; j += 2) {

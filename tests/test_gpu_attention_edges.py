@@ -87,3 +87,26 @@ def test_infinite_keys_beside_query_rows_that_end_inside_a_tile(R, shape, dtype)
     for name in ("out", "dk", "dv"):
         assert_within(got[name], want[name], name)
     assert not got["dk"].cpu()[torch.from_numpy(out)].any() and not got["dv"].cpu()[torch.from_numpy(out)].any()
+
+
+# --------------------------------------------------------------------------------------------- long rows and many parts
+@pytest.mark.parametrize("D, Tq", [(64, 1), (64, 40), (32, 40), (128, 40), (128, 1), (256, 40)])
+def test_fp16_keeps_the_tail_of_a_long_row(R, D, Tq):
+    """One dominant key and thousands whose probabilities lie below fp16's smallest number: together they count.  (Enough
+    sequences that the keys are not divided; they share the operands.)"""
+    N, Tk = 512, 8192
+    q, k, v = torch.zeros(1, Tq, 1, D), torch.zeros(1, Tk, 1, D), torch.ones(1, Tk, 1, D)
+    q[..., 0] = 4.0
+    k[0, 0, 0, 0], v[0, 0] = 4.5, 0.0         # scores of 18 and 0: 2^-25.97
+    v[..., D // 2:] = 0.0
+    q, k, v = q.half(), k.half(), v.half()
+    g = rand(np.random.default_rng(0), (1, Tq, 1, D), "f16")
+    want = A.attention(*(host(x) for x in (q, k, v, g)), None, scale=1.0, dtype="f16")
+    t = [x.cuda().expand(N, -1, -1, -1).detach().requires_grad_() for x in (q, k, v)]
+    out = R.cross_attention_hip(*t, scale=1.0)
+    assert torch.equal(out, out[:1].expand_as(out))
+    assert_within(out[:1], want["out"], "out")
+    if D == 64:
+        grads = torch.autograd.grad(out, t, g.cuda().expand(N, -1, -1, -1))
+        for name, d in zip(("dq", "dk", "dv"), grads):
+            assert_within(d[:1], want[name], name)
