@@ -12,6 +12,7 @@ torch's, like the convolutions of the update block.  There is no CPU or eager fa
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from raft_stereo_amd import _lib
@@ -40,6 +41,14 @@ def _check_same(t, like, what, of):
         raise TypeError(f"{what} is {t.dtype}, {of} {like.dtype}")
     if t.device != like.device:
         raise RuntimeError(f"{what} and {of} live on different devices")
+
+
+def _refuse_duals(what, *tensors):
+    """There is no forward-mode derivative, and the kernels would drop a dual tensor's tangent without a word."""
+    if getattr(forward_ad, "_current_level", 0) < 0:      # (outside every dual_level: nothing to look for)
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative: its operands must not be dual tensors")
 
 
 def _heads_view(t):
@@ -184,7 +193,8 @@ def qk_norm_rotate_hip(q, k=None, q_weight=None, k_weight=None, freqs=None, q_po
     first `2 n` for the n frequencies in `freqs` (float32 or float64, radians per position; None: the norm alone).
     Positions are `[T]` or `[N, T]`, int32, int64 or float32 (None: 0, 1, ...); angles are reduced to one turn in
     64 bits, so positions far along lose nothing.  Everything else is fp32 and rounded once.  n must be a multiple of 4.
-    Returns `(q', k')`, contiguous, or `q'` alone if k is None.  Differentiable w.r.t. q, k and the weights."""
+    Returns `(q', k')`, contiguous, or `q'` alone if k is None.  Differentiable w.r.t. q, k and the weights, once, in
+    reverse mode (dual tensors are refused)."""
     _check_heads(q, "q")
     _check_weight(q_weight, q, "q_weight")
     if k is not None:
@@ -195,6 +205,7 @@ def qk_norm_rotate_hip(q, k=None, q_weight=None, k_weight=None, freqs=None, q_po
         _check_weight(k_weight, k, "k_weight")
     elif k_weight is not None or k_pos is not None:
         raise ValueError("k_weight and k_pos need k")
+    _refuse_duals("qk_norm_rotate_hip", q, k, q_weight, k_weight, freqs, q_pos, k_pos)
     if freqs is not None:
         if freqs.dim() != 1 or freqs.shape[0] % 4 or 2 * freqs.shape[0] > q.shape[3]:
             raise ValueError(f"freqs must be [n] with n a multiple of 4 and at most {q.shape[3] // 2}, "
@@ -299,7 +310,8 @@ def cross_attention_hip(q, k, v, key_mask=None, key_lengths=None, scale=None):
     `[N, Tk]`); what the others hold, infinities and NaN included, has no influence.  A sequence without any key gives
     zeros, and zero gradients.  Scores, the softmax's maximum and sum, and all products' sums are fp32; 16-bit operands
     have their probabilities (and in the backward pass their scores' gradients) rounded to 16 bits for the second
-    product.  Returns `[N, Tq, Hq, D]` contiguous.  Differentiable w.r.t. q, k and v, the same bits on every run."""
+    product.  Returns `[N, Tq, Hq, D]` contiguous.  Differentiable w.r.t. q, k and v, once, in reverse mode (dual tensors
+    are refused); the same bits on every run."""
     for t, what in ((q, "q"), (k, "k"), (v, "v")):
         _check_heads(t, what)
     for t, what in ((k, "k"), (v, "v")):
@@ -327,6 +339,7 @@ def cross_attention_hip(q, k, v, key_mask=None, key_lengths=None, scale=None):
         if key_lengths.device != q.device:
             raise RuntimeError("key_lengths lives on a different device than q")
         key_lengths = key_lengths.contiguous()
+    _refuse_duals("cross_attention_hip", q, k, v)
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"scale must be positive and finite, got {scale}")

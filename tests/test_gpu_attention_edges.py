@@ -110,3 +110,26 @@ def test_fp16_keeps_the_tail_of_a_long_row(R, D, Tq):
         grads = torch.autograd.grad(out, t, g.cuda().expand(N, -1, -1, -1))
         for name, d in zip(("dq", "dk", "dv"), grads):
             assert_within(d[:1], want[name], name)
+
+
+# -------------------------------------------------------------------------------------------------- forward mode
+def test_forward_mode_is_refused(R):
+    """There is no forward-mode derivative: a dual operand raises, it does not lose its tangent."""
+    x, w = torch.randn(1, 6, 2, 32, device="cuda"), torch.ones(32, device="cuda")
+    freqs = torch.ones(16, device="cuda")
+    plain = R.cross_attention_hip(x, x, x), R.qk_norm_rotate_hip(x, x, w, w, freqs)
+    with forward_ad.dual_level():
+        for i in range(3):
+            args = [x, x, x]
+            args[i] = forward_ad.make_dual(x, torch.ones_like(x))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                R.cross_attention_hip(*args)
+        for i in range(4):
+            args = [x, x, w, w]
+            args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                R.qk_norm_rotate_hip(*args, freqs)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            R.qk_norm_rotate_hip(x, x, w, w, forward_ad.make_dual(freqs, freqs))
+        assert torch.equal(R.cross_attention_hip(x, x, x), plain[0])     # no dual operand: nothing to refuse
+        assert torch.equal(R.qk_norm_rotate_hip(x, x, w, w, freqs)[0], plain[1][0])
