@@ -357,7 +357,7 @@ class RowAttentionHip(nn.Module):
     (rectified stereo: its match lies there, which is also why the correlation is one-dimensional, core/corr.py:148-156).
     Queries and keys are normalised per head and rotated by their column.  `width1` / `width2` (int32 or int64 `[B]`):
     columns of each image that hold data; the padding behind them is not attended to.  Handed to
-    `make_corr_fn(..., attention=module)`, it runs in front of the volume."""
+    `make_corr_fn(..., attention=module)`, which takes the widths too, it runs in front of the volume."""
 
     def __init__(self, dim, heads=4, kv_heads=None, head_dim=None, base=10000.0, eps=1e-6):
         super().__init__()

@@ -26,20 +26,24 @@ def wants_autocast(corr_implementation):
 
 
 def make_corr_fn(corr_implementation, fmap1, fmap2, radius=4, num_levels=4, mixed_precision=False, out_dtype=None,
-                 attention=None):
+                 attention=None, width1=None, width2=None):
     """What core/raft_stereo.py:90-100 does for the names this package owns.  Unknown names
     raise (the reference falls through its if/elif and dies with UnboundLocalError).
     out_dtype (reg_hip with 16-bit feature maps only): the taps in the volume's dtype, as the reference's
     reg_cuda block returns them (core/corr.py:44-51), instead of fp32.
-    attention: a module (RowAttentionHip) that takes both feature maps and returns them, run in front of the volume."""
+    attention: a module (RowAttentionHip) that takes both feature maps and returns them, run in front of the volume.
+    width1 / width2 (with attention, for padded batches): columns of each image that hold data, handed on to it."""
     if corr_implementation not in CORR_IMPLEMENTATIONS:
         raise ValueError(f"corr_implementation {corr_implementation!r} is not provided by raft_stereo_amd; "
                          f"choices: {sorted(CORR_IMPLEMENTATIONS)}")
+    widths = {name: w for name, w in (("width1", width1), ("width2", width2)) if w is not None}
+    if widths and attention is None:
+        raise ValueError("width1 and width2 say what attention may look at: they need attention")
     cls, to_fp32 = CORR_IMPLEMENTATIONS[corr_implementation]
     if to_fp32 and not mixed_precision:
         fmap1, fmap2 = fmap1.float(), fmap2.float()
     if attention is not None:
-        fmap1, fmap2 = attention(fmap1, fmap2)
+        fmap1, fmap2 = attention(fmap1, fmap2, **widths)
     if out_dtype is not None:
         if cls is not CorrBlock1DHip:
             raise ValueError(f"out_dtype is a reg_hip option, not one of {corr_implementation!r}")

@@ -1,0 +1,21 @@
+"""CPU-side checks of the attention operators beside test_cpu_attention.py: arguments that are handed on or refused before
+anything is launched."""
+import pytest
+import torch
+
+
+def test_widths_reach_the_attention_in_front_of_the_volume():
+    import raft_stereo_amd as R
+    f, w1, w2 = torch.zeros(2, 8, 2, 16), torch.tensor([16, 9]), torch.tensor([7, 16])
+    seen = []
+
+    def attention(*args, **kw):
+        seen.append((len(args), kw))
+        return args[:2]
+    for kw in ({}, dict(width1=w1), dict(width2=w2), dict(width1=w1, width2=w2)):
+        with pytest.raises(RuntimeError, match="no CPU path"):       # from the block, behind the attention
+            R.make_corr_fn("reg_hip", f, f, attention=attention, **kw)
+        assert seen.pop() == (2, kw)
+    for kw in (dict(width1=w1), dict(width2=w2)):
+        with pytest.raises(ValueError, match="need attention"):
+            R.make_corr_fn("reg_hip", f, f, **kw)

@@ -133,3 +133,19 @@ def test_forward_mode_is_refused(R):
             R.qk_norm_rotate_hip(x, x, w, w, forward_ad.make_dual(freqs, freqs))
         assert torch.equal(R.cross_attention_hip(x, x, x), plain[0])     # no dual operand: nothing to refuse
         assert torch.equal(R.qk_norm_rotate_hip(x, x, w, w, freqs)[0], plain[1][0])
+
+
+# ------------------------------------------------------------------------------------------------ widths on the way
+@pytest.mark.parametrize("impl", ["reg_hip", "alt_hip"])
+def test_padded_batches_in_front_of_the_volume(R, impl):
+    """What lies behind an image's columns has no influence on the other image's features."""
+    torch.manual_seed(3)
+    m = R.RowAttentionHip(32, heads=2).cuda()
+    f1, f2 = torch.randn(2, 32, 4, 48, device="cuda"), torch.randn(2, 32, 4, 48, device="cuda")
+    w1, w2 = torch.tensor([48, 30], device="cuda"), torch.tensor([41, 48], device="cuda")
+    coords = torch.rand(2, 2, 4, 48, device="cuda") * 48
+    with torch.no_grad():
+        got = R.make_corr_fn(impl, f1, f2, attention=m, width1=w1, width2=w2)(coords)
+        assert torch.equal(got, R.make_corr_fn(impl, *m(f1, f2, w1, w2))(coords))
+        one = R.make_corr_fn(impl, f1, f2, attention=m, width2=w2)(coords)
+        assert torch.equal(one, R.make_corr_fn(impl, *m(f1, f2, None, w2))(coords)) and not torch.equal(one, got)
