@@ -503,7 +503,7 @@ typedef struct rc_attn {
   const unsigned char* key_mask;    /* [N, Tk]; NULL */
   int32_t Hq, Hk, D, dtype;
   int32_t lengths_i64;
-  float scale;                      /* positive and finite */
+  float scale;                      /* positive and below 2^127 */
 } rc_attn;
 
 /* out [N, Tq, Hq, D].  For the backward pass, NULL in inference: lse float [N, Hq, Tq], the log-sum-exp of each row's

@@ -341,8 +341,8 @@ def cross_attention_hip(q, k, v, key_mask=None, key_lengths=None, scale=None):
         key_lengths = key_lengths.contiguous()
     _refuse_duals("cross_attention_hip", q, k, v)
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 0.0 < scale < 2.0 ** 127:       # (times log2 e, it has to be an fp32 number)
+        raise ValueError(f"scale must be positive and below 2^127, got {scale}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _CrossAttentionFn.apply(q, k, v, key_mask, key_lengths, scale)
     return _attention_raw(*_attn_desc(q, k, v, key_mask, key_lengths, scale), False)[0]

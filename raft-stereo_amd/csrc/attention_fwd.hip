@@ -524,7 +524,8 @@ int at_check(const rc_attn* a) {
   RC_REQUIRE(a->Tq < (1ll << 30) && a->Tk < (1ll << 30) && a->N * a->Tq < (1ll << 31) && a->N * a->Tk < (1ll << 31) &&
                  a->N * a->Tq * a->Hq < (1ll << 31) && a->N * a->Tk * a->Hk < (1ll << 31) && a->N * a->Hk < (1ll << 31),
              RC_EINVAL, "rc_cross_attn: more than 2^31 heads");
-  RC_REQUIRE(a->scale > 0.0f && a->scale < INFINITY, RC_EINVAL, "rc_cross_attn: scale must be positive and finite");
+  // (scale log2 e has to be finite too: an infinite factor makes NaN of a score of zero)
+  RC_REQUIRE(a->scale > 0.0f && a->scale < 0x1p127f, RC_EINVAL, "rc_cross_attn: scale must be positive and below 2^127");
   const int64_t es = a->dtype == RC_F32 ? 4 : 2;
   const int64_t* st[3] = {a->q_stride, a->k_stride, a->v_stride};
   for (int o = 0; o < 3; ++o)

@@ -19,3 +19,13 @@ def test_widths_reach_the_attention_in_front_of_the_volume():
     for kw in (dict(width1=w1), dict(width2=w2)):
         with pytest.raises(ValueError, match="need attention"):
             R.make_corr_fn("reg_hip", f, f, **kw)
+
+
+def test_scales_beyond_fp32_in_log2_are_refused():
+    from raft_stereo_amd._lib import lib
+    from test_cpu_attention import attn
+    assert lib.rc_cross_attn_fwd_work_bytes(attn(scale=2.0 ** 126)) >= 0
+    for scale in (2.0 ** 127, 3.0e38):         # finite, but not times log2 e
+        a = attn(scale=scale)
+        assert lib.rc_cross_attn_fwd_work_bytes(a) == lib.rc_cross_attn_bwd_work_bytes(a) == -1
+        assert lib.rc_cross_attn_fwd(a, 16, 16, 16, 16, None, None, 16, None) == -1
