@@ -379,12 +379,14 @@ class RowAttentionHip(nn.Module):
 
     def _make_freqs(self, device):
         n = self.head_dim // 8 * 4
-        return (self.base ** (-torch.arange(n, dtype=torch.float64) / n)).to(device)   # the same bits on any device
+        return (self.base ** (-torch.arange(n, dtype=torch.float64, device="cpu") / n)).to(device)   # the same bits on any device
 
     def _apply(self, *args, **kwargs):
-        """`.half()` and the like move the frequencies, but do not round them."""
+        """The frequencies are moved with the module, but neither rounded (`.half()`) nor left as empty storage is
+        (`.to_empty()`): wherever they are replaced, they are made again."""
+        before = self.freqs
         super()._apply(*args, **kwargs)
-        if self.freqs.dtype is not torch.float64:
+        if self.freqs is not before:        # (a captured graph reads them where they are)
             self.freqs = self._make_freqs(self.freqs.device)
         return self
 

@@ -29,3 +29,21 @@ def test_scales_beyond_fp32_in_log2_are_refused():
         a = attn(scale=scale)
         assert lib.rc_cross_attn_fwd_work_bytes(a) == lib.rc_cross_attn_bwd_work_bytes(a) == -1
         assert lib.rc_cross_attn_fwd(a, 16, 16, 16, 16, None, None, 16, None) == -1
+
+
+def test_row_attention_frequencies_survive_empty_storage():
+    """Deferred initialisation: parameters come from a checkpoint, the frequencies do not."""
+    import raft_stereo_amd as R
+    want = R.RowAttentionHip(32, heads=2).freqs.clone()
+    before = torch.are_deterministic_algorithms_enabled()
+    torch.use_deterministic_algorithms(True)       # (fills empty storage with NaN)
+    try:
+        assert torch.equal(R.RowAttentionHip(32, heads=2).to_empty(device="cpu").freqs, want)
+        assert torch.equal(R.RowAttentionHip(32, heads=2).to("meta").to_empty(device="cpu").freqs, want)
+        with torch.device("meta"):
+            m = R.RowAttentionHip(32, heads=2)
+        assert torch.equal(m.to_empty(device="cpu").half().freqs, want) and m.q.weight.device.type == "cpu"
+        ptr = m.freqs.data_ptr()
+        assert m.to("cpu").freqs.data_ptr() == ptr      # nothing to move: a captured graph may read them there
+    finally:
+        torch.use_deterministic_algorithms(before)
