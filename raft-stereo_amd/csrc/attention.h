@@ -440,9 +440,10 @@ template <typename T, int DC, int KT, int WAVES> struct at_key_tiles {
   }
 };
 
-// every load of this wave has landed, and every wave has said so
+// every load of this wave has landed, its reads of LDS are done (the tile that they read may be filled next), and every
+// wave has said so
 __device__ __forceinline__ void at_landed() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
