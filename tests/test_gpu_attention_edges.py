@@ -112,6 +112,45 @@ def test_fp16_keeps_the_tail_of_a_long_row(R, D, Tq):
             assert_within(d[:1], want[name], name)
 
 
+LONG = [  # Tq, Tk, Hq, D and keys of a part: the few-row form and the one of many rows, up to 512 parts of one row
+    ("bf16", 1, 16385, 2, 64, 256), ("f16", 3, 70000, 1, 64, 256), ("bf16", 1, 131067, 2, 64, 256), ("f16", 1, 131067, 1, 128, 256),
+    ("f32", 1, 16385, 2, 64, 64), ("f32", 2, 32760, 1, 64, 64), ("f32", 1, 9000, 2, 256, 64), ("f32", 1, 65500, 1, 32, 128),
+    ("bf16", 40, 65500, 1, 64, 128), ("f32", 40, 32760, 1, 40, 64),
+]
+
+
+@pytest.mark.parametrize("dtype, Tq, Tk, Hq, D, part", LONG)
+@pytest.mark.parametrize("kind", ["none", "lengths", "parts"])
+def test_many_parts_match_the_formula(R, dtype, Tq, Tk, Hq, D, part, kind):
+    """Long rows, with parts (and runs of them) that no key is left in, forward and back."""
+    rng = np.random.default_rng(Tk + len(kind))
+    q, k, v = rand(rng, (1, Tq, Hq, D), dtype, 1.5), rand(rng, (1, Tk, 1, D), dtype), rand(rng, (1, Tk, 1, D), dtype)
+    g = rand(rng, (1, Tq, Hq, D), dtype)
+    lengths = [Tk - 3 * part - 7] if kind == "lengths" else None
+    mask = None
+    if kind == "parts":
+        mask = np.repeat(rng.random((1, Tk // part + 1)) < 0.5, part, axis=1)[:, :Tk] & (rng.random((1, Tk)) < 0.9)
+        mask[:, Tk // 4:Tk // 2] = False
+    want = A.attention(*(host(x) for x in (q, k, v, g)), A.allowed_keys(1, Tk, lengths, mask), dtype=dtype)
+    got = run_attention(R, q, k, v, g, lengths, mask, dtype)
+    for name in ("out", "dq", "dk", "dv"):
+        assert_within(got[name], want[name], name)
+
+
+@pytest.mark.parametrize("dtype, Tq, Tk, Hq, D, part", LONG)
+def test_every_part_counts_once(R, dtype, Tq, Tk, Hq, D, part):
+    """Equal probabilities, and a one in the first and the last place of each part, the parts' ones dealt to the elements in
+    turn: an element sums few parts, so that one lost or doubled is far outside the bound."""
+    q, k, v = torch.zeros(1, Tq, Hq, D), rand(np.random.default_rng(3), (1, Tk, 1, D), dtype).float(), torch.zeros(1, Tk, 1, D)
+    for s in range((Tk + part - 1) // part):
+        for at in (s * part, min(Tk, (s + 1) * part) - 1):
+            v[0, at, 0, s % D] += 1.0
+    q, k, v = (x.to(DT[dtype]) for x in (q, k, v))
+    value, bound = A.attention(host(q), host(k), host(v), None, None, dtype=dtype)["out"]
+    assert (bound[value > 0] < 0.5 / Tk).all()                    # a part brings 1 / Tk at least
+    assert_within(run_attention(R, q, k, v, None, None, None, dtype)["out"], (value, bound), "out")
+
+
 # -------------------------------------------------------------------------------------------------- forward mode
 def test_forward_mode_is_refused(R):
     """There is no forward-mode derivative: a dual operand raises, it does not lose its tangent."""
@@ -149,3 +188,95 @@ def test_padded_batches_in_front_of_the_volume(R, impl):
         assert torch.equal(got, R.make_corr_fn(impl, *m(f1, f2, w1, w2))(coords))
         one = R.make_corr_fn(impl, f1, f2, attention=m, width2=w2)(coords)
         assert torch.equal(one, R.make_corr_fn(impl, *m(f1, f2, None, w2))(coords)) and not torch.equal(one, got)
+
+
+# ------------------------------------------------------------------------------- norm and rotation of many tokens
+def norm_plan(tokens, H, D, most):
+    """The launch that the library makes: heads of a group, chunks of a token, blocks, and the longest fp32 chain of a
+    weight gradient's sum (what a lane goes through, then the block's groups)."""
+    lanes = 1
+    while lanes * 8 < D:
+        lanes *= 2
+    per, hp = 256 // lanes, H
+    while hp > 1 and tokens * -(-H // hp) < 2048 * per:
+        hp = (hp + 1) // 2
+    chunks = -(-H // hp)
+    wanted = -(-tokens * chunks // per)
+    blocks = min(wanted, most)
+    return hp, chunks, blocks, wanted, -(-wanted // blocks) * hp + per
+
+
+MANY = [  # N, Tq, Tk, Hq, Hk, D, rotated, positions, pairs, slices of a wider projection
+    (2, 4100, 4150, 5, 3, 256, 128, "far", False, True),       # several heads a group, the last chunk with fewer
+    (1, 8200, 0, 9, 0, 256, 256, "float", True, False),        # five heads: two loads of four
+    (1, 16500, 700, 3, 4, 200, 64, "shared", False, True),     # all three heads in one group; the other side a small one
+    (3, 470, 0, 5, 0, 256, 64, "far", True, True),             # 512 to 1024 blocks: the weights' sums in two turns
+    (1, 33000, 2100, 2, 6, 128, 128, "index", False, False),
+    (5, 3300, 3301, 6, 7, 72, 16, "far", True, True),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", MANY, ids=lambda s: "x".join(map(str, s[:7])))
+def test_norm_rotate_of_many_tokens_matches_the_formula(R, shape, dtype):
+    N, D = shape[0], shape[5]
+    pos, interleaved, sliced = shape[7:]
+    rng = np.random.default_rng(sum(shape[:7]))
+    freqs, sides = norm_inputs(shape[:7], dtype, rng, pos)
+    eps = 1e-5
+    leaves, xs, ws, ps, plans = [], [], [], [], []
+    for s in sides:
+        if s is None:
+            xs.append(None), ws.append(None), ps.append(None), plans.append(None)
+            continue
+        x, g, w, p = s
+        H = x.shape[2]
+        leaf = x.cuda()
+        if sliced:
+            wide = torch.full((N, x.shape[1], 2 * H + 1, D), 7.0, dtype=x.dtype, device="cuda")
+            wide[:, :, 1:H + 1] = leaf
+            leaf = wide[:, :, 1:H + 1]
+        leaf = leaf.detach().requires_grad_()
+        w = w.to(x.dtype)      # weights in the operands' type
+        s[2].copy_(w)
+        xs.append(leaf), ws.append(w.cuda().requires_grad_()), ps.append(None if p is None else p.cuda())
+        leaves += [leaf, ws[-1]]
+        plans.append(norm_plan(N * x.shape[1], H, D, 1024 if sides[1] is None else 512))
+    # the ways that small calls do not take
+    hp, chunks, blocks, wanted, _ = plans[0]
+    assert blocks > 512 or wanted > blocks
+    assert hp > 1 or wanted > 512
+    out = R.qk_norm_rotate_hip(xs[0], xs[1], ws[0], ws[1], torch.from_numpy(freqs).cuda(), ps[0], ps[1], eps=eps, interleaved=interleaved)
+    outs = (out,) if sides[1] is None else out
+    used = [i for i in (0, 1) if sides[i] is not None]
+    grads = torch.autograd.grad(outs, leaves, [sides[i][1].cuda() for i in used])
+    for j, i in enumerate(used):
+        x, g, w, p = sides[i]
+        want = A.norm_rotate(host(x), host(w), freqs, None if p is None else p.numpy(), eps, interleaved, host(g), dtype, sums=plans[i][4])
+        assert_within(outs[j], want["y"], ("y", i))
+        assert_within(grads[2 * j], want["dx"], ("dx", i))
+        dw, bound = want["dw"]
+        assert grads[2 * j + 1].dtype == x.dtype
+        assert_within(grads[2 * j + 1], (dw, bound + A.HALF_STEP[dtype] * (np.abs(dw) + bound)), ("dw", i))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", MANY, ids=lambda s: "x".join(map(str, s[:6])))
+def test_every_head_counts_once_in_the_weights_gradient(R, shape, dtype):
+    """Heads of ones and minus ones have the norm 1, so the gradients of the weights are sums of small whole numbers, exact
+    in fp32 in any order where r is: a head that is lost or counted twice changes some of them by one or more."""
+    N, Tq, Tk, Hq, Hk, D = shape[:6]
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    xs, gs = [], []
+    for T, H in ((Tq, Hq), (Tk, Hk)):
+        if H:
+            xs.append((torch.randint(0, 2, (N, T, H, D), generator=gen, device="cuda") * 2 - 1).to(DT[dtype]))
+            gs.append((torch.randint(1, 3, (N, T, H, 1), generator=gen, device="cuda") * xs[-1]).to(DT[dtype]))
+    ws = [torch.ones(D, device="cuda", requires_grad=True) for _ in xs]
+    out = R.qk_norm_rotate_hip(xs[0], xs[1] if len(xs) > 1 else None, *ws, eps=0.0)
+    dws = torch.autograd.grad(out, ws, gs)
+    for x, g, dw in zip(xs, gs, dws):
+        want = (x.double() * g.double()).sum(dim=(0, 1, 2))
+        chain = norm_plan(N * x.shape[1], x.shape[2], D, 1024 if len(xs) == 1 else 512)[4]
+        # r may be off by 2 * 2^-24 (the mean's rounding, the root's), and the sums are rounded then
+        assert (dw.double() - want).abs().max() <= (3 + chain) * 2.0 ** -24 * want.max() < 0.5
