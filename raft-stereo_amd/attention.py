@@ -69,6 +69,11 @@ def _heads_view(t):
     return t, st
 
 
+def _unit_stride(t):
+    """Positions or a mask, None or with the tokens side by side."""
+    return t if t is None or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
 def _dense(t):
     """`t` contiguous and on a 16-byte boundary."""
     t = t.contiguous()
@@ -98,7 +103,7 @@ def _check_pos(pos, x, what):
     N, T = x.shape[:2]
     if tuple(pos.shape) not in ((T,), (N, T)):
         raise ValueError(f"{what} must be [{T}] or [{N}, {T}], got {tuple(pos.shape)}")
-    return pos.contiguous() if T > 1 and pos.stride(-1) != 1 else pos
+    return _unit_stride(pos)
 
 
 def _heads_desc(x, st, weight, pos):
@@ -141,8 +146,8 @@ def _norm_rotate_raw(q, k, desc_q, desc_k, tail):
 
 
 class _NormRotateFn(torch.autograd.Function):
-    """Keeps its inputs for the backward pass, which works the norm out again.  (They are described again there: a hook
-    on saved tensors may have moved them.)"""
+    """Keeps its inputs for the backward pass, which works the norm out again.  (They are laid out and described again
+    there: a hook on saved tensors may have moved them.)"""
 
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, freqs, q_pos, k_pos, rest):
@@ -157,6 +162,8 @@ class _NormRotateFn(torch.autograd.Function):
         if gq is None and gk is None:
             return (None,) * 8
         q, k, qw, kw, freqs, q_pos, k_pos = ctx.saved_tensors
+        qw, kw, freqs = (None if t is None else t.contiguous() for t in (qw, kw, freqs))
+        q_pos, k_pos = _unit_stride(q_pos), _unit_stride(k_pos)      # (by name: they have to outlive the call)
         q, k, desc_q, desc_k, tail = _norm_rotate_desc(q, k, qw, kw, freqs, q_pos, k_pos, ctx.rest)
         dev, D = q.device, q.shape[3]
         want = ctx.needs_input_grad
@@ -272,7 +279,8 @@ def _attention_raw(a, q, k, v, train):
 
 class _CrossAttentionFn(torch.autograd.Function):
     """Keeps the operands, the result (16-bit: with what rounding took from it) and each row's log-sum-exp; the backward
-    pass works the scores out again.  (The operands are described again there: a hook on saved tensors may have moved them.)"""
+    pass works the scores out again.  (All of them are laid out and described again there: a hook on saved tensors may have
+    moved them.)"""
 
     @staticmethod
     def forward(ctx, q, k, v, key_mask, key_lengths, scale):
@@ -285,6 +293,8 @@ class _CrossAttentionFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_out):
         q, k, v, out, rest, lse, key_mask, key_lengths = ctx.saved_tensors
+        out, lse, rest = _dense(out), _dense(lse), None if rest is None else _dense(rest)
+        key_mask, key_lengths = _unit_stride(key_mask), None if key_lengths is None else key_lengths.contiguous()
         a, q, k, v = _attn_desc(q, k, v, key_mask, key_lengths, ctx.scale)
         dev = q.device
         g = _dense(grad_out)
@@ -329,8 +339,7 @@ def cross_attention_hip(q, k, v, key_mask=None, key_lengths=None, scale=None):
             raise ValueError(f"key_mask must be [{N}, {Tk}], got {tuple(key_mask.shape)}")
         if key_mask.device != q.device:
             raise RuntimeError("key_mask lives on a different device than q")
-        if Tk > 1 and key_mask.stride(1) != 1:
-            key_mask = key_mask.contiguous()
+        key_mask = _unit_stride(key_mask)
     if key_lengths is not None:
         if key_lengths.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"key_lengths must be int32 or int64, got {key_lengths.dtype}")

@@ -280,3 +280,63 @@ def test_every_head_counts_once_in_the_weights_gradient(R, shape, dtype):
         chain = norm_plan(N * x.shape[1], x.shape[2], D, 1024 if len(xs) == 1 else 512)[4]
         # r may be off by 2 * 2^-24 (the mean's rounding, the root's), and the sums are rounded then
         assert (dw.double() - want).abs().max() <= (3 + chain) * 2.0 ** -24 * want.max() < 0.5
+
+
+# ------------------------------------------------------------------------------------------- saved tensors and graphs
+def test_saved_tensors_come_back_with_other_strides(R):
+    """A hook may hand saved tensors back in another layout and off 16-byte boundaries: the values count."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    mk = lambda *s: torch.randn(s, generator=gen, device="cuda")
+    q, k, v, go, w = mk(2, 40, 4, 64), mk(2, 50, 2, 64), mk(2, 50, 2, 64), mk(2, 40, 4, 64), 1 + 0.1 * mk(64)
+    mask, lengths = torch.rand(2, 50, generator=gen, device="cuda") < 0.7, torch.tensor([50, 30], device="cuda")
+    freqs, pos = torch.linspace(0.01, 1.0, 32, device="cuda"), torch.randint(0, 900, (2, 40), generator=gen, device="cuda")
+
+    def turned(t):
+        """The same values, the first dimension the fastest, from an odd place on."""
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:]
+        back = flat.view(tuple(t.shape[1:]) + (t.shape[0],)).movedim(-1, 0) if t.dim() > 1 else \
+            torch.empty(2 * t.numel() + 1, dtype=t.dtype, device=t.device)[1::2]
+        return back.copy_(t)
+
+    def grads(dtype, unpack):
+        leaves = [x.to(dtype).requires_grad_() for x in (q, k, v)] + [w.clone().requires_grad_()]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            a, b = R.qk_norm_rotate_hip(leaves[0], leaves[1], leaves[3], leaves[3], freqs, pos)
+            out = R.cross_attention_hip(a, b, leaves[2], key_mask=mask, key_lengths=lengths)
+        return torch.autograd.grad(out, leaves, go.to(dtype))
+    for dtype in (torch.float32, torch.float16):
+        for a, b in zip(grads(dtype, lambda t: t), grads(dtype, lambda t: turned(t.detach()))):
+            assert torch.equal(a, b)
+
+
+def test_row_attention_with_widths_in_a_graph(R):
+    """Forward and gradients of padded batches, captured and replayed with other widths."""
+    torch.manual_seed(4)
+    m = R.RowAttentionHip(32, heads=2).cuda()
+    f = [torch.randn(2, 32, 3, 40, device="cuda") for _ in range(2)]
+    w = [torch.tensor([40, 17], device="cuda"), torch.tensor([25, 40], device="cuda")]
+    go = [torch.randn_like(x) for x in f]
+
+    def step():
+        t = [x.detach().requires_grad_() for x in f]
+        params = [p.detach().requires_grad_() for p in m.parameters()]
+        out = torch.func.functional_call(m, dict(zip((n for n, _ in m.named_parameters()), params)), (*t, *w))
+        return tuple(o.detach() for o in out) + torch.autograd.grad(out, t + params, go)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        step()
+    torch.cuda.current_stream().wait_stream(st)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        outs = step()
+    for r in range(4):
+        for x in f:
+            x.copy_(torch.randn_like(x))
+        w[0].copy_(torch.tensor([40 - r, 3 * r])), w[1].copy_(torch.tensor([7 * r, 40]))
+        want = step()
+        gr.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
