@@ -6,7 +6,8 @@
 // Two kernels, each of which owns what it adds up, so there are no atomics and every run gives the same bits; the price
 // is that S and dO V^T are worked out twice (7 products instead of 5).
 //   at_dq_kernel   a wave has 32 query rows and goes through the keys: S^T = K Q^T and dP^T = V dO^T leave a query in
-//                  each lane, dS^T is the right operand of dQ^T = K^T dS^T as it stands.  It also works out delta.
+//                  each lane, dS^T is the right operand of dQ^T = K^T dS^T as it stands.  It also works out delta (and that
+//                  alone where dq is not wanted).
 //   at_dkv_kernel  a wave has 32 keys and goes through the query rows of all heads that share them: S = Q K^T and
 //                  dP = dO V^T leave a key in each lane; dV^T = dO^T P, dK^T = Q^T dS.
 //
@@ -57,7 +58,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void at_dq_kernel(const T* __restrict
 
   const int len = at_length(a, n);
   const int k_begin = split * sp.per, k_end = min(len, k_begin + sp.per);
-  const int tiles = k_end > k_begin ? (k_end - k_begin + KT - 1) / KT : 0;
+  // (without dq only delta is wanted: no keys)
+  const int tiles = dq != nullptr && k_end > k_begin ? (k_end - k_begin + KT - 1) / KT : 0;
   at_key_tiles<T, DC, KT, NW> kv;
   kv.init(a, k, v, n, hk, k_begin, k_end, wave, lane);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(at_lds)smem;
@@ -425,7 +427,7 @@ template <typename T, int DC> int at_bwd(const at_bwd_call& c) {
     constexpr auto kernel = at_dq_kernel<T, DC, 4, NB, OCC>;
     if ((rc = at_allow_lds<kernel>(bytes))) return rc;
     at_parts sp = {};
-    sp.n = c.p.q_splits;
+    sp.n = c.dq ? c.p.q_splits : 1;
     sp.per = c.p.q_per;
     sp.p = c.parts;
     sp.part = c.a->N * c.a->Tq * c.a->Hq * c.a->D;

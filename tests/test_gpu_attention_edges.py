@@ -340,3 +340,21 @@ def test_row_attention_with_widths_in_a_graph(R):
         torch.cuda.synchronize()
         for a, b in zip(outs, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(130, 37, 100, 4, 2, 64), (300, 20, 50, 1, 1, 32), (1, 70, 1500, 2, 1, 96), (2, 150, 700, 2, 2, 128), (1, 600, 90, 2, 1, 256)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_gradients_of_some_operands(R, shape, dtype):
+    """What is not wanted changes nothing about what is."""
+    N, Tq, Tk, Hq, Hk, D = shape
+    rng = np.random.default_rng(8)
+    x = [rand(rng, s, dtype) for s in ((N, Tq, Hq, D), (N, Tk, Hk, D), (N, Tk, Hk, D))]
+    g, mask = rand(rng, (N, Tq, Hq, D), dtype), rng.random((N, Tk)) < 0.8
+    want = A.attention(*(host(t) for t in x), host(g), A.allowed_keys(N, Tk, None, mask), dtype=dtype)
+    for which in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1), (1, 0, 1)):
+        t = [a.cuda().requires_grad_(bool(w)) for a, w in zip(x, which)]
+        out = R.cross_attention_hip(*t, key_mask=torch.from_numpy(mask).cuda())
+        got = torch.autograd.grad(out, [a for a, w in zip(t, which) if w], g.cuda())
+        for name, d in zip([n for n, w in zip(("dq", "dk", "dv"), which) if w], got):
+            assert_within(d, want[name], (name, which))
