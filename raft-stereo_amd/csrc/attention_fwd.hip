@@ -457,17 +457,37 @@ at_plan at_make_plan(const rc_attn* a) {
   p.tile_rows = p.few ? 32 : 128;
   p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   p.items = a->N * a->Hk * p.row_tiles;
-  // Fewer work items than fill the card twice: the keys are divided too, down to 256 of them, or 128 where there are
-  // rows enough (3 x 1157 x 1102, 8/4 heads of 96 in fp16: 53 us with 256, 49 with 128; one token over 3426 keys, 4 heads
-  // of 192: 22 and 27); in fp32, whose products take sixteen times as long, down to 64 (128 for narrow heads, where that
-  // is the tile; 4 x 1124 keys, 4/2 heads of 256: 38 us, 90 with 256).  (One token in each of 16
-  // sequences, 8192 ragged keys, 32/8 heads of 128: 84 us; one over 16384 keys, 8/1 heads: 19 us, in splits of 1024 keys
-  // 29.)  Up to four such parts few rows stay whole: joining is a launch more (1000 keys in bf16: 14.7
-  // against 18.9 us a call); fp32 heads beyond 128, which one wave goes through alone, up to one.
-  const int64_t unit = a->dtype != RC_F32 ? (p.few ? 256 : 128) : a->D > 32 ? 64 : 128;
+  // Fewer work items than fill the card twice: the keys are divided too, into as many parts as it has room for (one more
+  // is a second turn: 33 x 1 x 1100, 8/8 heads of 128 in bf16, 264 items: 39 us, in two parts each 58).  A part has 256 keys
+  // at least, or 128 where there are rows enough (one token over 3426 keys, 4 heads of 192: 22 us, with 128 27); in fp32,
+  // whose products take sixteen times as long, 64 (128 for narrow heads, where that is the tile; 4 x 1124 keys, 4/2 heads
+  // of 256: 38 us, 90 with 256).  (One token in each of 16 sequences, 8192 ragged keys, 32/8 heads of 128: 84 us; one over
+  // 16384 keys, 8/1 heads: 19 us, in splits of 1024 keys 29.)
+  const bool f32 = a->dtype == RC_F32;
+  const int64_t unit = !f32 ? (p.few ? 256 : 128) : a->D > 32 ? 64 : 128;
+  // (many rows of narrow 16-bit heads: three workgroups a CU; 300 items of 100 rows and 4000 keys, heads of 64: 90 us, 102
+  // undivided; 64 such items, in eight parts: 26, in twelve 31)
+  const int64_t places = !f32 && !p.few && a->D <= 64 && p.items > 128 ? 768 : 512;
   int64_t n = 1;
-  if (p.items > 0 && p.items < 512 && !(p.few && a->Tk <= (a->dtype == RC_F32 && a->D > 128 ? 1 : 4) * unit)) {
-    n = (512 + p.items - 1) / p.items;
+  if (p.items > 0 && p.items < 512) {
+    n = places / p.items;
+    // (fp32 keeps the matrix pipe busy with one workgroup a CU: the second turn is half as long; 3 x 1000 x 2000, 16/16 heads
+    // of 64: 246 us, 285 undivided)
+    if (n == 1 && f32) n = 2;
+    // Joining is a launch more, and the parts of many rows are many bytes.  Up to so many keys an item goes through all of
+    // them.  Few rows: 4 units (1000 keys in bf16: 14.7 against 18.9 us a call); fp32 heads beyond 128, which one wave goes
+    // through alone, one.  Many rows, by the number of items (us, undivided and divided; heads of 64, 128 and 256 in 16
+    // bits): 64 items of 300 keys 13, 13, 24 and 18, 19, 25; of 1000 20, 28, 61 and 18, 23, 38; 130 items of 1000 keys 21,
+    // 28, 75 and 23, 31, 58; 256 items of 1000 keys 22, 36, 85 and 31, 47, 85, of 4000 92, 130, 293 and 75, 120, 225.  fp32,
+    // heads of 128: 40 items of 200 keys 37 and 25; heads of 64: 64 items of 300 keys 27 and 23, 130 items 28 and 34, of 1000 keys 80 and 67; 256 items of 1000 keys 88
+    // and 92, 300 items 146 and 130.
+    int64_t alone = (f32 && a->D > 128 ? 1 : 4) * unit;
+    if (!p.few) {
+      if (f32) alone = p.items <= 64 && a->D > 64 ? 128 : p.items <= 170 ? 256 : p.items <= 256 ? 1024 : 768;
+      else if (a->D > 128) alone = p.items <= 170 ? 512 : 1024;
+      else alone = p.items <= 64 ? 512 : p.items <= 170 ? 1024 : 2048;
+    }
+    if (a->Tk <= alone) n = 1;
     const int64_t most = (a->Tk + unit - 1) / unit;
     n = n < most ? n : most;
     n = n < AT_MOST_SPLITS ? n : AT_MOST_SPLITS;

@@ -47,3 +47,20 @@ def test_row_attention_frequencies_survive_empty_storage():
         assert m.to("cpu").freqs.data_ptr() == ptr      # nothing to move: a captured graph may read them there
     finally:
         torch.use_deterministic_algorithms(before)
+
+
+@pytest.mark.parametrize("dtype, N, Tq, Tk, Hq, Hk, D, divided", [
+    # as many items as the card has room for, or too few keys for what joining them costs
+    ("f32", 96, 128, 117, 4, 4, 64, False), ("f16", 96, 312, 312, 1, 1, 256, False), ("bf16", 300, 100, 300, 1, 1, 64, False),
+    ("f16", 3, 1157, 1102, 8, 4, 96, False), ("bf16", 33, 1, 1100, 8, 8, 128, False), ("bf16", 4, 1, 1000, 8, 8, 64, False),
+    ("f32", 256, 100, 300, 1, 1, 64, False),
+    # few items and many keys
+    ("bf16", 1, 1, 16384, 8, 1, 128, True), ("f32", 4, 1, 1124, 4, 2, 256, True), ("f16", 1, 4096, 4096, 4, 4, 128, True),
+    ("bf16", 20, 100, 1000, 1, 1, 128, True), ("f32", 64, 100, 300, 1, 1, 64, True), ("bf16", 16, 1, 8192, 32, 8, 128, True),
+    ("f32", 3, 1000, 2000, 16, 16, 64, True)])
+def test_keys_are_divided_where_it_pays(dtype, N, Tq, Tk, Hq, Hk, D, divided):
+    """Scratch without a mask is the parts of divided keys."""
+    from raft_stereo_amd import _lib
+    from test_cpu_attention import attn
+    a = attn(N=N, Tq=Tq, Tk=Tk, Hq=Hq, Hk=Hk, D=D, dtype={"f32": _lib.RC_F32, "f16": _lib.RC_F16, "bf16": _lib.RC_BF16}[dtype])
+    assert (_lib.lib.rc_cross_attn_fwd_work_bytes(a) > 0) == divided
