@@ -492,7 +492,8 @@ int rc_qk_norm_rotate_bwd(const rc_heads* q, const rc_heads* k, const void* gq, 
  * Hq query heads in groups of Hq / Hk that share a key and value head (head h reads key head h / (Hq / Hk)).  A key
  * is allowed if its index is below key_lengths[n] (NULL: all; lengths beyond Tk count as Tk, negative ones as 0) and
  * its byte of key_mask is not 0 (NULL: all).  What keys and values hold in places that are not allowed has no
- * influence, infinities and NaN included.  A sequence without an allowed key gives O = 0 and zero gradients.
+ * influence, infinities and NaN included.  A sequence without an allowed key gives O = 0 and zero gradients; a row whose
+ * allowed keys all score -inf gives NaN.  Lengths save the work of the keys behind them; a mask does not.
  * Scores, softmax statistics and sums are fp32.
  */
 typedef struct rc_attn {
@@ -508,9 +509,9 @@ typedef struct rc_attn {
 
 /* out [N, Tq, Hq, D].  For the backward pass, NULL in inference: lse float [N, Hq, Tq], the log-sum-exp of each row's
  * scores in base 2 (scores times log2 e; +inf for a row without a key), and out_rest, of out's shape and type (16-bit
- * types; may be NULL): what rounding took from out.  work: rc_cross_attn_fwd_work_bytes()
- * of scratch (0 in most cases: only a few query rows over many keys are split over workgroups); negative: *a is
- * invalid. */
+ * types; may be NULL): what rounding took from out.  work: rc_cross_attn_fwd_work_bytes() of scratch (a mask takes one
+ * bit a key; where there are fewer work items than the card has room for and keys enough, the keys are divided over
+ * workgroups, whose parts take 4 (D + 2) bytes a row each; 0 otherwise); negative: *a is invalid. */
 int64_t rc_cross_attn_fwd_work_bytes(const rc_attn* a);
 int rc_cross_attn_fwd(const rc_attn* a, const void* q, const void* k, const void* v, void* out,
                       void* out_rest, float* lse, void* work, void* stream);

@@ -277,8 +277,12 @@ template <typename T, int DC> struct at_places {
   }
 };
 
-// acc[db] += (32 rows of the tile from `row`)^T x, for all columns of the head: x is a result of 32 rows by 32 columns
-// (16-bit types: rounded to T).
+// acc[db] += (32 rows of the tile from `row`)^T x, for all columns of the head: x is a result of 32 rows by 32 columns.
+// In 16-bit types x (probabilities, or scores' gradients) is rounded to T, as the matrix instructions multiply nothing wider
+// by T: of independent roundings a sum keeps about the relative error of one, so that with the result's own the outputs are
+// 1.4 times as far from 64 bits as fp32 throughout (bf16: 0.0024 and 0.0017, fp16: 0.00030 and 0.00021), dq and dk up to 1.6
+// times where their sums cancel.  A second product with what rounding takes brings dq and dk back to 1.0 and costs a training
+// step of 2 x 2048 x 4096, 16/4 heads of 128, 15 % (629 -> 724 us on one card), 768 x 312 x 312, 4 heads of 64, 9 %.
 template <typename T, int DC>
 __device__ __forceinline__ void at_mma_cols(const at_places<T, DC>& at, const unsigned char* tile, int row, const at_f16& x,
                                             at_f16* acc) {

@@ -11,11 +11,13 @@
 //   at_dkv_kernel  a wave has 32 keys and goes through the query rows of all heads that share them: S = Q K^T and
 //                  dP = dO V^T leave a key in each lane; dV^T = dO^T P, dK^T = Q^T dS.
 //
-// Both are bound by the matrix pipe and what has to feed it: each product's left operand comes from LDS, once for every 32
-// queries or keys of a wave (with 64, the sums alone would take all registers).  2 x 2048 x 4096 ragged keys, 16/4 heads
-// of 128, bf16: 195 us (dq, matrix pipe busy 41 %) and 274 us (dk and dv, 37 %), 860 and 810 TFLOP/s of the products that
-// they work out; with the forward's 144 us 580 us a training step.  16-bit heads of 96 and 128: two waves share 32 keys,
-// with the values in LDS, so that four waves run on a SIMD instead of two (650 -> 615 us).
+// Bound by latency: a wave's blocks of scores go through product, exponential, product, difference and product one after
+// the other, with two or four waves a SIMD, and no unit is full.  2 x 2048 x 4096 ragged keys, 16/4 heads of 128, bf16
+// (medians of 300 launches): 189 us (dq; matrix pipe busy 40 %, vector pipe 29 %, LDS 20 %) and 254 us (dk and dv; 37 %,
+// 25 %, 28 %), 890 and 880 TFLOP/s of the products that they work out; with the forward's 139 us 574 us a training step.
+// Each product's left operand comes from LDS, once for every 32 queries or keys of a wave (with 64, the sums alone would
+// take all registers).  16-bit heads of 96 and 128: two waves share 32 keys, with the values in LDS, so that four waves run
+// on a SIMD instead of two (650 -> 615 us).
 #include "attention.h"
 
 #include <initializer_list>

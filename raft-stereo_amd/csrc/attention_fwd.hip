@@ -8,12 +8,15 @@
 // registers (maximum and sum need one exchange between the wave's halves), and is, exponentiated and rounded, the right
 // operand of O^T = V^T P^T as it stands -- probabilities never touch LDS.
 //
-// What bounds it, and what it reaches (the library's large bf16 product: 1217 TFLOP/s, a large copy 4.8 TB/s):
+// What bounds it, and what it reaches (kernel times, medians of 300 launches; the library's large bf16 product: 1217 TFLOP/s,
+// a large copy 4.8 TB/s):
 //   many rows, wide heads: the matrix and the vector pipe together; 8 x 2047 x 4095, 16/4 heads of 128, bf16, a mask with
-//     holes: 569 us, 965 TFLOP/s; the matrix pipe is busy 45 % of the time, the vector pipe 37 %
-//   rows of an image: latency, as a sequence is only a few tiles long; 768 x 312 x 312, a head of 256, fp16: 155 us,
-//     3.2 TB/s and 490 TFLOP/s (matrix pipe 21 %); 640 x 180 x 180, 8 heads of 32, bf16: 74 us, 3.2 TB/s, 290 TFLOP/s
-//   few rows: memory; 16 x 1 x 8192 ragged keys, 32/8 heads of 128, bf16: 82 us with the join's 4.5, 4.1 TB/s
+//     holes: 575 us, 957 TFLOP/s; the matrix pipe is busy 45 % of the time, the vector pipe 44 %
+//   rows of an image: latency, as a sequence is only a few tiles long; 768 x 312 x 312, a head of 256, fp16: 159 us,
+//     3.1 TB/s and 480 TFLOP/s (matrix pipe 21 %, vector pipe 22 %, LDS 10 %); 640 x 180 x 180, 8 heads of 32, bf16, with
+//     what the backward pass needs: 78 us, 3.8 TB/s, 270 TFLOP/s
+//   few rows: memory; 16 x 1 x 8192 ragged keys, 32/8 heads of 128, bf16: 75 us, 4.5 TB/s, and 4.8 of join
+//   a token over 1000 keys: one workgroup a head goes through its eight tiles, 11 us
 #include "attention.h"
 
 #include <initializer_list>
@@ -328,7 +331,7 @@ __global__ __launch_bounds__(64 * NWQ * NWK, OCC) void at_fwd_kernel(const T* __
 
 // Joins the splits: a wave per row, or four.  The lanes take a split's maximum and sum each, the weights exp2(m_i - max) go to LDS;
 // then a group of D / 4 lanes takes four elements each of every (64 / group)th split, many loads in flight.
-// Bound by latency: 512 rows of 128 in 4 splits take 4.5 us.
+// Bound by latency: 512 rows of 128 in 4 splits take 4.8 us.
 constexpr int AT_MOST_SPLITS = 512;
 
 template <typename T, int WAVES>
@@ -403,7 +406,9 @@ __global__ __launch_bounds__(256) void at_join_kernel(T* __restrict__ out, T* __
   if (lse != nullptr && lane == 0) lse[((int64_t)n * a.Hq + hq) * a.Tq + t] = none ? INFINITY : top + __builtin_amdgcn_logf(l);
 }
 
-// The mask as one bit per key: a scalar load tells a tile what it may skip.  8 x 4095 keys: 4.6 us, most of it the launch.
+// The mask as one bit per key: a scalar load tells a tile which keys take part.  (Nothing is skipped for it in this pass or
+// for dq: tiles go by the lengths, and one whose keys are all masked is multiplied with zeros.  Only the kernel of dk and dv
+// leaves out keys of which a whole workgroup has none.)  8 x 4095 keys: 4.8 us, most of it the launch.
 __global__ __launch_bounds__(256) void at_bits_kernel(const unsigned char* __restrict__ mask, int64_t stride,
                                                       uint64_t* __restrict__ bits, int64_t words, int Tk, int64_t total) {
   const int64_t w = (int64_t)at_block() * 4 + (threadIdx.x >> 6);  // a wave per word

@@ -10,9 +10,11 @@
 // once, and S and dP are worked out once (the two kernels for long sequences read the operands twice and multiply 7
 // products instead of 5).
 //
-// 640 x 180 x 180, 8 heads of 32, bf16: 185 us, 2.2 TB/s (the two kernels: 225); the matrix pipe is busy 14 % of the time
-// and LDS 40 %: the waves of a workgroup wait for each other at each 32 query rows, and two or three workgroups on a CU
-// fill each other's gaps.  96 x 128 x 117, 4 heads of 64, fp32: 84 us, matrix pipe 29 %.
+// 640 x 180 x 180, 8 heads of 32, bf16: 177 us (median of 300 launches), 2.3 TB/s of operands and gradients (in a call 227
+// instead of 267 with the two kernels, when it was measured); the matrix pipe is busy 14 % of the time, the vector pipe and
+// LDS 39 %, nearly half of LDS in bank conflicts of the 64-byte rows: the waves of a workgroup wait for each other at each 32
+// query rows, and two or three workgroups on a CU fill each other's gaps.  96 x 128 x 117, 4 heads of 64, fp32: 81 us, matrix
+// pipe 29 %: 384 workgroups of 135 KB of LDS, one to a CU, are one turn and half of another.
 #include "attention.h"
 
 namespace {

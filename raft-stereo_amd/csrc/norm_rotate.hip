@@ -12,10 +12,11 @@
 // heads of the token that the group goes through.  Lanes of 8 elements rather than 16 bytes each: one form for all
 // types, and 8-byte loads of neighbouring lanes fill their cache lines together.
 //
-// Measured (a large copy reaches 4.8 TB/s; what the 256 MiB cache still holds comes faster): forward, 768 x 312 fp16
-// queries and keys, 4 heads of 64 each: 107 us, 4.6 TB/s.  640 x 180 fp32, 8 and 8 heads of 32: forward 85 us, 5.5 TB/s,
-// backward 141 us, 5.0 TB/s.  8 x 2047 and 4095 bf16, 16 and 4 heads of 128: 48 us, 4.2 TB/s, and 68 us, 4.4 TB/s, and
-// 6 us for the sum of the weights' gradients.  One token in 16 sequences, 32 heads of 128: 5.4 us, in 12.5 of the call.
+// Measured (kernels, medians of 300 launches; a large copy reaches 4.8 TB/s; what the 256 MiB cache still holds comes
+// faster): forward, 768 x 312 fp16 queries and keys, 4 heads of 64 each: 110 us, 4.5 TB/s.  640 x 180 fp32, 8 and 8 heads of
+// 32: forward 88 us, 5.3 TB/s, backward 141 us, 5.0 TB/s.  8 x 2047 and 4095 bf16, 16 and 4 heads of 128: 47 us, 4.3 TB/s,
+// and 67 us, 4.5 TB/s, and 6 us for the sum of the weights' gradients.  One token in 16 sequences, 32 heads of 128: 5.4 us,
+// in 12.8 of the call.
 #include "rc_common.h"
 
 #include <math.h>
