@@ -319,9 +319,9 @@ def cross_attention_hip(q, k, v, key_mask=None, key_lengths=None, scale=None):
     `key_lengths[n]` (int32 or int64 `[N]`; beyond Tk counts as Tk, negative as 0) and `key_mask[n, t]` is True (bool
     `[N, Tk]`); what the others hold, infinities and NaN included, has no influence.  A sequence without any key gives
     zeros, and zero gradients; a row whose keys all score -inf gives NaN.  Lengths save the work of the keys behind them,
-    a mask does not: padding is better given as lengths.  Scores, the softmax's maximum and sum, and all products' sums are fp32; 16-bit operands
-    have their probabilities (and in the backward pass their scores' gradients) rounded to 16 bits for the second
-    product.  Returns `[N, Tq, Hq, D]` contiguous.  Differentiable w.r.t. q, k and v, once, in reverse mode (dual tensors
+    a mask does not: padding is better given as lengths.  Scores, the softmax's maximum and sum, and all products' sums
+    are fp32; 16-bit operands have their probabilities (and in the backward pass their scores' gradients) rounded to 16
+    bits for the second product.  Returns `[N, Tq, Hq, D]` contiguous.  Differentiable w.r.t. q, k and v, once, in reverse mode (dual tensors
     are refused); the same bits on every run."""
     for t, what in ((q, "q"), (k, "k"), (v, "v")):
         _check_heads(t, what)

@@ -484,8 +484,8 @@ at_plan at_make_plan(const rc_attn* a) {
     // through alone, one.  Many rows, by the number of items (us, undivided and divided; heads of 64, 128 and 256 in 16
     // bits): 64 items of 300 keys 13, 13, 24 and 18, 19, 25; of 1000 20, 28, 61 and 18, 23, 38; 130 items of 1000 keys 21,
     // 28, 75 and 23, 31, 58; 256 items of 1000 keys 22, 36, 85 and 31, 47, 85, of 4000 92, 130, 293 and 75, 120, 225.  fp32,
-    // heads of 128: 40 items of 200 keys 37 and 25; heads of 64: 64 items of 300 keys 27 and 23, 130 items 28 and 34, of 1000 keys 80 and 67; 256 items of 1000 keys 88
-    // and 92, 300 items 146 and 130.
+    // heads of 128: 40 items of 200 keys 37 and 25; heads of 64: 64 items of 300 keys 27 and 23, 130 items 28 and 34, of
+    // 1000 keys 80 and 67; 256 items of 1000 keys 88 and 92, 300 items 146 and 130.
     int64_t alone = (f32 && a->D > 128 ? 1 : 4) * unit;
     if (!p.few) {
       if (f32) alone = p.items <= 64 && a->D > 64 ? 128 : p.items <= 170 ? 256 : p.items <= 256 ? 1024 : 768;
